@@ -24,6 +24,7 @@ CL_LAUNCH_OUTPUTS_FREE = 4
 
 CL_DTYPE_F16 = 0
 CL_DTYPE_F32 = 1
+CL_DTYPE_BF16 = 2
 
 CL_VARIANTS_NORMAL = 0
 CL_VARIANTS_ALL = 1
@@ -39,6 +40,34 @@ _cs = ctypes.c_char_p
 _int = ctypes.c_int
 _size = ctypes.c_size_t
 _dp = ctypes.POINTER(ctypes.c_double)
+
+
+def _fields(names: str, ctype) -> list:
+    return [(n, ctype) for n in names.split()]
+
+
+class QkNormRopeDesc(ctypes.Structure):
+    """cl_qknorm_rope_desc"""
+    _fields_ = (_fields("tokens table_rows q_token q_head k_token k_head q_out_token q_out_head "
+                        "k_out_token k_out_head", _i64)
+                + _fields("q_heads kv_heads head_dim rotary interleaved positions64 dtype",
+                          ctypes.c_int32)
+                + [("eps", ctypes.c_float)])
+
+
+class KvCacheDesc(ctypes.Structure):
+    """cl_kvcache_desc"""
+    _fields_ = (_fields("tokens num_pages k_token k_head v_token v_head", _i64)
+                + _fields("kv_heads head_dim bits page_size dtype", ctypes.c_int32))
+
+
+class KvAttentionDesc(ctypes.Structure):
+    """cl_kvattention_desc"""
+    _fields_ = (_fields("num_pages table_stride q_batch q_new q_head", _i64)
+                + _fields("batch new_tokens q_heads kv_heads head_dim bits page_size max_pages "
+                          "window dtype prefix_length prefix_page_count", ctypes.c_int32)
+                + [("scale", ctypes.c_float)])
+
 
 # name -> (restype, argtypes); every symbol declared in the public header.
 PROTOTYPES = {
@@ -77,6 +106,11 @@ PROTOTYPES = {
     "cl_rmsnorm_f16": (_int, [_vp, _vp, ctypes.c_float, _vp, _i64, _i64, _vp, _u32]),
     "cl_int4gemv_rmsnorm": (_int, [_cs, _vp, _vp, _vp, _vp, ctypes.c_float, _vp, _i64, _i64,
                                    _i64, _vp, _u32]),
+    "cl_qknorm_rope": (_int, [_vp] * 8 + [ctypes.POINTER(QkNormRopeDesc), _vp]),
+    "cl_kvcache_write": (_int, [_vp] * 4 + [ctypes.POINTER(KvCacheDesc), _vp]),
+    "cl_kvcache_read": (_int, [_vp] * 4 + [ctypes.POINTER(KvCacheDesc), _vp]),
+    "cl_kvattention_workspace": (_int, [ctypes.POINTER(_size)]),
+    "cl_kvattention": (_int, [_vp] * 10 + [ctypes.POINTER(KvAttentionDesc), _vp]),
 }
 
 CL_MAX_PEERS = 8

@@ -36,7 +36,8 @@ ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 # kernels in parallel on every host core (the kernel unit holds dozens of
 # template instantiations)
 NVCC_FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "--split-compile", "0"]
-SOURCES = ["gemv_kernels.cu", "gemv_dense.cu", "quantize.cu", "capi.cu"]
+SOURCES = ["gemv_kernels.cu", "gemv_dense.cu", "quantize.cu", "qknorm_rope.cu", "kv_cache.cu",
+           "kv_attention.cu", "capi.cu"]
 
 
 def _nvcc() -> str:
@@ -159,7 +160,7 @@ def build_binding(force: bool = False) -> Path:
 
 def build(op: str = "int4gemv", force: bool = False, verbose: bool = False):
     """Return the extension object of operator `op` ("int4gemv" | "qgemv" | "gemv" |
-    "rmsnorm")."""
+    "rmsnorm" | "qknorm_rope" | "kvcache" | "kvattention")."""
     build_library(force=force, verbose=verbose)
     build_binding(force=force)
     from .ext import get_ext

@@ -19,6 +19,7 @@
 #include "../../include/cudalab_gemv.h"
 #include "gemv_launch.h"
 #include "gemv_quantize.h"
+#include "kv_layout.cuh"
 
 namespace {
 
@@ -316,8 +317,18 @@ const char* cl_last_error(void) { return g_last_error.c_str(); }
 
 int cl_device_status(int clear, int* status_out) {
     if (!status_out) return fail(CL_ERR_INVALID_ARGUMENT, "status_out is null");
-    cudaError_t e = clb::read_device_status(clear, status_out);
-    if (e != cudaSuccess) return cuda_fail(e, "read device status");
+    // one word per translation unit with a status; the first nonzero one is reported
+    cudaError_t (*const words[])(int, int*) = {clb::read_device_status,
+                                               clb::read_kv_attention_status, clb::read_kv_status,
+                                               clb::read_qknorm_rope_status};
+    int status = 0;
+    for (auto read : words) {
+        int v = 0;
+        cudaError_t e = read(clear, &v);
+        if (e != cudaSuccess) return cuda_fail(e, "read device status");
+        if (status == 0) status = v;
+    }
+    *status_out = status;
     return CL_OK;
 }
 
@@ -607,6 +618,221 @@ int cl_qgemv_sharded(const char* variant, const int8_t* W_shard, const float* sc
     const clb::ShardedVariantDesc* t = clb::int8_sharded_variants(&n);
     return run_sharded(t, n, "qgemv", variant, W_shard, scale_shard, x, M, y_peers, flag_peers,
                        rank, world, row0, N_shard, N_total, K, stream, flags, false);
+}
+
+// ---- attention of a decode step over a quantised paged cache ----
+namespace {
+
+int bad(const char* op, const char* what) {
+    return fail(CL_ERR_INVALID_ARGUMENT, std::string(op) + ": " + what);
+}
+
+bool misaligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) != 0; }
+
+// 16-bit element type of the descriptor -> the kernels' type, -1 if neither.
+int type16(int dtype) {
+    return dtype == CL_DTYPE_F16 ? clb::kTypeF16 : dtype == CL_DTYPE_BF16 ? clb::kTypeBf16 : -1;
+}
+
+// The cache's format, shared by the cache and the attention calls.
+int check_cache(const char* op, int64_t num_pages, int kv_heads, int head_dim, int bits,
+                int page_size, const void* pages) {
+    if (head_dim != 64 && head_dim != 128 && head_dim != 256)
+        return bad(op, "head_dim must be 64, 128 or 256");
+    if (bits != 8 && bits != 4) return bad(op, "bits must be 8 or 4");
+    if (kv_heads <= 0 || kv_heads > 65535) return bad(op, "kv_heads must be in [1, 65535]");
+    if (num_pages <= 0 || num_pages > INT32_MAX) return bad(op, "num_pages must be in [1, 2^31)");
+    if (page_size <= 0 || page_size % clb::kKvBlock != 0 || page_size > (1 << 20))
+        return bad(op, "page_size must be a multiple of 16, at most 2^20");
+    if (!pages) return bad(op, "null device pointer");
+    if (misaligned16(pages)) return bad(op, "pages must be 16-byte aligned");
+    return CL_OK;
+}
+
+int cache_args(const char* op, const void* k, const void* v, const void* pages, const int64_t* slots,
+               const cl_kvcache_desc* d, clb::KvCacheArgs* a) {
+    if (!d) return bad(op, "null descriptor");
+    if (d->tokens < 0) return bad(op, "tokens must be >= 0");
+    const int type = type16(d->dtype);
+    if (type < 0) return bad(op, "dtype must be CL_DTYPE_F16 or CL_DTYPE_BF16");
+    const int rc = check_cache(op, d->num_pages, d->kv_heads, d->head_dim, d->bits, d->page_size, pages);
+    if (rc != CL_OK) return rc;
+    if (d->tokens > 0 && (!k || !v || !slots)) return bad(op, "null device pointer");
+    if (d->tokens > ((int64_t)1 << 38) / (d->kv_heads * (d->head_dim / 16)))
+        return bad(op, "too many tokens for one launch");
+    *a = clb::KvCacheArgs{const_cast<uint8_t*>(static_cast<const uint8_t*>(pages)), slots,
+                          const_cast<void*>(k), const_cast<void*>(v), d->k_token, d->k_head,
+                          d->v_token, d->v_head, d->tokens, d->num_pages, d->kv_heads, d->head_dim,
+                          d->bits, d->page_size, type};
+    return CL_OK;
+}
+
+}  // namespace
+
+int cl_qknorm_rope(const void* q, const void* k, const void* q_weight, const void* k_weight,
+                   const float* table, const void* positions, void* q_out, void* k_out,
+                   const cl_qknorm_rope_desc* d, void* stream) {
+    const char* op = "qknorm_rope";
+    if (!d) return bad(op, "null descriptor");
+    if (d->tokens < 0) return bad(op, "tokens must be >= 0");
+    if (d->q_heads <= 0 || d->kv_heads <= 0 || d->q_heads > (1 << 20) || d->kv_heads > (1 << 20))
+        return bad(op, "q_heads and kv_heads must be in [1, 2^20]");
+    if (d->head_dim <= 0 || d->head_dim % 16 != 0 || d->head_dim > 256)
+        return bad(op, "head_dim must be a multiple of 16, at most 256");
+    if (d->rotary <= 0 || d->rotary % 16 != 0 || d->rotary > d->head_dim)
+        return bad(op, "rotary must be a multiple of 16, at most head_dim");
+    const int type = type16(d->dtype);
+    if (type < 0) return bad(op, "dtype must be CL_DTYPE_F16 or CL_DTYPE_BF16");
+    if (!(d->eps >= 0.f) || !std::isfinite(d->eps)) return bad(op, "eps must be finite and >= 0");
+    if ((q_weight == nullptr) != (k_weight == nullptr))
+        return bad(op, "q_weight and k_weight must both be given, or neither");
+    if (d->table_rows <= 0) return bad(op, "table_rows must be > 0");
+    if (d->tokens == 0) return CL_OK;
+    if (!q || !k || !table || !positions || !q_out || !k_out) return bad(op, "null device pointer");
+    if (misaligned16(table)) return bad(op, "table must be 16-byte aligned");
+    if (d->tokens > ((int64_t)1 << 37) / ((d->q_heads + d->kv_heads) * 16))
+        return bad(op, "too many tokens for one launch");
+    const clb::QkRopeArgs a{{q, k},
+                            {q_out, k_out},
+                            {q_weight, k_weight},
+                            {d->q_token, d->k_token},
+                            {d->q_head, d->k_head},
+                            {d->q_out_token, d->k_out_token},
+                            {d->q_out_head, d->k_out_head},
+                            {d->q_heads, d->kv_heads},
+                            table,
+                            d->table_rows,
+                            positions,
+                            d->positions64,
+                            d->tokens,
+                            d->head_dim,
+                            d->rotary,
+                            d->interleaved,
+                            type,
+                            d->eps};
+    cudaError_t e = clb::launch_qknorm_rope(a, static_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) return cuda_fail(e, "qknorm_rope launch");
+    return CL_OK;
+}
+
+int cl_kvcache_write(const void* k, const void* v, uint8_t* pages, const int64_t* slots,
+                     const cl_kvcache_desc* d, void* stream) {
+    clb::KvCacheArgs a;
+    const int rc = cache_args("kvcache_write", k, v, pages, slots, d, &a);
+    if (rc != CL_OK) return rc;
+    cudaError_t e = clb::launch_kv_write(a, static_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) return cuda_fail(e, "kvcache_write launch");
+    return CL_OK;
+}
+
+int cl_kvcache_read(const uint8_t* pages, const int64_t* slots, void* k, void* v,
+                    const cl_kvcache_desc* d, void* stream) {
+    clb::KvCacheArgs a;
+    const int rc = cache_args("kvcache_read", k, v, pages, slots, d, &a);
+    if (rc != CL_OK) return rc;
+    cudaError_t e = clb::launch_kv_read(a, static_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) return cuda_fail(e, "kvcache_read launch");
+    return CL_OK;
+}
+
+int cl_kvattention_workspace(size_t* bytes) {
+    if (!bytes) return bad("kvattention_workspace", "bytes is null");
+    *bytes = clb::kv_attention_workspace();
+    return CL_OK;
+}
+
+int cl_kvattention(const void* q, const uint8_t* pages, const int32_t* page_table,
+                   const int32_t* lengths, const int32_t* prefix_pages, void* out, float* lse,
+                   float* prefix_out, float* prefix_lse, void* workspace,
+                   const cl_kvattention_desc* d, void* stream) {
+    const char* op = "kvattention";
+    if (!d) return bad(op, "null descriptor");
+    const int type = type16(d->dtype);
+    if (type < 0) return bad(op, "dtype must be CL_DTYPE_F16 or CL_DTYPE_BF16");
+    int rc = check_cache(op, d->num_pages, d->kv_heads, d->head_dim, d->bits, d->page_size, pages);
+    if (rc != CL_OK) return rc;
+    if (d->batch < 0 || d->batch > 4096) return bad(op, "batch must be in [0, 4096]");
+    if (d->new_tokens <= 0 || d->new_tokens > (1 << 20))
+        return bad(op, "new_tokens must be in [1, 2^20]");
+    if (d->q_heads <= 0 || d->q_heads % d->kv_heads != 0)
+        return bad(op, "q_heads must be a multiple of kv_heads");
+    if ((int64_t)d->batch * d->new_tokens * d->q_heads > INT32_MAX)
+        return bad(op, "more than 2^31 - 1 query rows");
+    if (d->window < 0) return bad(op, "window must be >= 0");
+    if (!std::isfinite(d->scale)) return bad(op, "scale must be finite");
+    if (d->max_pages < 0 || (int64_t)d->max_pages * d->page_size > INT32_MAX)
+        return bad(op, "max_pages * page_size exceeds 2^31 - 1 tokens");
+    if (d->prefix_length < 0 || d->prefix_page_count < 0) return bad(op, "negative prefix");
+    if (d->batch == 0) return CL_OK;
+    if (!q || !out || !workspace || !lengths || (d->max_pages > 0 && !page_table))
+        return bad(op, "null device pointer");
+    if (misaligned16(out) || misaligned16(workspace))
+        return bad(op, "out and workspace must be 16-byte aligned");
+    clb::KvAttentionArgs a{};
+    a.q = q;
+    a.q_batch = d->q_batch;
+    a.q_new = d->q_new;
+    a.q_head = d->q_head;
+    a.pages = pages;
+    a.num_pages = d->num_pages;
+    a.table = page_table;
+    a.table_stride = d->table_stride;
+    a.max_pages = d->max_pages;
+    a.lengths = lengths;
+    a.fixed_length = -1;
+    a.batch = d->batch;
+    a.new_tokens = d->new_tokens;
+    a.kv_heads = d->kv_heads;
+    a.group = d->q_heads / d->kv_heads;
+    a.head_dim = d->head_dim;
+    a.bits = d->bits;
+    a.page_size = d->page_size;
+    a.type = type;
+    a.causal = 1;
+    a.window = d->window;
+    a.scale = d->scale;
+    a.out = out;
+    a.lse = lse;
+    a.workspace = workspace;
+    const clb::KvAttentionArgs* both[2] = {&a, nullptr};
+    clb::KvAttentionArgs f = a;
+    if (d->prefix_length > 0) {
+        if (d->window != 0) return bad(op, "a prefix and a window exclude each other");
+        if ((int64_t)d->prefix_page_count * d->page_size > INT32_MAX)
+            return bad(op, "prefix_page_count * page_size exceeds 2^31 - 1 tokens");
+        if ((int64_t)d->prefix_page_count * d->page_size < d->prefix_length)
+            return bad(op, "prefix_pages hold fewer than prefix_length tokens");
+        if (!prefix_pages || !prefix_out || !prefix_lse) return bad(op, "null prefix pointer");
+        if (misaligned16(prefix_out)) return bad(op, "prefix_out must be 16-byte aligned");
+        if (d->batch > 1 && d->new_tokens > 1 && d->q_batch != d->new_tokens * d->q_new)
+            return bad(op, "with a prefix the q rows must be evenly spaced");
+        // the whole batch as the new tokens of one sequence that sees all of it
+        f.q_new = d->new_tokens > 1 ? d->q_new : d->q_batch;
+        f.table = prefix_pages;
+        f.table_stride = 0;
+        f.max_pages = d->prefix_page_count;
+        f.fixed_length = d->prefix_length;
+        f.batch = 1;
+        f.new_tokens = d->batch * d->new_tokens;
+        f.causal = 0;
+        f.out = nullptr;
+        f.out_f32 = prefix_out;
+        f.lse = prefix_lse;
+        a.front = prefix_out;
+        a.front_lse = prefix_lse;
+        both[0] = &f;
+        both[1] = &a;
+    }
+    for (const clb::KvAttentionArgs* one : both) {
+        if (one && !clb::kv_attention_fits(*one))
+            return bad(op, "the page tables span too many blocks for one launch");
+    }
+    for (const clb::KvAttentionArgs* one : both) {
+        if (!one) continue;
+        cudaError_t e = clb::launch_kv_attention(*one, static_cast<cudaStream_t>(stream));
+        if (e != cudaSuccess) return cuda_fail(e, "kvattention launch");
+    }
+    return CL_OK;
 }
 
 }  // extern "C"

@@ -886,4 +886,6 @@ long long set_wait_budget(long long cycles) {
     return g_wait_budget.exchange(cycles > 0 ? cycles : kWaitTimeoutCycles);
 }
 
+long long wait_budget() { return g_wait_budget.load(std::memory_order_relaxed); }
+
 }  // namespace clb

@@ -79,5 +79,6 @@ cudaError_t read_device_status(int clear, int* status);
 // Sets the bound of the device-side waits of later launches (SM cycles; <= 0
 // restores the default of about two seconds) and returns the previous bound.
 long long set_wait_budget(long long cycles);
+long long wait_budget();
 
 }  // namespace clb

@@ -1,0 +1,224 @@
+// Quantisation of K and V as they are written into the paged cache
+// (kv_layout.cuh), and reading tokens back.
+//
+// Per token and head: s = fp16(min(max|x| / top, 65504)), top = 127 (int8) or
+// 7 (int4); q = clamp(rint(x * (1 / s)), -top, top) with the stored s, so the
+// rounding of s to fp16 costs no accuracy; s = 0 gives q = 0, NaN is stored
+// as 0 and infinities saturate.  Every step is one IEEE operation in fp32.
+// x * (1 / s) instead of x / s: one division per row instead of one per
+// element, which at the instruction count of an IEEE division would bound the
+// kernel; it can differ from x / s only where x lies within an fp32 rounding
+// of the middle between two steps, where both are as near.
+//
+// Both kernels are bound by memory: the write reads 2 B and writes bits / 8 B
+// per element, the read the reverse.  A lane holds 16 elements (two 16-byte
+// loads, one 16- or 8-byte store of a chunk), head_dim / 16 lanes share a
+// row, and the same lanes take K and V so that four loads are in flight.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "gemv_common.cuh"
+#include "kv_device.cuh"
+#include "kv_layout.cuh"
+
+namespace clb {
+namespace {
+
+__device__ int g_kv_status;
+
+constexpr int kThreads = 256;
+
+// Place of a slot: its page's block, and the token's row j in the block.
+struct Place {
+    const uint8_t* block;
+    int j;
+};
+
+__device__ __forceinline__ bool find_slot(const KvCacheArgs& a, int64_t slot, int head,
+                                          int block_bytes, Place* p) {
+    if (slot < 0) return false;
+    int64_t page;
+    int off;
+    if (slot <= 0x7fffffff) {
+        page = (unsigned)slot / (unsigned)a.page_size;
+        off = (int)((unsigned)slot % (unsigned)a.page_size);
+    } else {
+        page = slot / a.page_size;
+        off = (int)(slot % a.page_size);
+    }
+    if (page >= a.num_pages) {
+        atomicCAS(&g_kv_status, 0, kStatusKvIndex);
+        return false;
+    }
+    const int64_t blocks = a.page_size / kKvBlock;
+    p->block = a.pages + ((page * a.kv_heads + head) * blocks + off / kKvBlock) * block_bytes;
+    p->j = off % kKvBlock;
+    return true;
+}
+
+template <int kBits>
+__device__ __forceinline__ void quantise16(const float (&x)[16], float s, uint32_t* out) {
+    const float inv = s == 0.f ? 0.f : __frcp_rn(s);
+    constexpr float kTop = kBits == 8 ? 127.f : 7.f;
+    uint32_t q[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        // fminf / fmaxf drop a NaN, so the select keeps it at 0
+        const float y = x[i] == x[i] ? __fmul_rn(x[i], inv) : 0.f;
+        q[i] = (uint32_t)__float2int_rn(fminf(fmaxf(y, -kTop), kTop));
+    }
+    if (kBits == 8) {
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+            out[w] = prmt_i<0x5410u>(prmt_i<0x0040u>(q[4 * w], q[4 * w + 1]),
+                                     prmt_i<0x0040u>(q[4 * w + 2], q[4 * w + 3]));
+    } else {
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+            uint32_t r = 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) r |= (q[8 * w + i] & 15u) << (4 * i);
+            out[w] = r;
+        }
+    }
+}
+
+template <int kDim, int kBits, bool kBf16, bool kVec>
+__global__ void __launch_bounds__(kThreads) kv_write_kernel(const KvCacheArgs a) {
+    constexpr int kRow = kDim * kBits / 8, kLanes = kDim / 16;
+    constexpr int kBlockBytes = kv_block_bytes(kRow);
+    pdl_allow_dependents();
+    pdl_wait_prior_grids();
+    const int64_t row = ((int64_t)blockIdx.x * kThreads + threadIdx.x) / kLanes;
+    const int l = threadIdx.x % kLanes;
+    const int64_t token = row / a.kv_heads;
+    const int head = (int)(row % a.kv_heads);
+    const bool in = token < a.tokens;
+    const int64_t slot = in ? a.slots[token] : -1;
+    float x[2][16];
+    if (in) {
+        load16<kBf16, kVec>(a.k, token * a.k_token + head * a.k_head + 16 * l, x[0]);
+        load16<kBf16, kVec>(a.v, token * a.v_token + head * a.v_head + 16 * l, x[1]);
+    }
+    Place p;
+    const bool put = find_slot(a, slot, head, kBlockBytes, &p);
+#pragma unroll
+    for (int part = 0; part < 2; ++part) {
+        float m = 0.f;
+        if (in) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) m = fmaxf(m, fabsf(x[part][i]));  // drops NaN
+        }
+#pragma unroll
+        for (int o = kLanes / 2; o > 0; o >>= 1)
+            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        const float top = kBits == 8 ? 127.f : 7.f;
+        const __half s = __float2half_rn(fminf(__fdiv_rn(m, top), 65504.f));
+        if (!put) continue;
+        uint32_t q[4];
+        quantise16<kBits>(x[part], __half2float(s), q);
+        uint8_t* rows = const_cast<uint8_t*>(p.block) + part * kKvBlock * kRow;
+        if (kBits == 8)
+            *reinterpret_cast<uint4*>(rows + kv_offset<kRow>(p.j, 16 * l)) =
+                make_uint4(q[0], q[1], q[2], q[3]);
+        else
+            *reinterpret_cast<uint2*>(rows + kv_offset<kRow>(p.j, 8 * l)) = make_uint2(q[0], q[1]);
+        if (l == 0)
+            reinterpret_cast<__half*>(const_cast<uint8_t*>(p.block) +
+                                      2 * kKvBlock * kRow)[part * kKvBlock + p.j] = s;
+    }
+}
+
+template <int kDim, int kBits, bool kBf16, bool kVec>
+__global__ void __launch_bounds__(kThreads) kv_read_kernel(const KvCacheArgs a) {
+    constexpr int kRow = kDim * kBits / 8, kLanes = kDim / 16;
+    constexpr int kBlockBytes = kv_block_bytes(kRow);
+    pdl_allow_dependents();
+    pdl_wait_prior_grids();
+    const int64_t row = ((int64_t)blockIdx.x * kThreads + threadIdx.x) / kLanes;
+    const int l = threadIdx.x % kLanes;
+    const int64_t token = row / a.kv_heads;
+    const int head = (int)(row % a.kv_heads);
+    if (token >= a.tokens) return;
+    Place p;
+    const bool have = find_slot(a, a.slots[token], head, kBlockBytes, &p);
+    uint32_t raw[2][4] = {};
+    float s[2] = {0.f, 0.f};
+    if (have) {
+#pragma unroll
+        for (int part = 0; part < 2; ++part) {
+            const uint8_t* rows = p.block + part * kKvBlock * kRow;
+            if (kBits == 8) {
+                const uint4 r = *reinterpret_cast<const uint4*>(rows + kv_offset<kRow>(p.j, 16 * l));
+                raw[part][0] = r.x, raw[part][1] = r.y, raw[part][2] = r.z, raw[part][3] = r.w;
+            } else {
+                const uint2 r = *reinterpret_cast<const uint2*>(rows + kv_offset<kRow>(p.j, 8 * l));
+                raw[part][0] = r.x, raw[part][1] = r.y;
+            }
+            s[part] = __half2float(reinterpret_cast<const __half*>(
+                p.block + 2 * kKvBlock * kRow)[part * kKvBlock + p.j]);
+        }
+    }
+#pragma unroll
+    for (int part = 0; part < 2; ++part) {
+        float x[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            // sign extension of the field by a shift pair
+            const int v = kBits == 8 ? (int)(raw[part][i / 4] << (24 - 8 * (i % 4))) >> 24
+                                     : (int)(raw[part][i / 8] << (28 - 4 * (i % 8))) >> 28;
+            x[i] = __fmul_rn((float)v, s[part]);
+        }
+        void* y = part ? a.v : a.k;
+        const int64_t at = part ? token * a.v_token + head * a.v_head
+                                : token * a.k_token + head * a.k_head;
+        store16<kBf16, kVec>(y, at + 16 * l, x);
+    }
+}
+
+using Kernel = void (*)(KvCacheArgs);
+
+template <bool kWrite, int kDim, int kBits>
+Kernel pick(bool bf16, bool vec) {
+    if constexpr (kWrite)
+        return bf16 ? (vec ? kv_write_kernel<kDim, kBits, true, true>
+                           : kv_write_kernel<kDim, kBits, true, false>)
+                    : (vec ? kv_write_kernel<kDim, kBits, false, true>
+                           : kv_write_kernel<kDim, kBits, false, false>);
+    else
+        return bf16 ? (vec ? kv_read_kernel<kDim, kBits, true, true>
+                           : kv_read_kernel<kDim, kBits, true, false>)
+                    : (vec ? kv_read_kernel<kDim, kBits, false, true>
+                           : kv_read_kernel<kDim, kBits, false, false>);
+}
+
+template <bool kWrite>
+cudaError_t launch(const KvCacheArgs& a, cudaStream_t stream) {
+    if (a.tokens == 0) return cudaSuccess;
+    const bool vec = aligned16(a.k, a.k_token, a.k_head) && aligned16(a.v, a.v_token, a.v_head);
+    const bool bf16 = a.type == kTypeBf16;
+    Kernel k = nullptr;
+    if (a.head_dim == 64)
+        k = a.bits == 8 ? pick<kWrite, 64, 8>(bf16, vec) : pick<kWrite, 64, 4>(bf16, vec);
+    else if (a.head_dim == 128)
+        k = a.bits == 8 ? pick<kWrite, 128, 8>(bf16, vec) : pick<kWrite, 128, 4>(bf16, vec);
+    else
+        k = a.bits == 8 ? pick<kWrite, 256, 8>(bf16, vec) : pick<kWrite, 256, 4>(bf16, vec);
+    const int64_t threads = a.tokens * a.kv_heads * (a.head_dim / 16);
+    return launch_pdl(k, dim3((unsigned)((threads + kThreads - 1) / kThreads)), dim3(kThreads), 0,
+                      stream, a);
+}
+
+}  // namespace
+
+cudaError_t launch_kv_write(const KvCacheArgs& a, cudaStream_t s) { return launch<true>(a, s); }
+cudaError_t launch_kv_read(const KvCacheArgs& a, cudaStream_t s) { return launch<false>(a, s); }
+
+cudaError_t read_kv_status(int clear, int* status) {
+    return read_status_symbol(g_kv_status, clear, status);
+}
+
+}  // namespace clb

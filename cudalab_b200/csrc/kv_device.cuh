@@ -1,0 +1,118 @@
+// Device and launch helpers shared by the attention-side kernels: 16-element
+// row pieces of fp16 / bf16 tensors, programmatic dependent launch, the status
+// words of these translation units.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+namespace clb {
+
+template <bool kBf16>
+__device__ __forceinline__ float2 unpack2(uint32_t v) {
+    if (kBf16) return __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&v));
+    return __half22float2(*reinterpret_cast<__half2*>(&v));
+}
+
+template <bool kBf16>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    if (kBf16) {
+        __nv_bfloat162 r = __floats2bfloat162_rn(lo, hi);
+        return *reinterpret_cast<uint32_t*>(&r);
+    }
+    __half2 r = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<uint32_t*>(&r);
+}
+
+// 8 consecutive elements starting at element `at`; kVec: 16-byte aligned.
+template <bool kBf16, bool kVec>
+__device__ __forceinline__ uint4 load8(const void* p, int64_t at) {
+    const uint16_t* e = static_cast<const uint16_t*>(p) + at;
+    if (kVec) return *reinterpret_cast<const uint4*>(e);
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = (uint32_t)e[2 * i] | ((uint32_t)e[2 * i + 1] << 16);
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+template <bool kVec>
+__device__ __forceinline__ void store8(void* p, int64_t at, uint4 v) {
+    uint16_t* e = static_cast<uint16_t*>(p) + at;
+    if (kVec) {
+        *reinterpret_cast<uint4*>(e) = v;
+        return;
+    }
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        e[2 * i] = (uint16_t)w[i];
+        e[2 * i + 1] = (uint16_t)(w[i] >> 16);
+    }
+}
+
+template <bool kBf16>
+__device__ __forceinline__ void unpack8(uint4 v, float* x) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = unpack2<kBf16>(w[i]);
+        x[2 * i] = f.x;
+        x[2 * i + 1] = f.y;
+    }
+}
+
+template <bool kBf16>
+__device__ __forceinline__ uint4 pack8(const float* x) {
+    return make_uint4(pack2<kBf16>(x[0], x[1]), pack2<kBf16>(x[2], x[3]),
+                      pack2<kBf16>(x[4], x[5]), pack2<kBf16>(x[6], x[7]));
+}
+
+template <bool kBf16, bool kVec>
+__device__ __forceinline__ void load16(const void* p, int64_t at, float (&x)[16]) {
+    const uint4 a = load8<kBf16, kVec>(p, at), b = load8<kBf16, kVec>(p, at + 8);
+    unpack8<kBf16>(a, x);
+    unpack8<kBf16>(b, x + 8);
+}
+
+template <bool kBf16, bool kVec>
+__device__ __forceinline__ void store16(void* p, int64_t at, const float (&x)[16]) {
+    store8<kVec>(p, at, pack8<kBf16>(x));
+    store8<kVec>(p, at + 8, pack8<kBf16>(x + 8));
+}
+
+// Rows of 16-bit elements that 16-byte accesses may be used on.
+inline bool aligned16(const void* p, int64_t stride0, int64_t stride1) {
+    return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && stride0 % 8 == 0 && stride1 % 8 == 0;
+}
+
+// Programmatic dependent launch: the kernel waits (griddepcontrol.wait) before
+// its first global access, so the launch latency is hidden and stream order kept.
+template <typename... P, typename... A>
+cudaError_t launch_pdl(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem,
+                       cudaStream_t stream, const A&... args) {
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+// Reads (optionally clears) a status word of the calling translation unit.
+template <typename Symbol>
+cudaError_t read_status_symbol(Symbol& symbol, int clear, int* status) {
+    cudaError_t e = cudaMemcpyFromSymbol(status, symbol, sizeof(int));
+    const int zero = 0;
+    if (e == cudaSuccess && clear) e = cudaMemcpyToSymbol(symbol, &zero, sizeof(int));
+    return e;
+}
+
+}  // namespace clb

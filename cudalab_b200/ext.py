@@ -605,13 +605,18 @@ class RmsnormExt:
         self._launch(x, w, out, eps, flags)
 
 
-_EXT_TYPES = {"int4gemv": Int4gemvExt, "qgemv": QgemvExt, "gemv": GemvExt, "rmsnorm": RmsnormExt}
+def _ext_types() -> dict:
+    from . import attention_ext as att
+    return {"int4gemv": Int4gemvExt, "qgemv": QgemvExt, "gemv": GemvExt, "rmsnorm": RmsnormExt,
+            "qknorm_rope": att.QkNormRopeExt, "kvcache": att.KvCacheExt,
+            "kvattention": att.KvAttentionExt}
 
 
 def get_ext(op: str):
     """Singleton extension object for `op`."""
-    if op not in _EXT_TYPES:
-        raise RuntimeError(f"unknown operator {op!r}; available: {', '.join(_EXT_TYPES)}")
     if op not in _EXTS:
-        _EXTS[op] = _EXT_TYPES[op]()
+        types = _ext_types()
+        if op not in types:
+            raise RuntimeError(f"unknown operator {op!r}; available: {', '.join(types)}")
+        _EXTS[op] = types[op]()
     return _EXTS[op]

@@ -75,7 +75,8 @@ const char* cl_version(void);
 const char* cl_last_error(void);
 
 /* Reads (and optionally clears) the bounded-wait status word of the current
- * device: 0 = no device-side wait expired since the last clear. */
+ * device: 0 = no device-side wait expired and no index error was recorded
+ * since the last clear. */
 int cl_device_status(int clear, int* status_out);
 
 /* No counterpart in the reference (its kernels never wait on device-side
@@ -289,6 +290,100 @@ int cl_qgemv_sharded(const char* variant, const int8_t* W_shard, const float* sc
                      const void* x, int64_t M, void* const* y_peers, void* const* flag_peers,
                      int rank, int world, int64_t row0, int64_t N_shard, int64_t N_total,
                      int64_t K, void* stream, uint32_t flags);
+
+/* ---- attention of a decode step over a quantised paged cache ----
+ * No counterpart in the reference, whose operators end at the projections:
+ * these compute what lies between the q / k / v projection and the output
+ * projection of a decoder layer.  Element types of q, k, v and the outputs:
+ * CL_DTYPE_F16 or CL_DTYPE_BF16; strides are in elements, the last dimension
+ * is contiguous; rows whose base and strides are 16-byte aligned are accessed
+ * 16 bytes at a time, others element by element.  Index errors that only the
+ * device can see (a slot, page or position outside its range, a length
+ * outside the page table) are recorded as status 7 in cl_device_status; the
+ * entry is then skipped or clamped, no memory outside the arguments is
+ * touched.  Every launch is a programmatic dependent launch that waits for
+ * the preceding kernel before its first global access.
+ *
+ * The cache.  pages: uint8 [num_pages, kv_heads, page_size / 16, block bytes],
+ * 16-byte aligned; block bytes = 4 * head_dim * bits + 64 for bits 8 or 4,
+ * head_dim 64, 128 or 256, page_size a multiple of 16.  A block holds 16
+ * tokens of one head: their K rows, their V rows (whole values, two's
+ * complement, int4 low nibble = even element; rows permuted inside the block,
+ * csrc/kv_layout.cuh), then 16 fp16 scales of K and 16 of V, one per token.
+ * Token slot = page * page_size + offset in the page. */
+#define CL_DTYPE_BF16 2
+
+/* RMSNorm of every head of q [tokens, q_heads, head_dim] and k [tokens,
+ * kv_heads, head_dim] (q_weight, k_weight [head_dim]; both null: no norm) and
+ * the rotation by position, in one pass: of the normalised row, the first
+ * `rotary` elements turn in pairs (i, i + rotary / 2), or (2i, 2i + 1) when
+ * `interleaved`, by row positions[t] of table fp32 [table_rows, rotary]
+ * (rotary / 2 cosines, then the sines; 16-byte aligned).  head_dim and rotary
+ * are multiples of 16, head_dim <= 256.  q_out / k_out may be q / k.
+ * positions: int32, or int64 with positions64. */
+typedef struct cl_qknorm_rope_desc {
+    int64_t tokens, table_rows;
+    int64_t q_token, q_head, k_token, k_head;                 /* strides of q and k */
+    int64_t q_out_token, q_out_head, k_out_token, k_out_head; /* of the outputs */
+    int32_t q_heads, kv_heads, head_dim, rotary;
+    int32_t interleaved, positions64, dtype;
+    float eps;
+} cl_qknorm_rope_desc;
+int cl_qknorm_rope(const void* q, const void* k, const void* q_weight, const void* k_weight,
+                   const float* table, const void* positions, void* q_out, void* k_out,
+                   const cl_qknorm_rope_desc* desc, void* stream);
+
+/* Write: quantises k, v [tokens, kv_heads, head_dim] into their slots (int64
+ * [tokens]; negative: the token is skipped; no two the same).  Per token and
+ * head s = fp16(min(max|x| / top, 65504)), top = 127 or 7, q = clamp(rint(x *
+ * (1 / s)), -top, top) in fp32 with the stored s; s = 0 gives q = 0, NaN is
+ * stored as 0, infinities saturate.
+ * Read: k, v of the slots as dtype(q * s); zeros for a skipped slot. */
+typedef struct cl_kvcache_desc {
+    int64_t tokens, num_pages;
+    int64_t k_token, k_head, v_token, v_head; /* strides of k and v */
+    int32_t kv_heads, head_dim, bits, page_size, dtype;
+} cl_kvcache_desc;
+int cl_kvcache_write(const void* k, const void* v, uint8_t* pages, const int64_t* slots,
+                     const cl_kvcache_desc* desc, void* stream);
+int cl_kvcache_read(const uint8_t* pages, const int64_t* slots, void* k, void* v,
+                    const cl_kvcache_desc* desc, void* stream);
+
+/* Attention of q [batch, new_tokens, q_heads, head_dim] over the cached
+ * tokens of each sequence: page_table int32 [batch, max_pages] (row stride
+ * table_stride), lengths int32 [batch], the new tokens included.  Row i of a
+ * sequence sees its tokens up to length - new_tokens + i (with window > 0 the
+ * last `window` of them); q_heads is a multiple of kv_heads, head h reads
+ * cache head h / (q_heads / kv_heads).  out [batch, new_tokens, q_heads,
+ * head_dim] contiguous; lse fp32 [batch, new_tokens, q_heads] (natural log of
+ * the softmax's denominator) or null.  A row that sees nothing gives zeros
+ * and -inf.  batch <= 4096.
+ *
+ * With prefix_pages (int32 [prefix_page_count]) and prefix_length > 0 the
+ * tokens of those pages stand in front of every sequence's own (length counts
+ * the own ones) and are read once for the whole batch: one launch over the
+ * prefix, then one over the sequences that joins the two.  prefix_out (fp32
+ * [batch, new_tokens, q_heads, head_dim], 16-byte aligned) and prefix_lse
+ * (fp32 [batch, new_tokens, q_heads]) are scratch of the call.  The q rows
+ * must then be evenly spaced (q_batch == new_tokens * q_new when both batch
+ * and new_tokens exceed 1) and window must be 0.
+ *
+ * workspace: cl_kvattention_workspace bytes, 16-byte aligned, zero-filled
+ * once before its first use and again only after a launch that failed; each
+ * call leaves it ready for the next one on the same stream.  Calls that may
+ * overlap (other streams) need workspaces of their own. */
+typedef struct cl_kvattention_desc {
+    int64_t num_pages, table_stride;
+    int64_t q_batch, q_new, q_head; /* strides of q */
+    int32_t batch, new_tokens, q_heads, kv_heads, head_dim, bits, page_size, max_pages;
+    int32_t window, dtype, prefix_length, prefix_page_count;
+    float scale;
+} cl_kvattention_desc;
+int cl_kvattention_workspace(size_t* bytes);
+int cl_kvattention(const void* q, const uint8_t* pages, const int32_t* page_table,
+                   const int32_t* lengths, const int32_t* prefix_pages, void* out, float* lse,
+                   float* prefix_out, float* prefix_lse, void* workspace,
+                   const cl_kvattention_desc* desc, void* stream);
 
 #ifdef __cplusplus
 } /* extern "C" */

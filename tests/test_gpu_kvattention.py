@@ -1,0 +1,241 @@
+"""Attention over the quantised paged cache (cl_kvattention) against the
+formula in 64 bits on the values the cache holds; tolerances from the kernel's
+roundings (oracle.attention_oracle.attention_tolerance)."""
+import numpy as np
+import pytest
+import torch
+
+from cudalab_b200 import _native as nat
+from cudalab_b200.build import build
+from oracle import attention_oracle as oa
+
+pytestmark = pytest.mark.gpu
+F16, BF16 = torch.float16, torch.bfloat16
+
+
+class Cache:
+    """`tokens` random tokens per sequence in shuffled pages, and their values."""
+
+    def __init__(self, lengths, H, D, bits, page, seed, spread=0.5, scales=0.5):
+        self.ext = build("kvcache")
+        g = torch.Generator().manual_seed(seed)
+        self.page, self.D, self.H = page, D, H
+        width = max(1, max(-(-n // page) for n in lengths))
+        total = len(lengths) * width + 2
+        order = torch.randperm(total, generator=g)
+        self.table = order[:len(lengths) * width].view(len(lengths), width).int().cuda()
+        self.pages = self.ext.empty(total, H, D, bits, page)
+        # what no token was written to holds NaN scales and arbitrary bytes
+        self.pages.fill_(0xFF)
+        self.lengths = list(lengths)
+        self.k, self.v = [], []
+        for b, n in enumerate(lengths):
+            k = torch.randn(n, H, D, generator=g) * torch.exp(spread * torch.randn(n, H, 1, generator=g))
+            v = torch.randn(n, H, D, generator=g) * torch.exp(scales * torch.randn(n, H, 1, generator=g))
+            j = torch.arange(n)
+            slots = (self.table[b].cpu().long()[j // page] * page + j % page).cuda()
+            k, v = k.half().cuda(), v.half().cuda()
+            self.ext.write(k, v, self.pages, slots)
+            vals = []
+            for x in (k, v):
+                q, s = oa.quantise(x.float().cpu().numpy(), bits)
+                vals.append(q.astype(np.float64) * s.astype(np.float64)[..., None])
+            self.k.append(vals[0])
+            self.v.append(vals[1])
+
+    def len_tensor(self):
+        return torch.tensor(self.lengths, dtype=torch.int32, device="cuda")
+
+
+def _q(B, n, Hq, D, dtype, seed, scale=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return (scale * torch.randn(B, n, Hq, D, generator=g)).to(dtype).cuda()
+
+
+def _check(out, lse, q, c, scale, window=0, prefix=None):
+    """q, out [B, n, Hq, D], lse [B, n, Hq]."""
+    out, lse = out.double().cpu().numpy(), lse.double().cpu().numpy()
+    bits = 11 if q.dtype == F16 else 8
+    for b, n in enumerate(c.lengths):
+        k, v, pre = c.k[b], c.v[b], 0
+        if prefix is not None:
+            k, v, pre = (np.concatenate((prefix.k[0], k)), np.concatenate((prefix.v[0], v)),
+                         prefix.lengths[0])
+        ref, rl, pv, mag = oa.attention(q[b].double().cpu().numpy(), k, v, n, scale, window, pre)
+        tokens, vmax = len(k), np.abs(v).max() if len(v) else 0.0
+        tol = oa.attention_tolerance(ref, pv, mag, vmax, tokens, q.shape[-1], bits)
+        err = np.abs(out[b] - ref)
+        assert (err <= tol).all(), (b, n, float((err / tol).max()))
+        assert np.array_equal(np.isinf(rl), np.isinf(lse[b])), (b, n)
+        fin = np.isfinite(rl)
+        ltol = oa.lse_tolerance(rl, mag, tokens, q.shape[-1])
+        assert (np.abs(lse[b] - rl)[fin] <= ltol[fin]).all(), (b, n)
+    assert nat.device_status(clear=True) == 0
+
+
+# every head_dim and format, lengths around the block, the page and the split
+LENGTHS = [0, 1, 2, 15, 16, 17, 31, 33, 63, 64, 65, 127, 200, 517]
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=str)
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("group", [1, 5, 8, 12])
+def test_lengths_and_formats(group, D, bits, dtype):
+    c = Cache(LENGTHS, 2, D, bits, 32, seed=D + bits + group)
+    q = _q(len(LENGTHS), 1, 2 * group, D, dtype, seed=group)
+    att = build("kvattention")
+    ws = att.workspace()
+    for _ in range(2):  # the second call meets the workspace the first one left
+        out, lse = att.forward(q[:, 0], c.pages, c.table, c.len_tensor(), workspace=ws,
+                               return_lse=True)
+        _check(out[:, None], lse[:, None], q, c, D ** -0.5)
+
+
+@pytest.mark.parametrize("n,window", [(2, 0), (5, 0), (1, 16), (1, 1), (4, 7), (8, 100), (3, 5000)])
+@pytest.mark.parametrize("D,bits,page", [(64, 8, 16), (128, 4, 64), (256, 8, 48)])
+def test_new_tokens_and_windows(D, bits, page, n, window):
+    """Rows in front of a sequence's first token see nothing: zeros and -inf."""
+    c = Cache([0, 1, 3, 8, 50, 300], 2, D, bits, page, seed=n + window + D)
+    q = _q(6, n, 6, D, F16, seed=n)
+    out, lse = build("kvattention").forward(q, c.pages, c.table, c.len_tensor(), window=window,
+                                            return_lse=True)
+    _check(out, lse, q, c, D ** -0.5, window)
+    for b, length in enumerate(c.lengths):
+        for i in range(n):
+            if length - n + i < 0:
+                assert torch.count_nonzero(out[b, i]) == 0 and (lse[b, i] == float("-inf")).all()
+
+
+@pytest.mark.parametrize("D,bits", [(64, 4), (128, 8), (256, 4)])
+def test_long_sequence_split_over_many_ctas(D, bits):
+    """One head of one long sequence: every CTA holds a part of it, the parts
+    are joined in two levels, and a second call gives the same bits."""
+    c = Cache([20011], 1, D, bits, 64, seed=D)
+    q = _q(1, 1, 4, D, F16, seed=5, scale=2.0)
+    att = build("kvattention")
+    ws = att.workspace()
+    out, lse = att.forward(q, c.pages, c.table, c.len_tensor(), workspace=ws, return_lse=True)
+    _check(out, lse, q, c, D ** -0.5)
+    again = att.forward(q, c.pages, c.table, c.len_tensor(), workspace=ws)
+    assert torch.equal(again, out)
+
+
+def test_many_sequences():
+    lengths = [(7 * i) % 90 for i in range(300)]
+    c = Cache(lengths, 1, 64, 8, 16, seed=11)
+    q = _q(300, 1, 3, 64, F16, seed=12)
+    out, lse = build("kvattention").forward(q, c.pages, c.table, c.len_tensor(), return_lse=True)
+    _check(out, lse, q, c, 64 ** -0.5)
+
+
+def test_scales_of_every_size():
+    """Values and keys whose scales span fp16: weights stay accurate because the
+    softmax reference carries the scale."""
+    c = Cache([700, 40], 2, 128, 8, 64, seed=13, spread=1.5, scales=3.0)
+    q = _q(2, 1, 8, 128, F16, seed=14, scale=3.0)
+    out, lse = build("kvattention").forward(q, c.pages, c.table, c.len_tensor(), return_lse=True)
+    _check(out, lse, q, c, 128 ** -0.5)
+
+
+def test_large_and_small_bf16_queries():
+    c = Cache([300, 5], 1, 128, 8, 16, seed=15)
+    for size in (1e-20, 1e30):
+        q = _q(2, 1, 8, 128, BF16, seed=16, scale=size)
+        scale = 0.1 / size
+        out, lse = build("kvattention").forward(q, c.pages, c.table, c.len_tensor(), scale=scale,
+                                                return_lse=True)
+        _check(out, lse, q, c, scale)
+
+
+def test_scale_argument_and_strided_q():
+    c = Cache([90, 33, 1], 2, 128, 8, 32, seed=17)
+    att = build("kvattention")
+    qkv = _q(3, 2, 12, 131, F16, seed=18)
+    q = qkv[:, :, 2:10, 1:129]  # odd strides: element accesses
+    out, lse = att.forward(q, c.pages, c.table, c.len_tensor(), scale=0.3, return_lse=True)
+    _check(out, lse, q, c, 0.3)
+    same = torch.empty_like(out)
+    att.forward_into(q.contiguous(), c.pages, c.table, c.len_tensor(), same, scale=0.3)
+    assert torch.equal(same, out)
+
+
+def test_nan_and_inf_stay_in_their_row():
+    c = Cache([40, 40], 1, 128, 8, 16, seed=19)
+    q = _q(2, 1, 8, 128, F16, seed=20)
+    att = build("kvattention")
+    clean = att.forward(q, c.pages, c.table, c.len_tensor())
+    q[0, 0, 3, 7] = float("nan")
+    q[1, 0, 5, 9] = float("inf")
+    out, lse = att.forward(q, c.pages, c.table, c.len_tensor(), return_lse=True)
+    bad = torch.isnan(out).any(-1)
+    assert bad.sum() == 2 and bad[0, 0, 3] and bad[1, 0, 5]
+    assert torch.isnan(lse[0, 0, 3])
+    assert torch.equal(out[~bad], clean[~bad])
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=str)
+@pytest.mark.parametrize("D,bits,group,n", [(64, 8, 1, 1), (128, 8, 8, 1), (128, 4, 4, 3),
+                                            (256, 8, 2, 2), (64, 4, 16, 1)])
+@pytest.mark.parametrize("prefix", [1, 16, 100, 1037])
+def test_shared_prefix(prefix, D, bits, group, n, dtype):
+    p = Cache([prefix], 2, D, bits, 32, seed=prefix)
+    c = Cache([0, 1, 40, 7, 133], 2, D, bits, 32, seed=prefix + 1)
+    # one cache: the prefix's pages behind the sequences'
+    pages = torch.cat((c.pages, p.pages))
+    prefix_pages = p.table[0] + c.pages.shape[0]
+    q = _q(5, n, 2 * group, D, dtype, seed=prefix + 2)
+    att = build("kvattention")
+    out, lse = att.forward_shared(q, pages, prefix_pages, prefix, c.table, c.len_tensor(),
+                                  workspace=att.workspace(), return_lse=True)
+    _check(out, lse, q, c, D ** -0.5, prefix=p)
+    none = att.forward_shared(q, pages, prefix_pages, 0, c.table, c.len_tensor())
+    assert torch.equal(none, att.forward(q, pages, c.table, c.len_tensor()))
+
+
+def test_index_errors_are_recorded():
+    """A page outside the cache is skipped, a length beyond the table clamped."""
+    c = Cache([64, 20], 1, 128, 8, 16, seed=21)
+    q = _q(2, 1, 8, 128, F16, seed=22)
+    att = build("kvattention")
+    table = c.table.clone()
+    table[0, 1] = c.pages.shape[0]
+    table[0, 2] = -1
+    out = att.forward(q, c.pages, table, c.len_tensor())
+    torch.cuda.synchronize()
+    assert nat.device_status(clear=True) == 7 and torch.isfinite(out).all()
+    keep = np.r_[0:16, 48:64]
+    ref, _, pv, mag = oa.attention(q[0].double().cpu().numpy(), c.k[0][keep], c.v[0][keep], 32,
+                                   128 ** -0.5)
+    tol = oa.attention_tolerance(ref, pv, mag, np.abs(c.v[0]).max(), 64, 128, 11)
+    assert (np.abs(out[0].double().cpu().numpy() - ref) <= tol).all()
+    lengths = torch.tensor([64, 10 ** 6], dtype=torch.int32, device="cuda")
+    att.forward(q, c.pages, c.table, lengths)
+    torch.cuda.synchronize()
+    assert nat.device_status(clear=True) == 7
+
+
+def test_other_stream_and_graph():
+    c = Cache([500, 77, 0], 2, 128, 8, 64, seed=23)
+    q = _q(3, 1, 16, 128, F16, seed=24)
+    att = build("kvattention")
+    ws, lens = att.workspace(), c.len_tensor()
+    ref = att.forward(q, c.pages, c.table, lens, workspace=ws)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        y = att.forward(q, c.pages, c.table, lens, workspace=ws)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            z = att.forward(q, c.pages, c.table, lens, workspace=ws)
+        for _ in range(3):
+            g.replay()
+    s.synchronize()
+    assert torch.equal(y, ref) and torch.equal(z, ref)
+
+
+def test_empty_batch():
+    c = Cache([3], 1, 64, 8, 16, seed=25)
+    q = torch.empty(0, 2, 64, dtype=F16, device="cuda")
+    out = build("kvattention").forward(q, c.pages, c.table[:0], c.len_tensor()[:0])
+    assert out.shape == (0, 2, 64)
