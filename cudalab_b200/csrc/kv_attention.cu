@@ -27,8 +27,9 @@
 //
 // Split.  The 16-token blocks of all (sequence, head, row tile) segments form
 // one line that is cut into equal ranges, one per CTA of a persistent grid, so
-// ragged batches balance whatever their lengths; the four warps of a CTA take
-// its blocks in turn.  Each warp has its own ring of block buffers filled by
+// ragged batches balance whatever their lengths; few segments are instead cut
+// into equal chunks that no CTA shares with another segment.  The four warps
+// of a CTA take its blocks in turn.  Each warp has its own ring of block buffers filled by
 // bulk copies (one per block) and never waits for another warp until a segment
 // ends.  A segment cut over several CTAs leaves partial results in the
 // workspace; the CTA that arrives last at a group's counter adds the group's
@@ -54,8 +55,8 @@ __device__ int g_kv_attention_status;
 
 constexpr int kWarps = 4, kThreads = 32 * kWarps;
 constexpr int kMaxBatch = 4096;  // lengths and their running sum are kept in shared memory
-constexpr int kMaxGrid = 148 * 8;
-constexpr int kFan = 16;         // partial results added by one CTA
+constexpr int kMaxGrid = 148 * 5;
+constexpr int kFan = 16;         // partial results added by one CTA at a time
 constexpr float kSlack = 8.f;    // weights stay below 2^8, far inside fp16
 constexpr int kPartialFloats = 16 * 128 + 2 * 16;  // O, m and l of one partial result
 constexpr size_t kCounterBytes = (size_t)kMaxGrid * 3 * sizeof(int);
@@ -67,7 +68,7 @@ __device__ __forceinline__ float ex2(float x) {
 }
 __device__ __forceinline__ float lg2(float x) {
     float y;
-    asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
 
@@ -104,33 +105,46 @@ __device__ __forceinline__ uint32_t nibbles15(uint32_t w) {
     return h2_add(lop3_sel_xor_i<0x00F000F0u, 0x54805480u>(w), kH_m72);
 }
 
-// kWords words of a row from shared memory, at byte offset `at` of its part:
-// one 4-, 8- or 16-byte access.
+// kWords words of a row from shared memory: one 4-, 8- or 16-byte access.
 template <int kWords>
-__device__ __forceinline__ void lds_words(uint32_t addr, uint32_t* w) {
+__device__ __forceinline__ void lds_words(const uint8_t* at, uint32_t* w) {
     if constexpr (kWords == 4) {
-        const uint4 v = lds16(addr);
+        const uint4 v = *reinterpret_cast<const uint4*>(at);
         w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
     } else if constexpr (kWords == 2) {
-        asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(addr));
+        const uint2 v = *reinterpret_cast<const uint2*>(at);
+        w[0] = v.x, w[1] = v.y;
     } else {
-        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[0]) : "r"(addr));
+        w[0] = *reinterpret_cast<const uint32_t*>(at);
     }
 }
-__device__ __forceinline__ float lds_half(uint32_t addr) {
-    uint16_t v;
-    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(addr));
-    return __half2float(__ushort_as_half(v));
+__device__ __forceinline__ float lds_half(const uint8_t* at) {
+    return __half2float(*reinterpret_cast<const __half*>(at));
 }
+
+// n / d for 0 <= n < 2^31 by a multiplication, d fixed at launch.
+struct FastDiv {
+    uint32_t d, mul, shift;
+    FastDiv() = default;
+    explicit FastDiv(uint32_t divisor) : d(divisor), mul(0), shift(0) {
+        while (((uint64_t)1 << shift) < d) ++shift;
+        mul = (uint32_t)((((uint64_t)1 << 32) * (((uint64_t)1 << shift) - d)) / d + 1);
+    }
+    __device__ __forceinline__ int div(int n) const {
+        return (int)((__umulhi((uint32_t)n, mul) + (uint32_t)n) >> shift);
+    }
+    __device__ __forceinline__ int mod(int n) const { return n - div(n) * (int)d; }
+};
 
 struct Params {
     KvAttentionArgs a;
     float* partial;
     int* counters;
-    int row_tiles;       // of kCols rows each, per (sequence, head)
-    int blocks_per_page;
-    uint32_t page_magic; // ceil(2^32 / blocks_per_page)
-    int min_blocks;      // smallest range of a CTA
+    FastDiv row_tiles;   // of kCols rows each, per (sequence, head)
+    FastDiv page_blocks; // blocks of a page
+    FastDiv group;       // query heads per cache head
+    int min_units;       // smallest range of a CTA
+    int every_chunk;     // the grid holds every chunk of min_units
     int q_vec;
     long long wait_cycles;
 };
@@ -140,26 +154,33 @@ struct Shape {
     static constexpr int kRow = kDim * kBits / 8;
     static constexpr int kBlockBytes = kv_block_bytes(kRow);
     static constexpr int kCols = 8 * kNB;
-    // Ring depth per warp: what keeps 16 KB or more in flight per warp slot of
-    // an SM without taking the third CTA's shared memory.
-    static constexpr int kStages = kBlockBytes <= 1088 ? 6 : kBlockBytes <= 2112 ? 5
-                                   : kBlockBytes <= 4160 ? 3 : 2;
-    static constexpr int kRingBytes = kWarps * kStages * kBlockBytes;
+    // Blocks that a warp takes at a time: two give its instruction stream two
+    // independent chains and halve what is paid per step.
+    static constexpr int kU = kDim == 256 ? 1 : 2;
+    // CTAs per SM that the registers allow, and the ring depth per warp that
+    // the shared memory allows beside them.
+    static constexpr int kPerSm = kDim == 256 || (kDim == 128 && kNB == 2) ? 2 : 3;
+    static constexpr int kStageBytes = kU * kBlockBytes;
     static constexpr int kRedBytes = kWarps * 8 * kDim * 4;
     static constexpr int kStatBytes = kWarps * kCols * 2 * 4;
+    static constexpr int kSpare = 227 * 1024 / kPerSm - 4096 - kRedBytes - kStatBytes;
+    static constexpr int kFit = kSpare / (kWarps * kStageBytes);
+    static constexpr int kStages = kFit < 2 ? 2 : kFit > 6 ? 6 : kFit;
+    static constexpr int kRingBytes = kWarps * kStages * kStageBytes;
 };
 
-// The walk over the line of blocks: segment s covers [seg0, seg0 + blocks).
-struct Cursor {
-    int seq, unit;    // sequence; head * row_tiles + tile
-    int seg0, blocks;
+// A segment of the line: its units are [begin, begin + units).
+struct Segment {
+    int seq, part;  // sequence; head * row_tiles + row tile
+    int begin, units;
 };
 
 template <int kDim, int kBits, int kNB, bool kBf16>
-__global__ void __launch_bounds__(kThreads, kDim == 256 ? 2 : 3)
+__global__ void __launch_bounds__(kThreads, Shape<kDim, kBits, kNB>::kPerSm)
     kv_attention_kernel(const Params p) {
     using S = Shape<kDim, kBits, kNB>;
     constexpr int kRow = S::kRow, kStages = S::kStages, kBlockBytes = S::kBlockBytes;
+    constexpr int kU = S::kU, kStageBytes = S::kStageBytes;
     constexpr int kSteps = kDim / 16;  // mma steps of q . k, and 16-row blocks of O^T
     extern __shared__ __align__(128) uint8_t smem[];
     uint8_t* ring = smem;
@@ -168,16 +189,16 @@ __global__ void __launch_bounds__(kThreads, kDim == 256 ? 2 : 3)
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::kRingBytes + S::kRedBytes + S::kStatBytes);
     int* flag = reinterpret_cast<int*>(bars + kWarps * kStages);
     int* s_len = flag + 4;                 // [batch]
-    int* s_cum = s_len + p.a.batch;        // [batch + 1] blocks in front of a sequence
+    int* s_cum = s_len + p.a.batch;        // [batch + 1] cells in front of a sequence
 
     const KvAttentionArgs& a = p.a;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int g = lane >> 2, t = lane & 3;
-    const int units = a.kv_heads * p.row_tiles;
+    const int heads_tiles = a.kv_heads * (int)p.row_tiles.d;  // segments of a sequence
     const int rows = a.new_tokens * a.group;
 
     pdl_allow_dependents();
-    const uint32_t my_ring = smem_u32(ring) + warp * kStages * kBlockBytes;
+    uint8_t* my_ring = ring + warp * kStages * kStageBytes;
     const uint32_t my_bars = smem_u32(bars) + warp * kStages * 8;
     if (lane == 0) {
         for (int i = 0; i < kStages; ++i) mbar_init(my_bars + 8 * i, 1);
@@ -185,50 +206,91 @@ __global__ void __launch_bounds__(kThreads, kDim == 256 ? 2 : 3)
     }
     pdl_wait_prior_grids();
 
-    // Lengths, and the blocks of each sequence summed up.  A window drops the
-    // blocks in front of the first token that any row sees.
+    // Units of each sequence (a window drops the blocks in front of the first
+    // token that any row sees), and how the line of all segments is cut.
     auto first_block = [&](int len) {
         if (a.window <= 0) return 0;
         const int first = len - a.new_tokens + 1 - a.window;
         return first > 0 ? first / kKvBlock : 0;
     };
-    const int most = a.max_pages * a.page_size;
-    {
-        const int per = (a.batch + kThreads - 1) / kThreads, b0 = tid * per;
-        int sum = 0;
-        for (int b = b0; b < min(b0 + per, a.batch); ++b) {
-            int len = a.fixed_length >= 0 ? a.fixed_length : a.lengths[b];
-            if (len > most || len < 0) {
-                if (blockIdx.x == 0) atomicCAS(&g_kv_attention_status, 0, kStatusKvIndex);
-                len = len < 0 ? 0 : most;
-            }
-            s_len[b] = len;
-            s_cum[b] = sum;  // of this thread's sequences, for now
-            sum += (len + kKvBlock - 1) / kKvBlock - first_block(len);
+    auto units_of = [&](int len) {
+        return ((len + kKvBlock - 1) / kKvBlock - first_block(len) + kU - 1) / kU;
+    };
+    const int most = a.max_pages * a.page_size, grid = (int)gridDim.x;
+    // Up to 32 sequences every warp plans for itself (all write the same values
+    // and read their own), more are planned by the first warp.
+    const bool few = a.batch <= 32;
+    for (int b = few ? lane : tid; b < a.batch; b += few ? 32 : kThreads) {
+        int len = a.fixed_length >= 0 ? a.fixed_length : __ldg(a.lengths + b);
+        if (len > most || len < 0) {
+            if (blockIdx.x == 0) atomicCAS(&g_kv_attention_status, 0, kStatusKvIndex);
+            len = len < 0 ? 0 : most;
         }
-        int scan = sum;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int v = __shfl_up_sync(0xffffffffu, scan, o);
-            if (lane >= o) scan += v;
-        }
-        int* tot = reinterpret_cast<int*>(red);
-        if (lane == 31) tot[warp] = scan;
-        __syncthreads();
-        int before = scan - sum;
-        for (int w = 0; w < warp; ++w) before += tot[w];
-        for (int b = b0; b < min(b0 + per, a.batch); ++b) s_cum[b] += before;
-        if (tid == kThreads - 1) s_cum[a.batch] = before + sum;
-        __syncthreads();
+        s_len[b] = len;
     }
-    const int total = s_cum[a.batch] * units;
-    const int share = max(p.min_blocks, (total + (int)gridDim.x - 1) / (int)gridDim.x);
-    const int u0 = min(total, (int)blockIdx.x * share), u1 = min(total, u0 + share);
+    int cell = 1;   // units of a cell of the line (s_cum counts cells)
+    int share = 1;  // cells of a CTA
+    if (few) __syncwarp(); else __syncthreads();
+    if (few || warp == 0) {
+        if (p.every_chunk) {
+            cell = p.min_units;
+        } else {
+            int units = 0, segments = 0;
+            for (int b = lane; b < a.batch; b += 32) {
+                const int n = units_of(s_len[b]);
+                units += n;
+                segments += n > 0;
+            }
+            units = __reduce_add_sync(0xffffffffu, units) * heads_tiles;
+            segments = __reduce_add_sync(0xffffffffu, segments) * heads_tiles;
+            share = max(p.min_units, (units + grid - 1) / grid);  // equal ranges of the line
+            if (2 * segments <= grid) {
+                // Few segments: each is cut into chunks of its own, one per CTA,
+                // so that a CTA works on one segment.  Eight sizes between the
+                // equal range and the one that must fit, four lanes on each; the
+                // smallest with which the grid holds all chunks is taken.
+                const int fits = max(share, (units + grid - segments - 1) / (grid - segments));
+                const int mine = share + (fits - share) * (lane >> 2) / 7;
+                int chunks = 0;
+                for (int b = lane & 3; b < a.batch; b += 4)
+                    chunks += (int)(((unsigned)units_of(s_len[b]) + mine - 1) / (unsigned)mine);
+                chunks += __shfl_xor_sync(0xffffffffu, chunks, 1);
+                chunks += __shfl_xor_sync(0xffffffffu, chunks, 2);
+                const uint32_t ok = __ballot_sync(0xffffffffu, chunks * heads_tiles <= grid);
+                cell = __shfl_sync(0xffffffffu, mine, __ffs(ok | 0x80000000u) - 1);
+                share = 1;
+            }
+        }
+        int before = 0;
+        for (int b0 = 0; b0 < a.batch; b0 += 32) {
+            const int b = b0 + lane;
+            int n = b < a.batch ? units_of(s_len[b]) : 0;
+            if (cell > 1) n = (int)((unsigned)(n + cell - 1) / (unsigned)cell);
+            int scan = n;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int v = __shfl_up_sync(0xffffffffu, scan, o);
+                if (lane >= o) scan += v;
+            }
+            if (b < a.batch) s_cum[b] = before + scan - n;
+            before += __shfl_sync(0xffffffffu, scan, 31);
+        }
+        if (lane == 0) s_cum[a.batch] = before, flag[1] = cell, flag[2] = share;
+    }
+    if (few) {
+        __syncwarp();
+    } else {
+        __syncthreads();
+        cell = flag[1];
+        share = flag[2];
+    }
+    const bool chunked = cell > 1;
+    const int total = s_cum[a.batch] * heads_tiles;
 
-    // Row `r` of a tile of sequence `seq`: where it is in q and in the outputs.
+    // Row `r` of a tile of sequence `seq`: where it is in the outputs.
     auto out_row = [&](int seq, int head, int r) {
-        return ((int64_t)seq * a.new_tokens + r / a.group) * (a.kv_heads * a.group) +
-               head * a.group + r % a.group;
+        const int i = p.group.div(r);
+        return ((int64_t)seq * a.new_tokens + i) * (a.kv_heads * a.group) + (head - i) * a.group + r;
     };
     // One normalised output: 4 elements d.. of row `row`; `front` joins the
     // result over the tokens in front.
@@ -259,7 +321,7 @@ __global__ void __launch_bounds__(kThreads, kDim == 256 ? 2 : 3)
     };
 
     // Sequences with nothing to read (their rows see no cached token).
-    for (int b = blockIdx.x; b < a.batch; b += gridDim.x) {
+    for (int b = blockIdx.x; b < a.batch; b += grid) {
         if (s_cum[b + 1] != s_cum[b]) continue;
         const int n = rows * a.kv_heads * (kDim / 4);
         for (int i = tid; i < n; i += kThreads) {
@@ -268,122 +330,174 @@ __global__ void __launch_bounds__(kThreads, kDim == 256 ? 2 : 3)
                       -INFINITY, 0.f, d == 0);
         }
     }
-    if (u0 >= u1) return;
+    const int x0 = (int)min((int64_t)total, (int64_t)blockIdx.x * share);
+    const int x1 = min(total, x0 + share);
+    if (x0 >= x1) return;
 
-    // First segment of the range.
-    Cursor start;
+    // The CTA's range [u0, u1) and its first segment.  Chunked, the line is the
+    // units of the one segment; else the units of all segments.
+    Segment start;
+    int u0 = x0, u1 = x1, c0 = 0, parts = 0;  // chunked: first CTA and CTAs of the segment
     {
-        int lo = 0, hi = a.batch;  // last sequence whose blocks begin at or before u0
+        int lo = 0, hi = a.batch;  // last sequence whose cells begin at or before x0
         while (hi - lo > 1) {
             const int mid = (lo + hi) >> 1;
-            if (s_cum[mid] <= u0 / units) lo = mid; else hi = mid;
+            if (s_cum[mid] * heads_tiles <= x0) lo = mid; else hi = mid;
         }
+        const int cells = s_cum[lo + 1] - s_cum[lo], in = x0 - s_cum[lo] * heads_tiles;
         start.seq = lo;
-        start.blocks = s_cum[lo + 1] - s_cum[lo];
-        const int in = u0 - s_cum[lo] * units;
-        start.unit = in / start.blocks;
-        start.seg0 = s_cum[lo] * units + start.unit * start.blocks;
+        start.part = in / cells;
+        start.units = cells;
+        start.begin = s_cum[lo] * heads_tiles + start.part * cells;
+        if (chunked) {
+            const int chunk = in - start.part * cells;
+            c0 = (int)blockIdx.x - chunk;
+            parts = cells;
+            start.begin = 0;
+            start.units = units_of(s_len[lo]);
+            u0 = chunk * cell;
+            u1 = min(u0 + cell, start.units);
+        }
     }
-    auto next_segment = [&](Cursor& c) {
-        c.seg0 += c.blocks;
-        if (++c.unit == units) {
-            c.unit = 0;
+    auto next_segment = [&](Segment& c) {
+        c.begin += c.units;
+        if (++c.part == heads_tiles) {
+            c.part = 0;
             do ++c.seq; while (c.seq < a.batch && s_cum[c.seq + 1] == s_cum[c.seq]);
-            if (c.seq < a.batch) c.blocks = s_cum[c.seq + 1] - s_cum[c.seq];
+            if (c.seq < a.batch) c.units = s_cum[c.seq + 1] - s_cum[c.seq];  // not chunked
         }
     };
 
-    // The warp's copies run kStages blocks ahead of its arithmetic.  The page
-    // of a copy is loaded one step before the copy is issued.
-    const uint64_t policy = policy_evict_first();
-    const int64_t head_bytes = (int64_t)p.blocks_per_page * kBlockBytes;
-    Cursor ic = start;   // segment of the next copy
-    int iu = u0 + warp;  // its block
-    int page = 0, sub = 0;
-    auto load_page = [&]() {
-        if (iu >= u1) return;
-        while (iu >= ic.seg0 + ic.blocks) next_segment(ic);
-        const int blk = iu - ic.seg0 + first_block(s_len[ic.seq]);
-        const int n = (int)__umulhi((uint32_t)blk, p.page_magic);
-        const int index = p.blocks_per_page == 1 ? blk : n;
-        sub = blk - index * p.blocks_per_page;
-        page = __ldg(a.table + ic.seq * a.table_stride + index);
-    };
-    uint32_t bad = 0;      // stages whose block has no valid page
-    uint32_t pending = 0;  // stages with a copy that nothing has waited for
-    auto issue = [&](int stage) {
-        if (iu >= u1) return;
-        const bool ok = page >= 0 && page < a.num_pages;
-        bad = ok ? bad & ~(1u << stage) : bad | (1u << stage);
-        pending |= (uint32_t)ok << stage;
-        if (lane == 0) {
-            if (ok) {
-                const uint32_t bar = my_bars + 8 * stage;
-                mbar_arrive_expect_tx(bar, kBlockBytes);
-                const uint8_t* src = a.pages +
-                                     ((int64_t)page * a.kv_heads + ic.unit / p.row_tiles) * head_bytes +
-                                     (int64_t)sub * kBlockBytes;
-                bulk_g2s(my_ring + stage * kBlockBytes, src, kBlockBytes, bar, policy);
-            } else {
-                atomicCAS(&g_kv_attention_status, 0, kStatusKvIndex);
-            }
-        }
-        iu += kWarps;
-    };
-    load_page();
-#pragma unroll 1
-    for (int i = 0; i < kStages; ++i) {
-        issue(i);
-        load_page();
-    }
-
-    // Byte offsets of this lane's pieces inside a K part and a V part.
+    // q of a segment's rows g + 8 n, this lane's pieces, as stored.
     constexpr int kKWords = kRow / 16, kKPer = kKWords < 4 ? kKWords : 4;
     constexpr int kVWords = kRow / 32, kVPer = kVWords < 4 ? kVWords : 4;
-    auto k_byte = [&](int i) {  // i-th access of a quarter row
+    constexpr int kKAccess = kKWords / kKPer, kVAccess = kVWords / kVPer;
+    auto k_byte = [&](int i) {  // byte offset of the i-th access of a quarter row
         return kRow == 256 ? (i >> 1) * 128 + 32 * t + 16 * (i & 1)
                            : kRow == 128 ? 32 * t + 16 * i : (kRow / 4) * t;
     };
-    auto v_byte = [&](int i) { return kRow == 256 ? 128 * i + 16 * g : (kRow / 8) * g; };
+    uint4 qraw[kNB][kDim / 32];
+    auto load_q = [&](const Segment& c) {
+        const int head = p.row_tiles.div(c.part), first = p.row_tiles.mod(c.part) * S::kCols;
+#pragma unroll
+        for (int n = 0; n < kNB; ++n) {
+            const int r = first + 8 * n + g;
+            const int i0 = p.group.div(r);
+            const uint16_t* at = static_cast<const uint16_t*>(a.q) + c.seq * a.q_batch +
+                                 i0 * a.q_new + ((head - i0) * a.group + r) * a.q_head;
+            constexpr int kElements = kKPer * 32 / kBits;  // of an access of the cache
+#pragma unroll
+            for (int i = 0; i < kDim / 32; ++i) {
+                qraw[n][i] = make_uint4(0, 0, 0, 0);
+                const int e = k_byte(8 * i / kElements) * 8 / kBits + 8 * i % kElements;
+                if (r < rows)
+                    qraw[n][i] = p.q_vec ? load8<kBf16, true>(at, e) : load8<kBf16, false>(at, e);
+            }
+        }
+    };
+    load_q(start);
 
-    int stage = 0, phase = 0;
+    // The warp's copies run kStages units ahead of its arithmetic.  The blocks
+    // are looked up 32 units at a time, one unit per lane, and the lane that
+    // holds a unit issues its copies, so the walk over segments and pages costs
+    // a step a compare.
+    constexpr uint32_t kAbsent = 0xffffffffu, kInvalid = 0xfffffffeu;
+    const uint64_t policy = policy_evict_first();
+    auto look_up = [&](int u, int seq, uint32_t (&at)[kU]) {
+#pragma unroll
+        for (int k = 0; k < kU; ++k) at[k] = kAbsent;
+        if (u >= u1) return;
+        int part = start.part, in = u;
+        if (!chunked) {
+            int hi = a.batch;
+            while (hi - seq > 1) {
+                const int mid = (seq + hi) >> 1;
+                if (s_cum[mid] * heads_tiles <= u) seq = mid; else hi = mid;
+            }
+            const int units = s_cum[seq + 1] - s_cum[seq];
+            in = u - s_cum[seq] * heads_tiles;
+            part = in / units;
+            in -= part * units;
+        }
+        const int len = s_len[seq];
+        const uint32_t head = p.row_tiles.div(part);
+#pragma unroll
+        for (int k = 0; k < kU; ++k) {
+            const int blk = in * kU + k + first_block(len);
+            if (k > 0 && blk * kKvBlock >= len) break;
+            const int index = p.page_blocks.div(blk);
+            const int page = __ldg(a.table + seq * a.table_stride + index);
+            if (page < 0 || page >= a.num_pages) {
+                atomicCAS(&g_kv_attention_status, 0, kStatusKvIndex);
+                at[k] = kInvalid;
+            } else {
+                at[k] = ((uint32_t)page * a.kv_heads + head) * p.page_blocks.d +
+                        (blk - index * p.page_blocks.d);
+            }
+        }
+    };
+    auto copy = [&](int stage, const uint32_t (&at)[kU]) {
+        const uint32_t bar = my_bars + 8 * stage, to = smem_u32(my_ring) + stage * kStageBytes;
+        if (kU == 2 && at[0] < kInvalid && at[kU - 1] == at[0] + 1) {  // one stretch of memory
+            mbar_arrive_expect_tx(bar, kStageBytes);
+            bulk_g2s(to, a.pages + (int64_t)at[0] * kBlockBytes, kStageBytes, bar, policy);
+            return;
+        }
+        uint32_t bytes = 0;
+#pragma unroll
+        for (int k = 0; k < kU; ++k) bytes += at[k] < kInvalid ? kBlockBytes : 0;
+        mbar_arrive_expect_tx(bar, bytes);  // none: the phase completes at once
+#pragma unroll
+        for (int k = 0; k < kU; ++k)
+            if (at[k] < kInvalid)
+                bulk_g2s(to + k * kBlockBytes, a.pages + (int64_t)at[k] * kBlockBytes, kBlockBytes,
+                         bar, policy);
+    };
+    int issued = kStages, done = 0;  // of this warp's units
+    const int mine = u0 + warp < u1 ? (u1 - u0 - warp + kWarps - 1) / kWarps : 0;
+    uint32_t at[kU];
+    look_up(u0 + warp + kWarps * lane, start.seq, at);
+    // units with an invalid page, of the batch in use and of the one being issued
+    uint32_t bad[kU], bad_next[kU];
+#pragma unroll
+    for (int k = 0; k < kU; ++k) bad[k] = bad_next[k] = __ballot_sync(0xffffffffu, at[k] == kInvalid);
+    if (lane < min(kStages, mine)) copy(lane, at);
+
+    // Places of this lane's pieces inside a block.
+    int k_at[kKAccess], v_at[2][kVAccess];
+#pragma unroll
+    for (int i = 0; i < kKAccess; ++i) k_at[i] = kv_offset<kRow>(g, k_byte(i));
+#pragma unroll
+    for (int i = 0; i < kVAccess; ++i)
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+            v_at[x][i] = kKvBlock * kRow +
+                         kv_offset<kRow>(2 * t + x, kRow == 256 ? 128 * i + 16 * g : (kRow / 8) * g);
+    const int scale_at = 2 * kKvBlock * kRow + 2 * g;
+
+    int stage = 0;
+    uint32_t phase = 0;
     bool failed = false;
     int cu = u0 + warp;
-    Cursor seg = start;
-    while (seg.seg0 < u1) {
-        const int sa = max(seg.seg0, u0), sb = min(seg.seg0 + seg.blocks, u1);
-        const int head = seg.unit / p.row_tiles, tile = seg.unit % p.row_tiles;
-        const int len = s_len[seg.seq], row0 = tile * S::kCols;
-        const int block0 = first_block(len) - seg.seg0;
+    Segment seg = start;
+    while (seg.begin < u1) {
+        const int sa = max(seg.begin, u0), sb = min(seg.begin + seg.units, u1);
+        const int head = p.row_tiles.div(seg.part), row0 = p.row_tiles.mod(seg.part) * S::kCols;
+        const int len = s_len[seg.seq];
+        const int token0 = first_block(len) * kKvBlock - seg.begin * (kU * kKvBlock);
 
-        // q of this lane's rows g + 8 n as B fragments.  bf16 rows are brought
-        // into fp16's range by a power of two (exact; elements 2^14 below
-        // their row's largest lose bits that fp32 sums would not keep either).
+        // q as B fragments.  bf16 rows are brought into fp16's range by a power
+        // of two (exact; elements 2^14 below their row's largest lose bits that
+        // fp32 sums would not keep either).
         uint32_t qf[kNB][kSteps][2];
         float rs[kNB][2];
 #pragma unroll
         for (int n = 0; n < kNB; ++n) {
-            const int r = row0 + 8 * n + g;
             float x[kDim / 4];
 #pragma unroll
-            for (int i = 0; i < kDim / 4; ++i) x[i] = 0.f;
-            if (r < rows) {
-                const uint16_t* src = static_cast<const uint16_t*>(a.q) + seg.seq * a.q_batch +
-                                      r / a.group * a.q_new +
-                                      (head * a.group + r % a.group) * a.q_head;
-                // piece i: the elements of access i, 16 bytes of q at a time
-                constexpr int kAccess = kKPer * 32 / kBits;  // elements per access
-#pragma unroll
-                for (int i = 0; i < kKWords / kKPer; ++i) {
-                    const int e0 = k_byte(i) * 8 / kBits;
-#pragma unroll
-                    for (int j = 0; j < kAccess; j += 8)
-                        unpack8<kBf16>(p.q_vec ? load8<kBf16, true>(src, e0 + j)
-                                               : load8<kBf16, false>(src, e0 + j),
-                                       x + i * kAccess + j);
-                }
-            }
+            for (int i = 0; i < kDim / 32; ++i) unpack8<kBf16>(qraw[n][i], x + 8 * i);
             float unit = a.scale * 1.4426950408889634f;
+            rs[n][0] = rs[n][1] = unit;
             if (kBf16) {
                 float m = 0.f;
 #pragma unroll
@@ -398,9 +512,9 @@ __global__ void __launch_bounds__(kThreads, kDim == 256 ? 2 : 3)
                     for (int i = 0; i < kDim / 4; ++i) x[i] *= down;
                     unit *= __uint_as_float((uint32_t)(127 + e) << 23);
                 }
+                rs[n][0] = __shfl_sync(0xffffffffu, unit, 8 * t);
+                rs[n][1] = __shfl_sync(0xffffffffu, unit, 8 * t + 4);
             }
-            rs[n][0] = __shfl_sync(0xffffffffu, unit, 8 * t);
-            rs[n][1] = __shfl_sync(0xffffffffu, unit, 8 * t + 4);
 #pragma unroll
             for (int w = 0; w < kKWords; ++w) {
                 if (kBits == 8) {
@@ -414,108 +528,128 @@ __global__ void __launch_bounds__(kThreads, kDim == 256 ? 2 : 3)
                 }
             }
         }
-        // Tokens [lo, hi) that the rows 2t, 2t + 1 (+ 8 n) see.
-        int hi[kNB][2], lo[kNB][2];
-#pragma unroll
-        for (int n = 0; n < kNB; ++n)
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                const int r = row0 + 8 * n + 2 * t + c;
-                const int at = len - a.new_tokens + r / a.group + 1;
-                hi[n][c] = a.causal ? min(at, len) : len;
-                lo[n][c] = a.window > 0 ? at - a.window : 0;
-            }
+        // Tokens [lo, hi) that every row of the sequence sees.
         const int all_hi = a.causal ? len - a.new_tokens + 1 : len;
         const int all_lo = a.window > 0 ? len - a.window : 0;
 
         float o[kSteps][kNB][4];
-        float m[kNB][2], l[kNB][2];
+        // the reference, 0 in its place while it is -inf, and what a score may reach under it
+        float m[kNB][2], ref[kNB][2], limit[kNB][2], l[kNB][2];
 #pragma unroll
         for (int n = 0; n < kNB; ++n) {
 #pragma unroll
             for (int i = 0; i < kSteps; ++i) o[i][n][0] = o[i][n][1] = o[i][n][2] = o[i][n][3] = 0.f;
-            m[n][0] = m[n][1] = -INFINITY;
-            l[n][0] = l[n][1] = 0.f;
+            m[n][0] = m[n][1] = limit[n][0] = limit[n][1] = -INFINITY;
+            l[n][0] = l[n][1] = ref[n][0] = ref[n][1] = 0.f;
         }
 
 #pragma unroll 1
         for (; cu < sb; cu += kWarps) {
-            const bool have = !((bad >> stage) & 1u) && !failed;
-            if (have && !mbar_wait_bounded(my_bars + 8 * stage, (uint32_t)phase >> stage & 1u,
-                                           p.wait_cycles)) {
-                if (lane == 0) atomicCAS(&g_kv_attention_status, 0, kStatusTimeoutKv);
-                failed = true;
+            // every lane leaves the wait with the same answer
+            if (!failed && !__all_sync(0xffffffffu, mbar_try_wait(my_bars + 8 * stage, phase >> stage & 1u))) {
+                const long long t0 = clock64();
+                while (!__all_sync(0xffffffffu, mbar_try_wait(my_bars + 8 * stage, phase >> stage & 1u))) {
+                    failed = __any_sync(0xffffffffu, clock64() - t0 > p.wait_cycles);
+                    if (failed) break;
+                }
+                if (failed && lane == 0) atomicCAS(&g_kv_attention_status, 0, kStatusTimeoutKv);
             }
-            failed = __any_sync(0xffffffffu, failed);
-            if (have && !failed) {
-                phase ^= 1 << stage;
-                pending &= ~(1u << stage);
-                const uint32_t base = my_ring + stage * kBlockBytes;
-                const int j0 = (cu + block0) * kKvBlock;
-                float s[kNB][4];
+            if (!failed) {
+                phase ^= 1u << stage;
+                const uint8_t* base = my_ring + stage * kStageBytes;
+                float s[kU][kNB][4];
 #pragma unroll
-                for (int n = 0; n < kNB; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+                for (int k = 0; k < kU; ++k)
 #pragma unroll
-                for (int i = 0; i < kKWords / kKPer; ++i) {
-                    uint32_t w0[kKPer], w1[kKPer];
-                    lds_words<kKPer>(base + kv_offset<kRow>(g, k_byte(i)), w0);
-                    lds_words<kKPer>(base + kv_offset<kRow>(g + 8, k_byte(i)), w1);
+                    for (int n = 0; n < kNB; ++n) s[k][n][0] = s[k][n][1] = s[k][n][2] = s[k][n][3] = 0.f;
 #pragma unroll
-                    for (int w = 0; w < kKPer; ++w) {
-                        const int x = i * kKPer + w;
-                        if (kBits == 8) {
-                            const uint32_t f[4] = {bytes02(w0[w]), bytes02(w1[w]),
-                                                   bytes02(w0[w] >> 8), bytes02(w1[w] >> 8)};
+                for (int i = 0; i < kKAccess; ++i)
 #pragma unroll
-                            for (int n = 0; n < kNB; ++n) mma_16816(s[n], f, qf[n][x][0], qf[n][x][1]);
-                        } else {
-                            const uint32_t e[4] = {nibbles04(w0[w]), nibbles04(w1[w]),
-                                                   nibbles15(w0[w]), nibbles15(w1[w])};
-                            const uint32_t h0 = w0[w] >> 8, h1 = w1[w] >> 8;
-                            const uint32_t f[4] = {nibbles04(h0), nibbles04(h1), nibbles15(h0),
-                                                   nibbles15(h1)};
+                    for (int k = 0; k < kU; ++k) {
+                        const uint8_t* kb = base + k * kBlockBytes + k_at[i];
+                        uint32_t w0[kKPer], w1[kKPer];
+                        lds_words<kKPer>(kb, w0);
+                        lds_words<kKPer>(kb + 8 * kRow, w1);
 #pragma unroll
-                            for (int n = 0; n < kNB; ++n) {
-                                mma_16816(s[n], e, qf[n][2 * x][0], qf[n][2 * x][1]);
-                                mma_16816(s[n], f, qf[n][2 * x + 1][0], qf[n][2 * x + 1][1]);
+                        for (int w = 0; w < kKPer; ++w) {
+                            const int x = i * kKPer + w;
+                            if (kBits == 8) {
+                                const uint32_t f[4] = {bytes02(w0[w]), bytes02(w1[w]),
+                                                       bytes02(w0[w] >> 8), bytes02(w1[w] >> 8)};
+#pragma unroll
+                                for (int n = 0; n < kNB; ++n)
+                                    mma_16816(s[k][n], f, qf[n][x][0], qf[n][x][1]);
+                            } else {
+                                const uint32_t e[4] = {nibbles04(w0[w]), nibbles04(w1[w]),
+                                                       nibbles15(w0[w]), nibbles15(w1[w])};
+                                const uint32_t h0 = w0[w] >> 8, h1 = w1[w] >> 8;
+                                const uint32_t f[4] = {nibbles04(h0), nibbles04(h1), nibbles15(h0),
+                                                       nibbles15(h1)};
+#pragma unroll
+                                for (int n = 0; n < kNB; ++n) {
+                                    mma_16816(s[k][n], e, qf[n][2 * x][0], qf[n][2 * x][1]);
+                                    mma_16816(s[k][n], f, qf[n][2 * x + 1][0], qf[n][2 * x + 1][1]);
+                                }
                             }
                         }
                     }
-                }
-                // Scores of tokens j0 + g (0, 1) and j0 + g + 8 (2, 3).
-                const uint32_t scales = base + 2 * kKvBlock * kRow + 2 * g;
-                const float ks0 = lds_half(scales), ks1 = lds_half(scales + 16);
-                // V scales; a zero scale has all-zero values, any weight will do
-                const float lv0 = fmaxf(lg2(lds_half(scales + 32)), -24.f);
-                const float lv1 = fmaxf(lg2(lds_half(scales + 48)), -24.f);
+                // Scores of tokens j0 + g (0, 1) and j0 + g + 8 (2, 3) of each block,
+                // log2 of V's scale added (a zero scale has all-zero values: any will do).
+                float iv[kU][2];
                 bool over = false;
 #pragma unroll
-                for (int n = 0; n < kNB; ++n) {
-                    s[n][0] = fmaf(s[n][0] * ks0, rs[n][0], lv0);
-                    s[n][1] = fmaf(s[n][1] * ks0, rs[n][1], lv0);
-                    s[n][2] = fmaf(s[n][2] * ks1, rs[n][0], lv1);
-                    s[n][3] = fmaf(s[n][3] * ks1, rs[n][1], lv1);
+                for (int k = 0; k < kU; ++k) {
+                    const uint8_t* sc = base + k * kBlockBytes + scale_at;
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const float ks = lds_half(sc + 16 * h);
+                        const float lv = fmaxf(lg2(lds_half(sc + 32 + 16 * h)), -24.f);
+                        iv[k][h] = ex2(-lv);  // finite whatever a masked token's scale holds
+#pragma unroll
+                        for (int n = 0; n < kNB; ++n)
+#pragma unroll
+                            for (int c = 0; c < 2; ++c)
+                                s[k][n][2 * h + c] = fmaf(s[k][n][2 * h + c], ks * rs[n][c], lv);
+                    }
                 }
-                if (j0 + kKvBlock > all_hi || j0 < all_lo) {
+                const int j0 = cu * (kU * kKvBlock) + token0;
+                bool cut = j0 + kU * kKvBlock > all_hi || j0 < all_lo;
+#pragma unroll
+                for (int k = 0; k < kU; ++k) cut |= (bad[k] >> (done & 31)) & 1u;
+                if (cut) {
 #pragma unroll
                     for (int n = 0; n < kNB; ++n)
 #pragma unroll
-                        for (int c = 0; c < 4; ++c) {
-                            const int j = j0 + g + 8 * (c >> 1);
-                            if (j >= hi[n][c & 1] || j < lo[n][c & 1]) s[n][c] = -INFINITY;
+                        for (int c = 0; c < 2; ++c) {
+                            const int r = row0 + 8 * n + 2 * t + c;
+                            const int end = len - a.new_tokens + p.group.div(r) + 1;
+                            const int hi = a.causal ? min(end, len) : len;
+                            const int lo = a.window > 0 ? end - a.window : 0;
+#pragma unroll
+                            for (int k = 0; k < kU; ++k)
+#pragma unroll
+                                for (int h = 0; h < 2; ++h) {
+                                    const int j = j0 + k * kKvBlock + g + 8 * h;
+                                    if (j >= hi || j < lo || ((bad[k] >> (done & 31)) & 1u))
+                                        s[k][n][2 * h + c] = -INFINITY;
+                                }
                         }
                 }
 #pragma unroll
-                for (int n = 0; n < kNB; ++n) {
-                    over |= fmaxf(s[n][0], s[n][2]) > m[n][0] + kSlack;
-                    over |= fmaxf(s[n][1], s[n][3]) > m[n][1] + kSlack;
-                }
+                for (int k = 0; k < kU; ++k)
+#pragma unroll
+                    for (int n = 0; n < kNB; ++n) {
+                        over |= fmaxf(s[k][n][0], s[k][n][2]) > limit[n][0];
+                        over |= fmaxf(s[k][n][1], s[k][n][3]) > limit[n][1];
+                    }
                 if (__any_sync(0xffffffffu, over)) {
 #pragma unroll
                     for (int n = 0; n < kNB; ++n)
 #pragma unroll
                         for (int c = 0; c < 2; ++c) {
-                            float top = fmaxf(s[n][c], s[n][c + 2]);
+                            float top = fmaxf(s[0][n][c], s[0][n][c + 2]);
+                            if (kU == 2)
+                                top = fmaxf(top, fmaxf(s[kU - 1][n][c], s[kU - 1][n][c + 2]));
 #pragma unroll
                             for (int x = 4; x < 32; x <<= 1)
                                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
@@ -523,6 +657,8 @@ __global__ void __launch_bounds__(kThreads, kDim == 256 ? 2 : 3)
                             // a row that has seen nothing keeps -inf and zeros
                             const float f = top == -INFINITY ? 1.f : ex2(m[n][c] - top);
                             m[n][c] = top;
+                            ref[n][c] = top == -INFINITY ? 0.f : top;
+                            limit[n][c] = top + kSlack;
                             l[n][c] *= f;
 #pragma unroll
                             for (int i = 0; i < kSteps; ++i) {
@@ -531,190 +667,221 @@ __global__ void __launch_bounds__(kThreads, kDim == 256 ? 2 : 3)
                             }
                         }
                 }
-                const float iv0 = ex2(-lv0), iv1 = ex2(-lv1);
-                uint32_t pf[kNB][2];
+                uint32_t pf[kU][kNB][2];
 #pragma unroll
-                for (int n = 0; n < kNB; ++n) {
-                    const float r0 = m[n][0] == -INFINITY ? 0.f : m[n][0];
-                    const float r1 = m[n][1] == -INFINITY ? 0.f : m[n][1];
-                    const float w0 = ex2(s[n][0] - r0), w1 = ex2(s[n][1] - r1);
-                    const float w2 = ex2(s[n][2] - r0), w3 = ex2(s[n][3] - r1);
-                    // masked tokens may hold any scale: 0 * inf must not reach the sum
-                    l[n][0] += (s[n][0] == -INFINITY ? 0.f : w0 * iv0) +
-                               (s[n][2] == -INFINITY ? 0.f : w2 * iv1);
-                    l[n][1] += (s[n][1] == -INFINITY ? 0.f : w1 * iv0) +
-                               (s[n][3] == -INFINITY ? 0.f : w3 * iv1);
-                    pf[n][0] = transpose8x8(pack2<false>(w0, w1));
-                    pf[n][1] = transpose8x8(pack2<false>(w2, w3));
-                }
-                // O^T += V^T P^T: tokens 2t, 2t + 1, 2t + 8, 2t + 9.
-                const uint32_t vb = base + kKvBlock * kRow;
+                for (int k = 0; k < kU; ++k)
 #pragma unroll
-                for (int i = 0; i < kVWords / kVPer; ++i) {
-                    uint32_t w[4][kVPer];
+                    for (int n = 0; n < kNB; ++n)
 #pragma unroll
-                    for (int x = 0; x < 4; ++x)
-                        lds_words<kVPer>(
-                            vb + kv_offset<kRow>(2 * t + (x & 1) + 8 * (x >> 1), v_byte(i)), w[x]);
+                        for (int h = 0; h < 2; ++h) {
+                            const float w0 = ex2(s[k][n][2 * h] - ref[n][0]);
+                            const float w1 = ex2(s[k][n][2 * h + 1] - ref[n][1]);
+                            l[n][0] = fmaf(w0, iv[k][h], l[n][0]);
+                            l[n][1] = fmaf(w1, iv[k][h], l[n][1]);
+                            pf[k][n][h] = transpose8x8(pack2<false>(w0, w1));
+                        }
+                // O^T += V^T P^T: tokens 2t, 2t + 1, 2t + 8, 2t + 9 of each block.
 #pragma unroll
-                    for (int y = 0; y < kVPer; ++y)
+                for (int k = 0; k < kU; ++k)
 #pragma unroll
-                        for (int h = 0; h < 2; ++h) {  // low and high half of the words
-                            const uint32_t c0 = h ? prmt_i<0x7632u>(w[0][y], w[1][y])
-                                                  : prmt_i<0x5410u>(w[0][y], w[1][y]);
-                            const uint32_t c1 = h ? prmt_i<0x7632u>(w[2][y], w[3][y])
-                                                  : prmt_i<0x5410u>(w[2][y], w[3][y]);
-                            const int x = 2 * (i * kVPer + y) + h;
-                            if (kBits == 8) {
-                                const uint32_t f[4] = {bytes02(c0), bytes02(c0 >> 8), bytes02(c1),
-                                                       bytes02(c1 >> 8)};
+                    for (int i = 0; i < kVAccess; ++i) {
+                        const uint8_t* vb = base + k * kBlockBytes;
+                        uint32_t w[4][kVPer];
 #pragma unroll
-                                for (int n = 0; n < kNB; ++n) mma_16816(o[x][n], f, pf[n][0], pf[n][1]);
-                            } else {
-                                const uint32_t d0 = c0 >> 8, d1 = c1 >> 8;
-                                const uint32_t e[4] = {nibbles04(c0), nibbles15(c0), nibbles04(c1),
-                                                       nibbles15(c1)};
-                                const uint32_t f[4] = {nibbles04(d0), nibbles15(d0), nibbles04(d1),
-                                                       nibbles15(d1)};
+                        for (int x = 0; x < 4; ++x)
+                            lds_words<kVPer>(vb + v_at[x & 1][i] + (x >> 1) * 8 * kRow, w[x]);
 #pragma unroll
-                                for (int n = 0; n < kNB; ++n) {
-                                    mma_16816(o[2 * x][n], e, pf[n][0], pf[n][1]);
-                                    mma_16816(o[2 * x + 1][n], f, pf[n][0], pf[n][1]);
+                        for (int y = 0; y < kVPer; ++y)
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) {  // low and high half of the words
+                                const uint32_t d0 = h ? prmt_i<0x7632u>(w[0][y], w[1][y])
+                                                      : prmt_i<0x5410u>(w[0][y], w[1][y]);
+                                const uint32_t d1 = h ? prmt_i<0x7632u>(w[2][y], w[3][y])
+                                                      : prmt_i<0x5410u>(w[2][y], w[3][y]);
+                                const uint32_t e0 = d0 >> 8, e1 = d1 >> 8;
+                                const int x = 2 * (i * kVPer + y) + h;
+                                if (kBits == 8) {
+                                    const uint32_t f[4] = {bytes02(d0), bytes02(e0), bytes02(d1),
+                                                           bytes02(e1)};
+#pragma unroll
+                                    for (int n = 0; n < kNB; ++n)
+                                        mma_16816(o[x][n], f, pf[k][n][0], pf[k][n][1]);
+                                } else {
+                                    const uint32_t e[4] = {nibbles04(d0), nibbles15(d0),
+                                                           nibbles04(d1), nibbles15(d1)};
+                                    const uint32_t f[4] = {nibbles04(e0), nibbles15(e0),
+                                                           nibbles04(e1), nibbles15(e1)};
+#pragma unroll
+                                    for (int n = 0; n < kNB; ++n) {
+                                        mma_16816(o[2 * x][n], e, pf[k][n][0], pf[k][n][1]);
+                                        mma_16816(o[2 * x + 1][n], f, pf[k][n][0], pf[k][n][1]);
+                                    }
                                 }
                             }
-                        }
+                    }
+                __syncwarp();  // every lane has read the stage before it is filled again
+                if (issued < mine) {
+                    const int i = issued & 31;
+                    if (i == 0) {
+                        look_up(u0 + warp + kWarps * (issued + lane), seg.seq, at);
+#pragma unroll
+                        for (int k = 0; k < kU; ++k)
+                            bad_next[k] = __ballot_sync(0xffffffffu, at[k] == kInvalid);
+                    }
+                    if (lane == i) copy(stage, at);
+                    ++issued;
                 }
-            }
-            __syncwarp();  // every lane has read the stage before it is filled again
-            if (!failed) {
-                issue(stage);
-                load_page();
+                if ((++done & 31) == 0) {
+#pragma unroll
+                    for (int k = 0; k < kU; ++k) bad[k] = bad_next[k];
+                }
             }
             stage = stage + 1 == kStages ? 0 : stage + 1;
         }
 
         // ---- the segment's end: the warps' results meet in shared memory ----
-#pragma unroll
-        for (int n = 0; n < kNB; ++n)
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-#pragma unroll
-                for (int x = 4; x < 32; x <<= 1) l[n][c] += __shfl_xor_sync(0xffffffffu, l[n][c], x);
-                if (g == 0) {
-                    const int col = 8 * n + 2 * t + c;
-                    stat[(warp * S::kCols + col) * 2] = m[n][c];
-                    stat[(warp * S::kCols + col) * 2 + 1] = l[n][c];
-                }
-            }
-        const bool whole = sa == seg.seg0 && sb == seg.seg0 + seg.blocks;
-        float* slot = p.partial + ((int64_t)blockIdx.x * 2 + (seg.seg0 >= u0)) * kPartialFloats;
+        // Value v of a lane: 4 elements of row 2t + v / (kSteps / 2) (+ 8 n),
+        // stored lane by lane; warp w joins and writes the values w, w + 4, ...
+        const Segment now = seg;
+        next_segment(seg);
+        const bool whole = sa == now.begin && sb == now.begin + now.units;
+        float* slot = p.partial + ((int64_t)blockIdx.x * 2 + (now.begin >= u0)) * kPartialFloats;
+        auto value_row = [&](int v) { return 2 * t + v / (kSteps / 2); };
+        auto value_d = [&](int v) {
+            const int i = v % (kSteps / 2) * 2;  // its first 16-row block of O^T
+            return kRow == 256 ? (i / 8) * 128 + 16 * g + 2 * (i % 8) : (kDim / 8) * g + 2 * i;
+        };
 #pragma unroll
         for (int n = 0; n < kNB; ++n) {
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                float* dst = red + (warp * 8 + 2 * t + c) * kDim;
-                // element of (block i, half h): contiguous in the lane's eighth of the row
 #pragma unroll
-                for (int i = 0; i < kSteps; i += 2) {
-                    const int d = kRow == 256 ? (i / 8) * 128 + 16 * g + 2 * (i % 8)
-                                              : (kDim / 8) * g + 2 * i;
-                    *reinterpret_cast<float4*>(dst + d) = make_float4(
-                        o[i][n][c], o[i][n][c + 2], o[i + 1][n][c], o[i + 1][n][c + 2]);
-                }
+                for (int x = 4; x < 32; x <<= 1) l[n][c] += __shfl_xor_sync(0xffffffffu, l[n][c], x);
+                if (g == 0)
+                    *reinterpret_cast<float2*>(stat + (warp * S::kCols + 8 * n + 2 * t + c) * 2) =
+                        make_float2(m[n][c], l[n][c]);
+#pragma unroll
+                for (int i = 0; i < kSteps; i += 2)
+                    reinterpret_cast<float4*>(red)[(warp * kSteps + c * (kSteps / 2) + i / 2) * 32 + lane] =
+                        make_float4(o[i][n][c], o[i][n][c + 2], o[i + 1][n][c], o[i + 1][n][c + 2]);
             }
             __syncthreads();
-            for (int i = tid; i < 8 * (kDim / 4); i += kThreads) {
-                const int d = i % (kDim / 4) * 4, rr = i / (kDim / 4), col = 8 * n + rr;
+#pragma unroll
+            for (int v0 = 0; v0 < kSteps; v0 += kWarps) {
+                const int v = v0 + warp, col = 8 * n + value_row(v), d = value_d(v);
+                float2 ml[kWarps];
                 float top = -INFINITY, sum = 0.f;
 #pragma unroll
-                for (int w = 0; w < kWarps; ++w)
-                    top = fmaxf(top, stat[(w * S::kCols + col) * 2]);
+                for (int w = 0; w < kWarps; ++w) {
+                    ml[w] = *reinterpret_cast<const float2*>(stat + (w * S::kCols + col) * 2);
+                    top = fmaxf(top, ml[w].x);
+                }
                 float4 r = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
                 for (int w = 0; w < kWarps; ++w) {
-                    const float mw = stat[(w * S::kCols + col) * 2];
                     // a warp that saw nothing has zeros here (or the NaN of its q)
-                    const float f = mw == -INFINITY ? 0.f : ex2(mw - top);
-                    const float4 v = *reinterpret_cast<const float4*>(red + (w * 8 + rr) * kDim + d);
-                    sum += f * stat[(w * S::kCols + col) * 2 + 1];
-                    r.x += f * v.x, r.y += f * v.y, r.z += f * v.z, r.w += f * v.w;
+                    const float f = ml[w].x == -INFINITY ? 0.f : ex2(ml[w].x - top);
+                    const float4 x = reinterpret_cast<const float4*>(red)[(w * kSteps + v) * 32 + lane];
+                    sum = fmaf(f, ml[w].y, sum);
+                    r.x = fmaf(f, x.x, r.x), r.y = fmaf(f, x.y, r.y);
+                    r.z = fmaf(f, x.z, r.z), r.w = fmaf(f, x.w, r.w);
                 }
-                if (whole) {
-                    if (row0 + col < rows)
-                        write_out(out_row(seg.seq, head, row0 + col), d, r, top, sum, d == 0);
-                } else {
-                    *reinterpret_cast<float4*>(slot + col * kDim + d) = r;
-                    if (d == 0) {
-                        slot[16 * 128 + 2 * col] = top;
-                        slot[16 * 128 + 2 * col + 1] = sum;
-                    }
+                if (!whole) {
+                    reinterpret_cast<float4*>(slot)[(n * kSteps + v) * 32 + lane] = r;
+                    if (d == 0)
+                        *reinterpret_cast<float2*>(slot + 16 * 128 + 2 * col) = make_float2(top, sum);
+                } else if (row0 + col < rows) {
+                    write_out(out_row(now.seq, head, row0 + col), d, r, top, sum, d == 0);
                 }
             }
             __syncthreads();
         }
+        if (seg.begin < u1) load_q(seg);
 
         if (!whole) {
-            // Adds `count` partial results at base, base + stride, ... in order.
-            const int c0 = seg.seg0 / share, c1 = (seg.seg0 + seg.blocks - 1) / share;
-            const int n = c1 - c0 + 1, me = (int)blockIdx.x - c0;
+            if (!chunked) {
+                c0 = now.begin / share;
+                parts = (now.begin + now.units - 1) / share - c0 + 1;
+            }
+            const int me = (int)blockIdx.x - c0;
             auto slot_of = [&](int i) {  // of the segment's i-th CTA
                 return p.partial + ((int64_t)(c0 + i) * 2 + (i == 0)) * kPartialFloats;
             };
             auto arrive = [&](int* counter, int count) {
-                __threadfence();
                 __syncthreads();
                 if (tid == 0) {
-                    const int old = atomicAdd(counter, 1);
+                    // releases this CTA's stores (ordered by the barrier) and
+                    // acquires those of the CTAs that came before
+                    int old;
+                    asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;"
+                                 : "=r"(old) : "l"(counter) : "memory");
                     *flag = old == count - 1;
                     if (old == count - 1) *counter = 0;  // ready for the next launch
                 }
                 __syncthreads();
-                const bool last = *flag != 0;
-                __threadfence();
-                __syncthreads();
-                return last;
+                return *flag != 0;
             };
+            // Adds the `count` partial results first, first + step, ... in order;
+            // eight are in flight at a time.
             auto add = [&](int first, int step, int count, float* to) {
 #pragma unroll 1
-                for (int i = tid; i < S::kCols * (kDim / 4); i += kThreads) {
-                    const int d = i % (kDim / 4) * 4, col = i / (kDim / 4);
+                for (int nv = warp; nv < kNB * kSteps; nv += kWarps) {
+                    const int v = nv % kSteps, d = value_d(v);
+                    const int col = nv / kSteps * 8 + value_row(v);
                     float top = -INFINITY, sum = 0.f;
                     float4 r = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-                    for (int k = 0; k < count; ++k) {
-                        const float* src = slot_of(first + k * step);
-                        const float4 v = __ldcg(reinterpret_cast<const float4*>(src + col * kDim + d));
-                        const float2 ml = __ldcg(reinterpret_cast<const float2*>(src + 16 * 128 + 2 * col));
-                        const float nt = fmaxf(top, ml.x);
-                        const float ref = nt == -INFINITY ? 0.f : nt;
-                        const float fo = ex2(top - ref), fn = ex2(ml.x - ref);
-                        sum = sum * fo + ml.y * fn;
-                        r.x = r.x * fo + v.x * fn, r.y = r.y * fo + v.y * fn;
-                        r.z = r.z * fo + v.z * fn, r.w = r.w * fo + v.w * fn;
-                        top = nt;
+#pragma unroll 1
+                    for (int k0 = 0; k0 < count; k0 += 8) {
+                        float2 ml[8];
+                        float4 x[8];
+                        float best = top;
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            ml[k] = make_float2(-INFINITY, 0.f);
+                            x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+                            if (k0 + k < count) {
+                                const float* src = slot_of(first + (k0 + k) * step);
+                                ml[k] = __ldcg(reinterpret_cast<const float2*>(src + 16 * 128 + 2 * col));
+                                x[k] = __ldcg(reinterpret_cast<const float4*>(src) + nv * 32 + lane);
+                            }
+                        }
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) best = fmaxf(best, ml[k].x);
+                        const float ref = best == -INFINITY ? 0.f : best;
+                        const float old = ex2(top - ref);
+                        top = best;
+                        sum *= old, r.x *= old, r.y *= old, r.z *= old, r.w *= old;
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            const float f = ex2(ml[k].x - ref);
+                            sum = fmaf(ml[k].y, f, sum);
+                            r.x = fmaf(x[k].x, f, r.x), r.y = fmaf(x[k].y, f, r.y);
+                            r.z = fmaf(x[k].z, f, r.z), r.w = fmaf(x[k].w, f, r.w);
+                        }
                     }
                     if (to == nullptr) {
                         if (row0 + col < rows)
-                            write_out(out_row(seg.seq, head, row0 + col), d, r, top, sum, d == 0);
+                            write_out(out_row(now.seq, head, row0 + col), d, r, top, sum, d == 0);
                     } else {
-                        // the leader's own place, read by nobody else in this group
-                        *reinterpret_cast<float4*>(to + col * kDim + d) = r;
-                        if (d == 0) red[2 * col] = top, red[2 * col + 1] = sum;
+                        // over the leader's own partial result, whose O this lane alone has
+                        // read; m and l go elsewhere until every warp has read them
+                        reinterpret_cast<float4*>(to)[nv * 32 + lane] = r;
+                        if (d == 0)
+                            *reinterpret_cast<float2*>(stat + 2 * col) = make_float2(top, sum);
                     }
                 }
                 if (to != nullptr) {
                     __syncthreads();
-                    if (tid < 2 * S::kCols) to[16 * 128 + tid] = red[tid];
+                    if (tid < 2 * S::kCols) to[16 * 128 + tid] = stat[tid];
                 }
             };
-            const int groups = (n + kFan - 1) / kFan, mine = me / kFan;
-            const int lead = mine * kFan, size = min(kFan, n - lead);
+            const int groups = (parts + kFan - 1) / kFan, mine_group = me / kFan;
+            const int lead = mine_group * kFan, size = min(kFan, parts - lead);
             // Counters: a CTA can lead the first group of the segment it
             // begins and a later group of the segment it is inside of.
-            int* first = p.counters + (mine == 0 ? 0 : kMaxGrid) + c0 + lead;
-            if (arrive(first, size)) {
+            if (arrive(p.counters + (mine_group == 0 ? 0 : kMaxGrid) + c0 + lead, size)) {
                 if (groups == 1) {
-                    add(0, 1, n, nullptr);
+                    add(0, 1, parts, nullptr);
                 } else {
                     add(lead, 1, size, slot_of(lead));
                     if (arrive(p.counters + 2 * kMaxGrid + c0, groups))
@@ -723,15 +890,15 @@ __global__ void __launch_bounds__(kThreads, kDim == 256 ? 2 : 3)
             }
             __syncthreads();
         }
-        next_segment(seg);
-        if (seg.seq >= a.batch) break;
     }
 
     if (failed) {
-        // Copies in flight must land before the CTA's shared memory is given up.
-        for (int i = 0; i < kStages; ++i)
-            if ((pending >> i) & 1u)
-                mbar_wait_bounded(my_bars + 8 * i, (uint32_t)phase >> i & 1u, p.wait_cycles);
+        // Copies in flight must land before the CTA's shared memory is given up:
+        // the units issued and not done are in the next stages of the ring.
+        for (int i = 0; i < min(issued, mine) - done; ++i) {
+            const int at_stage = (done + i) % kStages;
+            mbar_wait_bounded(my_bars + 8 * at_stage, phase >> at_stage & 1u, p.wait_cycles);
+        }
     }
 }
 
@@ -771,9 +938,14 @@ cudaError_t run(Params& p, cudaStream_t stream) {
         ctas = std::min(std::max(1, n) * sms, kMaxGrid);
         resident[dev].store(ctas, std::memory_order_release);
     }
-    p.row_tiles = (a.new_tokens * a.group + S::kCols - 1) / S::kCols;
-    const int64_t line = longest_line(a, p.row_tiles);
-    const int64_t grid = std::min<int64_t>(ctas, std::max<int64_t>(line / p.min_blocks + 1, a.batch));
+    p.row_tiles = FastDiv((a.new_tokens * a.group + S::kCols - 1) / S::kCols);
+    const int64_t line = longest_line(a, p.row_tiles.d);
+    // Never more CTAs than chunks of min_units in segments of the greatest length.
+    const int64_t segments = (int64_t)a.batch * a.kv_heads * p.row_tiles.d;
+    const int64_t unit_chunk = (int64_t)p.min_units * S::kU;  // blocks
+    const int64_t chunks = segments * ((line / segments + unit_chunk - 1) / unit_chunk);
+    const int64_t grid = std::max<int64_t>(1, std::min<int64_t>(ctas, chunks));
+    p.every_chunk = grid == chunks;
     return launch_pdl(kernel, dim3((unsigned)grid), dim3(kThreads), smem, stream, p);
 }
 
@@ -794,10 +966,9 @@ size_t kv_attention_workspace() {
 
 bool kv_attention_fits(const KvAttentionArgs& a) {
     const int64_t rows = (int64_t)a.new_tokens * a.group;
-    // the page division by multiplication is exact below 2^32 / blocks_per_page
     const int64_t per = a.page_size / kKvBlock;
     return longest_line(a, (rows + 7) / 8) < ((int64_t)1 << 31) - ((int64_t)1 << 21) &&
-           (int64_t)a.max_pages * per * per < (int64_t)1 << 32;
+           a.num_pages * a.kv_heads * per < ((int64_t)1 << 32) - 2;  // blocks are numbered
 }
 
 cudaError_t launch_kv_attention(const KvAttentionArgs& a, cudaStream_t stream) {
@@ -806,9 +977,9 @@ cudaError_t launch_kv_attention(const KvAttentionArgs& a, cudaStream_t stream) {
     p.a = a;
     p.counters = static_cast<int*>(a.workspace);
     p.partial = reinterpret_cast<float*>(static_cast<uint8_t*>(a.workspace) + kCounterBytes);
-    p.blocks_per_page = a.page_size / kKvBlock;
-    p.page_magic = (uint32_t)((((uint64_t)1 << 32) + p.blocks_per_page - 1) / p.blocks_per_page);
-    p.min_blocks = kWarps;
+    p.page_blocks = FastDiv(a.page_size / kKvBlock);
+    p.group = FastDiv(a.group);
+    p.min_units = 2 * kWarps;
     p.q_vec = (reinterpret_cast<uintptr_t>(a.q) & 15u) == 0 && a.q_batch % 8 == 0 &&
               a.q_new % 8 == 0 && a.q_head % 8 == 0;
     p.wait_cycles = wait_budget();
