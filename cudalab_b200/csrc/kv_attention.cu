@@ -122,6 +122,9 @@ __device__ __forceinline__ float lds_half(const uint8_t* at) {
     return __half2float(*reinterpret_cast<const __half*>(at));
 }
 
+// 8 elements of a q that 16-byte loads cannot take (a call, off the main path).
+__device__ __noinline__ uint4 load8_apart(const uint16_t* p) { return load8<false, false>(p, 0); }
+
 // n / d for 0 <= n < 2^31 by a multiplication, d fixed at launch.
 struct FastDiv {
     uint32_t d, mul, shift;
@@ -136,6 +139,14 @@ struct FastDiv {
     __device__ __forceinline__ int mod(int n) const { return n - div(n) * (int)d; }
 };
 
+// ceil(n / d) for 0 <= n < 2^22, inv = 1 / d within 2 ulp: (n - 1/2) / d keeps
+// half a step from the integers, more than the products' rounding.  The plan
+// runs once per launch, on cold instructions, where an integer division costs
+// more than its result.
+__device__ __forceinline__ int ceil_div(int n, float inv) {
+    return __float2int_ru(((float)n - 0.5f) * inv);
+}
+
 struct Params {
     KvAttentionArgs a;
     float* partial;
@@ -144,7 +155,11 @@ struct Params {
     FastDiv page_blocks; // blocks of a page
     FastDiv group;       // query heads per cache head
     int min_units;       // smallest range of a CTA
-    int every_chunk;     // the grid holds every chunk of min_units
+    int every_chunk;     // the grid holds every chunk of min_units of the longest lengths:
+    FastDiv seg_chunks;  // a segment has this many CTAs
+    FastDiv min_chunk;   // division by min_units
+    int may_chunk;       // lengths are short enough for ceil_div
+    float inv_grid;
     int q_vec;
     long long wait_cycles;
 };
@@ -217,24 +232,23 @@ __global__ void __launch_bounds__(kThreads, Shape<kDim, kBits, kNB>::kPerSm)
         return ((len + kKvBlock - 1) / kKvBlock - first_block(len) + kU - 1) / kU;
     };
     const int most = a.max_pages * a.page_size, grid = (int)gridDim.x;
+    auto length_of = [&](int b) {
+        int len = a.fixed_length >= 0 ? a.fixed_length : __ldg(a.lengths + b);
+        if (len > most || len < 0) {
+            atomicCAS(&g_kv_attention_status, 0, kStatusKvIndex);
+            len = len < 0 ? 0 : most;
+        }
+        return len;
+    };
     // Up to 32 sequences every warp plans for itself (all write the same values
     // and read their own), more are planned by the first warp.
     const bool few = a.batch <= 32;
-    for (int b = few ? lane : tid; b < a.batch; b += few ? 32 : kThreads) {
-        int len = a.fixed_length >= 0 ? a.fixed_length : __ldg(a.lengths + b);
-        if (len > most || len < 0) {
-            if (blockIdx.x == 0) atomicCAS(&g_kv_attention_status, 0, kStatusKvIndex);
-            len = len < 0 ? 0 : most;
-        }
-        s_len[b] = len;
-    }
     int cell = 1;   // units of a cell of the line (s_cum counts cells)
     int share = 1;  // cells of a CTA
-    if (few) __syncwarp(); else __syncthreads();
-    if (few || warp == 0) {
-        if (p.every_chunk) {
-            cell = p.min_units;
-        } else {
+    if (!p.every_chunk) {
+        for (int b = few ? lane : tid; b < a.batch; b += few ? 32 : kThreads) s_len[b] = length_of(b);
+        if (few) __syncwarp(); else __syncthreads();
+        if (few || warp == 0) {
             int units = 0, segments = 0;
             for (int b = lane; b < a.batch; b += 32) {
                 const int n = units_of(s_len[b]);
@@ -243,49 +257,51 @@ __global__ void __launch_bounds__(kThreads, Shape<kDim, kBits, kNB>::kPerSm)
             }
             units = __reduce_add_sync(0xffffffffu, units) * heads_tiles;
             segments = __reduce_add_sync(0xffffffffu, segments) * heads_tiles;
-            share = max(p.min_units, (units + grid - 1) / grid);  // equal ranges of the line
-            if (2 * segments <= grid) {
+            // equal ranges of the line (the estimate may be short on very long ones)
+            share = max(p.min_units, ceil_div(units, p.inv_grid));
+            if (share * (int64_t)grid < units) share += 1 + (share >> 20);
+            if (2 * segments <= grid && p.may_chunk) {
                 // Few segments: each is cut into chunks of its own, one per CTA,
                 // so that a CTA works on one segment.  Eight sizes between the
                 // equal range and the one that must fit, four lanes on each; the
                 // smallest with which the grid holds all chunks is taken.
-                const int fits = max(share, (units + grid - segments - 1) / (grid - segments));
-                const int mine = share + (fits - share) * (lane >> 2) / 7;
+                const int more = max(0, ceil_div(units, __fdividef(1.f, (float)(grid - segments))) + 1 - share);
+                const int mine = share + (more * (lane >> 2) * 37 >> 8);  // 37/256 > 1/7
+                const float inv = __fdividef(1.f, (float)mine);
                 int chunks = 0;
-                for (int b = lane & 3; b < a.batch; b += 4)
-                    chunks += (int)(((unsigned)units_of(s_len[b]) + mine - 1) / (unsigned)mine);
+                for (int b = lane & 3; b < a.batch; b += 4) chunks += ceil_div(units_of(s_len[b]), inv);
                 chunks += __shfl_xor_sync(0xffffffffu, chunks, 1);
                 chunks += __shfl_xor_sync(0xffffffffu, chunks, 2);
                 const uint32_t ok = __ballot_sync(0xffffffffu, chunks * heads_tiles <= grid);
                 cell = __shfl_sync(0xffffffffu, mine, __ffs(ok | 0x80000000u) - 1);
                 share = 1;
             }
-        }
-        int before = 0;
-        for (int b0 = 0; b0 < a.batch; b0 += 32) {
-            const int b = b0 + lane;
-            int n = b < a.batch ? units_of(s_len[b]) : 0;
-            if (cell > 1) n = (int)((unsigned)(n + cell - 1) / (unsigned)cell);
-            int scan = n;
+            const float inv = __fdividef(1.f, (float)cell);
+            int before = 0;
+            for (int b0 = 0; b0 < a.batch; b0 += 32) {
+                const int b = b0 + lane;
+                int n = b < a.batch ? units_of(s_len[b]) : 0;
+                if (cell > 1) n = ceil_div(n, inv);
+                int scan = n;
 #pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int v = __shfl_up_sync(0xffffffffu, scan, o);
-                if (lane >= o) scan += v;
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int v = __shfl_up_sync(0xffffffffu, scan, o);
+                    if (lane >= o) scan += v;
+                }
+                if (b < a.batch) s_cum[b] = before + scan - n;
+                before += __shfl_sync(0xffffffffu, scan, 31);
             }
-            if (b < a.batch) s_cum[b] = before + scan - n;
-            before += __shfl_sync(0xffffffffu, scan, 31);
+            if (lane == 0) s_cum[a.batch] = before, flag[1] = cell, flag[2] = share;
         }
-        if (lane == 0) s_cum[a.batch] = before, flag[1] = cell, flag[2] = share;
+        if (few) {
+            __syncwarp();
+        } else {
+            __syncthreads();
+            cell = flag[1];
+            share = flag[2];
+        }
     }
-    if (few) {
-        __syncwarp();
-    } else {
-        __syncthreads();
-        cell = flag[1];
-        share = flag[2];
-    }
-    const bool chunked = cell > 1;
-    const int total = s_cum[a.batch] * heads_tiles;
+    const bool chunked = p.every_chunk || cell > 1;
 
     // Row `r` of a tile of sequence `seq`: where it is in the outputs.
     auto out_row = [&](int seq, int head, int r) {
@@ -321,24 +337,45 @@ __global__ void __launch_bounds__(kThreads, Shape<kDim, kBits, kNB>::kPerSm)
     };
 
     // Sequences with nothing to read (their rows see no cached token).
-    for (int b = blockIdx.x; b < a.batch; b += grid) {
-        if (s_cum[b + 1] != s_cum[b]) continue;
-        const int n = rows * a.kv_heads * (kDim / 4);
-        for (int i = tid; i < n; i += kThreads) {
-            const int d = i % (kDim / 4) * 4, r = i / (kDim / 4);
-            write_out(out_row(b, r / rows, r % rows), d, make_float4(0.f, 0.f, 0.f, 0.f),
-                      -INFINITY, 0.f, d == 0);
-        }
-    }
-    const int x0 = (int)min((int64_t)total, (int64_t)blockIdx.x * share);
-    const int x1 = min(total, x0 + share);
-    if (x0 >= x1) return;
+    auto write_empty = [&](int b, int part0, int part1) {
+        const int n = rows * (kDim / 4);
+        for (int h = part0; h < part1; ++h)
+            for (int i = tid; i < n; i += kThreads) {
+                const int d = i % (kDim / 4) * 4;
+                write_out(out_row(b, h, i / (kDim / 4)), d, make_float4(0.f, 0.f, 0.f, 0.f),
+                          -INFINITY, 0.f, d == 0);
+            }
+    };
 
     // The CTA's range [u0, u1) and its first segment.  Chunked, the line is the
     // units of the one segment; else the units of all segments.
     Segment start;
-    int u0 = x0, u1 = x1, c0 = 0, parts = 0;  // chunked: first CTA and CTAs of the segment
-    {
+    int u0, u1, c0 = 0, parts = 0;  // chunked: first CTA and CTAs of the segment
+    int len0;                       // length of the first segment's sequence
+    if (p.every_chunk) {
+        const int segment = p.seg_chunks.div((int)blockIdx.x);
+        c0 = segment * (int)p.seg_chunks.d;
+        start.seq = (int)((unsigned)segment / (unsigned)heads_tiles);
+        start.part = segment - start.seq * heads_tiles;
+        len0 = length_of(start.seq);
+        start.begin = 0;
+        start.units = units_of(len0);
+        u0 = ((int)blockIdx.x - c0) * p.min_units;
+        u1 = min(u0 + p.min_units, start.units);
+        parts = p.min_chunk.div(start.units + p.min_units - 1);
+        if (u0 >= u1) {
+            if (start.units == 0 && u0 == 0 && p.row_tiles.mod(start.part) == 0)
+                write_empty(start.seq, p.row_tiles.div(start.part), p.row_tiles.div(start.part) + 1);
+            return;
+        }
+    } else {
+        for (int b = blockIdx.x; b < a.batch; b += grid)
+            if (s_cum[b + 1] == s_cum[b]) write_empty(b, 0, a.kv_heads);
+        const int total = s_cum[a.batch] * heads_tiles;
+        const int x0 = (int)min((int64_t)total, (int64_t)blockIdx.x * share);
+        u0 = x0;
+        u1 = min(total, x0 + share);
+        if (u0 >= u1) return;
         int lo = 0, hi = a.batch;  // last sequence whose cells begin at or before x0
         while (hi - lo > 1) {
             const int mid = (lo + hi) >> 1;
@@ -346,25 +383,26 @@ __global__ void __launch_bounds__(kThreads, Shape<kDim, kBits, kNB>::kPerSm)
         }
         const int cells = s_cum[lo + 1] - s_cum[lo], in = x0 - s_cum[lo] * heads_tiles;
         start.seq = lo;
-        start.part = in / cells;
+        start.part = (int)((unsigned)in / (unsigned)cells);
         start.units = cells;
         start.begin = s_cum[lo] * heads_tiles + start.part * cells;
+        len0 = s_len[lo];
         if (chunked) {
             const int chunk = in - start.part * cells;
             c0 = (int)blockIdx.x - chunk;
             parts = cells;
             start.begin = 0;
-            start.units = units_of(s_len[lo]);
+            start.units = units_of(len0);
             u0 = chunk * cell;
             u1 = min(u0 + cell, start.units);
         }
     }
     auto next_segment = [&](Segment& c) {
         c.begin += c.units;
-        if (++c.part == heads_tiles) {
+        if (!chunked && ++c.part == heads_tiles) {
             c.part = 0;
             do ++c.seq; while (c.seq < a.batch && s_cum[c.seq + 1] == s_cum[c.seq]);
-            if (c.seq < a.batch) c.units = s_cum[c.seq + 1] - s_cum[c.seq];  // not chunked
+            if (c.seq < a.batch) c.units = s_cum[c.seq + 1] - s_cum[c.seq];
         }
     };
 
@@ -390,8 +428,7 @@ __global__ void __launch_bounds__(kThreads, Shape<kDim, kBits, kNB>::kPerSm)
             for (int i = 0; i < kDim / 32; ++i) {
                 qraw[n][i] = make_uint4(0, 0, 0, 0);
                 const int e = k_byte(8 * i / kElements) * 8 / kBits + 8 * i % kElements;
-                if (r < rows)
-                    qraw[n][i] = p.q_vec ? load8<kBf16, true>(at, e) : load8<kBf16, false>(at, e);
+                if (r < rows) qraw[n][i] = p.q_vec ? load8<kBf16, true>(at, e) : load8_apart(at + e);
             }
         }
     };
@@ -419,7 +456,7 @@ __global__ void __launch_bounds__(kThreads, Shape<kDim, kBits, kNB>::kPerSm)
             part = in / units;
             in -= part * units;
         }
-        const int len = s_len[seq];
+        const int len = chunked ? len0 : s_len[seq];
         const uint32_t head = p.row_tiles.div(part);
 #pragma unroll
         for (int k = 0; k < kU; ++k) {
@@ -483,7 +520,7 @@ __global__ void __launch_bounds__(kThreads, Shape<kDim, kBits, kNB>::kPerSm)
     while (seg.begin < u1) {
         const int sa = max(seg.begin, u0), sb = min(seg.begin + seg.units, u1);
         const int head = p.row_tiles.div(seg.part), row0 = p.row_tiles.mod(seg.part) * S::kCols;
-        const int len = s_len[seg.seq];
+        const int len = chunked ? len0 : s_len[seg.seq];
         const int token0 = first_block(len) * kKvBlock - seg.begin * (kU * kKvBlock);
 
         // q as B fragments.  bf16 rows are brought into fp16's range by a power
@@ -943,9 +980,14 @@ cudaError_t run(Params& p, cudaStream_t stream) {
     // Never more CTAs than chunks of min_units in segments of the greatest length.
     const int64_t segments = (int64_t)a.batch * a.kv_heads * p.row_tiles.d;
     const int64_t unit_chunk = (int64_t)p.min_units * S::kU;  // blocks
-    const int64_t chunks = segments * ((line / segments + unit_chunk - 1) / unit_chunk);
-    const int64_t grid = std::max<int64_t>(1, std::min<int64_t>(ctas, chunks));
-    p.every_chunk = grid == chunks;
+    const int64_t per = std::max<int64_t>(1, (line / segments + unit_chunk - 1) / unit_chunk);
+    const int64_t grid = std::min<int64_t>(ctas, segments * per);
+    p.every_chunk = grid == segments * per;
+    p.seg_chunks = FastDiv((uint32_t)per);
+    p.min_chunk = FastDiv((uint32_t)p.min_units);
+    // blocks of all segments below 2^22: every count that the plan divides is
+    p.may_chunk = line < (int64_t)1 << 22;
+    p.inv_grid = 1.f / (float)grid;
     return launch_pdl(kernel, dim3((unsigned)grid), dim3(kThreads), smem, stream, p);
 }
 
