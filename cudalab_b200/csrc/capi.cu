@@ -658,7 +658,7 @@ int cache_args(const char* op, const void* k, const void* v, const void* pages, 
     const int rc = check_cache(op, d->num_pages, d->kv_heads, d->head_dim, d->bits, d->page_size, pages);
     if (rc != CL_OK) return rc;
     if (d->tokens > 0 && (!k || !v || !slots)) return bad(op, "null device pointer");
-    if (d->tokens > ((int64_t)1 << 38) / (d->kv_heads * (d->head_dim / 16)))
+    if (d->tokens > (((int64_t)1 << 31) - 256) / d->kv_heads)
         return bad(op, "too many tokens for one launch");
     *a = clb::KvCacheArgs{const_cast<uint8_t*>(static_cast<const uint8_t*>(pages)), slots,
                           const_cast<void*>(k), const_cast<void*>(v), d->k_token, d->k_head,
@@ -690,7 +690,7 @@ int cl_qknorm_rope(const void* q, const void* k, const void* q_weight, const voi
     if (d->tokens == 0) return CL_OK;
     if (!q || !k || !table || !positions || !q_out || !k_out) return bad(op, "null device pointer");
     if (misaligned16(table)) return bad(op, "table must be 16-byte aligned");
-    if (d->tokens > ((int64_t)1 << 37) / ((d->q_heads + d->kv_heads) * 16))
+    if (d->tokens > (((int64_t)1 << 31) - 256) / ((int64_t)d->q_heads + d->kv_heads))
         return bad(op, "too many tokens for one launch");
     const clb::QkRopeArgs a{{q, k},
                             {q_out, k_out},

@@ -125,20 +125,6 @@ __device__ __forceinline__ float lds_half(const uint8_t* at) {
 // 8 elements of a q that 16-byte loads cannot take (a call, off the main path).
 __device__ __noinline__ uint4 load8_apart(const uint16_t* p) { return load8<false, false>(p, 0); }
 
-// n / d for 0 <= n < 2^31 by a multiplication, d fixed at launch.
-struct FastDiv {
-    uint32_t d, mul, shift;
-    FastDiv() = default;
-    explicit FastDiv(uint32_t divisor) : d(divisor), mul(0), shift(0) {
-        while (((uint64_t)1 << shift) < d) ++shift;
-        mul = (uint32_t)((((uint64_t)1 << 32) * (((uint64_t)1 << shift) - d)) / d + 1);
-    }
-    __device__ __forceinline__ int div(int n) const {
-        return (int)((__umulhi((uint32_t)n, mul) + (uint32_t)n) >> shift);
-    }
-    __device__ __forceinline__ int mod(int n) const { return n - div(n) * (int)d; }
-};
-
 // ceil(n / d) for 0 <= n < 2^22, inv = 1 / d within 2 ulp: (n - 1/2) / d keeps
 // half a step from the integers, more than the products' rounding.  The plan
 // runs once per launch, on cold instructions, where an integer division costs

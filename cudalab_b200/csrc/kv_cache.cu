@@ -59,17 +59,25 @@ __device__ __forceinline__ bool find_slot(const KvCacheArgs& a, int64_t slot, in
     return true;
 }
 
+// Largest magnitude of 16 elements, NaN if one of them is.
+__device__ __forceinline__ float max16(const float (&x)[16]) {
+    float m = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+        asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(m), "f"(fabsf(x[i])));
+    return m;
+}
+
+// rint(x * inv) within +-top as two's complement fields.  Adding 1.5 * 2^23
+// rounds to the nearest even integer and leaves it in the low bits, without
+// the quarter-rate conversion.
 template <int kBits>
-__device__ __forceinline__ void quantise16(const float (&x)[16], float s, uint32_t* out) {
-    const float inv = s == 0.f ? 0.f : __frcp_rn(s);
+__device__ __forceinline__ void quantise16(const float (&x)[16], float inv, uint32_t* out) {
     constexpr float kTop = kBits == 8 ? 127.f : 7.f;
     uint32_t q[16];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        // fminf / fmaxf drop a NaN, so the select keeps it at 0
-        const float y = x[i] == x[i] ? __fmul_rn(x[i], inv) : 0.f;
-        q[i] = (uint32_t)__float2int_rn(fminf(fmaxf(y, -kTop), kTop));
-    }
+    for (int i = 0; i < 16; ++i)
+        q[i] = __float_as_uint(fminf(fmaxf(__fmul_rn(x[i], inv), -kTop), kTop) + 12582912.f);
     if (kBits == 8) {
 #pragma unroll
         for (int w = 0; w < 4; ++w)
@@ -86,16 +94,37 @@ __device__ __forceinline__ void quantise16(const float (&x)[16], float s, uint32
     }
 }
 
+// 16 fields as floats: the field, its sign bit flipped, in the mantissa of
+// 2^23, less 2^23 and the flip (exact).
+template <int kBits>
+__device__ __forceinline__ void expand16(const uint32_t (&raw)[4], float (&x)[16]) {
+    if (kBits == 8) {
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const uint32_t u = raw[w] ^ 0x80808080u;
+            x[4 * w] = __uint_as_float(prmt_i<0x7650u>(u, 0x4b000000u)) - 8388736.f;
+            x[4 * w + 1] = __uint_as_float(prmt_i<0x7651u>(u, 0x4b000000u)) - 8388736.f;
+            x[4 * w + 2] = __uint_as_float(prmt_i<0x7652u>(u, 0x4b000000u)) - 8388736.f;
+            x[4 * w + 3] = __uint_as_float(prmt_i<0x7653u>(u, 0x4b000000u)) - 8388736.f;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            x[i] = __uint_as_float(lop3_sel_xor(raw[i / 8] >> (4 * (i % 8)), 0xFu, 0x4b000008u)) -
+                   8388616.f;
+    }
+}
+
 template <int kDim, int kBits, bool kBf16, bool kVec>
-__global__ void __launch_bounds__(kThreads) kv_write_kernel(const KvCacheArgs a) {
+__global__ void __launch_bounds__(kThreads) kv_write_kernel(const KvCacheArgs a, const FastDiv heads) {
     constexpr int kRow = kDim * kBits / 8, kLanes = kDim / 16;
     constexpr int kBlockBytes = kv_block_bytes(kRow);
     pdl_allow_dependents();
     pdl_wait_prior_grids();
-    const int64_t row = ((int64_t)blockIdx.x * kThreads + threadIdx.x) / kLanes;
+    const int row = (int)(blockIdx.x * (kThreads / kLanes) + threadIdx.x / kLanes);
     const int l = threadIdx.x % kLanes;
-    const int64_t token = row / a.kv_heads;
-    const int head = (int)(row % a.kv_heads);
+    const int64_t token = heads.div(row);
+    const int head = heads.mod(row);
     const bool in = token < a.tokens;
     const int64_t slot = in ? a.slots[token] : -1;
     float x[2][16];
@@ -107,10 +136,11 @@ __global__ void __launch_bounds__(kThreads) kv_write_kernel(const KvCacheArgs a)
     const bool put = find_slot(a, slot, head, kBlockBytes, &p);
 #pragma unroll
     for (int part = 0; part < 2; ++part) {
-        float m = 0.f;
-        if (in) {
+        float m = in ? max16(x[part]) : 0.f;
+        if (!(m == m)) {  // NaN is stored as 0
 #pragma unroll
-            for (int i = 0; i < 16; ++i) m = fmaxf(m, fabsf(x[part][i]));  // drops NaN
+            for (int i = 0; i < 16; ++i) x[part][i] = x[part][i] == x[part][i] ? x[part][i] : 0.f;
+            m = max16(x[part]);
         }
 #pragma unroll
         for (int o = kLanes / 2; o > 0; o >>= 1)
@@ -119,7 +149,7 @@ __global__ void __launch_bounds__(kThreads) kv_write_kernel(const KvCacheArgs a)
         const __half s = __float2half_rn(fminf(__fdiv_rn(m, top), 65504.f));
         if (!put) continue;
         uint32_t q[4];
-        quantise16<kBits>(x[part], __half2float(s), q);
+        quantise16<kBits>(x[part], __hgt(s, __half(0.f)) ? __frcp_rn(__half2float(s)) : 0.f, q);
         uint8_t* rows = const_cast<uint8_t*>(p.block) + part * kKvBlock * kRow;
         if (kBits == 8)
             *reinterpret_cast<uint4*>(rows + kv_offset<kRow>(p.j, 16 * l)) =
@@ -133,15 +163,15 @@ __global__ void __launch_bounds__(kThreads) kv_write_kernel(const KvCacheArgs a)
 }
 
 template <int kDim, int kBits, bool kBf16, bool kVec>
-__global__ void __launch_bounds__(kThreads) kv_read_kernel(const KvCacheArgs a) {
+__global__ void __launch_bounds__(kThreads) kv_read_kernel(const KvCacheArgs a, const FastDiv heads) {
     constexpr int kRow = kDim * kBits / 8, kLanes = kDim / 16;
     constexpr int kBlockBytes = kv_block_bytes(kRow);
     pdl_allow_dependents();
     pdl_wait_prior_grids();
-    const int64_t row = ((int64_t)blockIdx.x * kThreads + threadIdx.x) / kLanes;
+    const int row = (int)(blockIdx.x * (kThreads / kLanes) + threadIdx.x / kLanes);
     const int l = threadIdx.x % kLanes;
-    const int64_t token = row / a.kv_heads;
-    const int head = (int)(row % a.kv_heads);
+    const int64_t token = heads.div(row);
+    const int head = heads.mod(row);
     if (token >= a.tokens) return;
     Place p;
     const bool have = find_slot(a, a.slots[token], head, kBlockBytes, &p);
@@ -165,13 +195,9 @@ __global__ void __launch_bounds__(kThreads) kv_read_kernel(const KvCacheArgs a) 
 #pragma unroll
     for (int part = 0; part < 2; ++part) {
         float x[16];
+        expand16<kBits>(raw[part], x);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            // sign extension of the field by a shift pair
-            const int v = kBits == 8 ? (int)(raw[part][i / 4] << (24 - 8 * (i % 4))) >> 24
-                                     : (int)(raw[part][i / 8] << (28 - 4 * (i % 8))) >> 28;
-            x[i] = __fmul_rn((float)v, s[part]);
-        }
+        for (int i = 0; i < 16; ++i) x[i] = __fmul_rn(x[i], s[part]);
         void* y = part ? a.v : a.k;
         const int64_t at = part ? token * a.v_token + head * a.v_head
                                 : token * a.k_token + head * a.k_head;
@@ -179,7 +205,7 @@ __global__ void __launch_bounds__(kThreads) kv_read_kernel(const KvCacheArgs a) 
     }
 }
 
-using Kernel = void (*)(KvCacheArgs);
+using Kernel = void (*)(KvCacheArgs, FastDiv);
 
 template <bool kWrite, int kDim, int kBits>
 Kernel pick(bool bf16, bool vec) {
@@ -209,7 +235,7 @@ cudaError_t launch(const KvCacheArgs& a, cudaStream_t stream) {
         k = a.bits == 8 ? pick<kWrite, 256, 8>(bf16, vec) : pick<kWrite, 256, 4>(bf16, vec);
     const int64_t threads = a.tokens * a.kv_heads * (a.head_dim / 16);
     return launch_pdl(k, dim3((unsigned)((threads + kThreads - 1) / kThreads)), dim3(kThreads), 0,
-                      stream, a);
+                      stream, a, FastDiv((uint32_t)a.kv_heads));
 }
 
 }  // namespace

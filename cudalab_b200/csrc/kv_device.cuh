@@ -83,6 +83,20 @@ __device__ __forceinline__ void store16(void* p, int64_t at, const float (&x)[16
     store8<kVec>(p, at + 8, pack8<kBf16>(x + 8));
 }
 
+// n / d for 0 <= n < 2^31 by a multiplication, d fixed at launch.
+struct FastDiv {
+    uint32_t d, mul, shift;
+    FastDiv() = default;
+    explicit FastDiv(uint32_t divisor) : d(divisor), mul(0), shift(0) {
+        while (((uint64_t)1 << shift) < d) ++shift;
+        mul = (uint32_t)((((uint64_t)1 << 32) * (((uint64_t)1 << shift) - d)) / d + 1);
+    }
+    __device__ __forceinline__ int div(int n) const {
+        return (int)((__umulhi((uint32_t)n, mul) + (uint32_t)n) >> shift);
+    }
+    __device__ __forceinline__ int mod(int n) const { return n - div(n) * (int)d; }
+};
+
 // Rows of 16-bit elements that 16-byte accesses may be used on.
 inline bool aligned16(const void* p, int64_t stride0, int64_t stride1) {
     return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && stride0 % 8 == 0 && stride1 % 8 == 0;

@@ -8,8 +8,11 @@
 // read and written once.  A lane holds two 8-element pieces (16-byte loads) of
 // a head; with pairs of halves they are the two pieces that rotate against
 // each other, so the rotation needs no exchange between lanes and the mean
-// three shuffles at head_dim 128.  The lanes of a head take kHeads heads of
-// one token, so the token's cosines and sines are loaded once for them.
+// three shuffles at head_dim 128.  The lanes of a head walk over `per` heads of
+// one token and of one of q and k, so cosines, sines and weights are loaded
+// once for them.  A lane's pieces of the next kDepth heads are on their way to
+// its own places in shared memory (16-byte asynchronous copies) while it
+// computes: what a lane waits for is held by no register.
 #include <cuda_runtime.h>
 
 #include <cstdint>
@@ -24,109 +27,149 @@ namespace {
 __device__ int g_rope_status;
 
 constexpr int kThreads = 256;
-constexpr int kHeads = 2;  // heads per lane group
-
 __device__ __forceinline__ void rotate(float& p, float& q, float c, float s) {
     const float y = p * c - q * s;
     q = q * c + p * s;
     p = y;
 }
 
-template <int kLanes, bool kBf16, bool kVec>
-__global__ void __launch_bounds__(kThreads) qknorm_rope_kernel(const QkRopeArgs a, int tasks) {
+constexpr int kDepth = 4;
+
+__device__ __forceinline__ void copy16(void* to, const void* from, bool go) {
+    if (go)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(to)), "l"(from)
+                     : "memory");
+}
+__device__ __forceinline__ void copies_end_group() {
+    asm volatile("cp.async.commit_group;" ::: "memory");
+}
+template <int kLeft>
+__device__ __forceinline__ void copies_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory");
+}
+
+struct Tasks {
+    int per;         // heads of a task
+    int q_tasks;     // tasks of a token's q; the rest are of its k
+    FastDiv tasks;   // of a token
+};
+
+template <int kLanes, bool kBf16, bool kVec, bool kInterleaved>
+__global__ void __launch_bounds__(kThreads, 4) qknorm_rope_kernel(const QkRopeArgs a,
+                                                                  const Tasks tasks) {
     pdl_allow_dependents();
     pdl_wait_prior_grids();
-    const int64_t group = ((int64_t)blockIdx.x * kThreads + threadIdx.x) / kLanes;
+    const int task = (int)(blockIdx.x * (kThreads / kLanes) + threadIdx.x / kLanes);
     const int l = threadIdx.x % kLanes;
-    const int64_t token = group / tasks;
-    const int first = (int)(group % tasks) * kHeads;
-    const int total = a.heads[0] + a.heads[1];
+    const int64_t token = tasks.tasks.div(task);
+    const int in_token = tasks.tasks.mod(task);
+    const int which = in_token >= tasks.q_tasks;
+    const int first = (which ? in_token - tasks.q_tasks : in_token) * tasks.per;
     const bool have = token < a.tokens && 16 * l < a.head_dim;
+    const int count = have ? min(tasks.per, a.heads[which] - first) : 0;
     // The two pieces of this lane: rotating lanes come first.
-    const int turning = a.rotary / 16;
-    const bool turn = l < turning;
-    int d0, d1, i0;
-    if (turn && !a.interleaved) {
-        d0 = 8 * l;
+    const bool turn = l < a.rotary / 16;
+    int d0 = 16 * l, d1 = d0 + 8, i0 = 8 * l;
+    if (!kInterleaved && turn) {
+        d0 = i0;
         d1 = d0 + a.rotary / 2;
-        i0 = d0;
-    } else {
-        d0 = 16 * l;
-        d1 = d0 + 8;
-        i0 = 8 * l;
     }
-    uint4 raw[kHeads][2];
-    int which[kHeads], head[kHeads];
+    const uint16_t* x0 = static_cast<const uint16_t*>(a.x[which]) + token * a.x_token[which] +
+                         first * a.x_head[which];
+    uint16_t* y0 = static_cast<uint16_t*>(a.y[which]) + token * a.y_token[which] +
+                   first * a.y_head[which];
+    __shared__ uint4 ring[kVec ? kDepth : 1][2][kVec ? kThreads : 1];
+    const int tid = threadIdx.x;
+    if (kVec) {
 #pragma unroll
-    for (int n = 0; n < kHeads; ++n) {
-        const int h = first + n;
-        which[n] = h >= a.heads[0];
-        head[n] = which[n] ? h - a.heads[0] : h;
-        raw[n][0] = raw[n][1] = make_uint4(0, 0, 0, 0);
-        if (have && h < total) {
-            const int64_t at = token * a.x_token[which[n]] + head[n] * a.x_head[which[n]];
-            raw[n][0] = load8<kBf16, kVec>(a.x[which[n]], at + d0);
-            raw[n][1] = load8<kBf16, kVec>(a.x[which[n]], at + d1);
+        for (int n = 0; n < kDepth - 1; ++n) {
+            copy16(&ring[n][0][tid], x0 + n * a.x_head[which] + d0, n < count);
+            copy16(&ring[n][1][tid], x0 + n * a.x_head[which] + d1, n < count);
+            copies_end_group();
         }
     }
     float c[8], s[8];
-    if (have && turn) {
-        int64_t pos = a.positions64 ? static_cast<const int64_t*>(a.positions)[token]
-                                    : static_cast<const int32_t*>(a.positions)[token];
-        if (pos < 0 || pos >= a.table_rows) {
-            atomicCAS(&g_rope_status, 0, kStatusKvIndex);
-            pos = pos < 0 ? 0 : a.table_rows - 1;
+    uint4 w[2] = {};
+    if (have) {
+        if (turn) {
+            int64_t pos = a.positions64 ? static_cast<const int64_t*>(a.positions)[token]
+                                        : static_cast<const int32_t*>(a.positions)[token];
+            if (pos < 0 || pos >= a.table_rows) {
+                atomicCAS(&g_rope_status, 0, kStatusKvIndex);
+                pos = pos < 0 ? 0 : a.table_rows - 1;
+            }
+            const float4* t = reinterpret_cast<const float4*>(a.table + pos * a.rotary + i0);
+            const float4* u = t + a.rotary / 8;
+            const float4 c0 = t[0], c1 = t[1], s0 = u[0], s1 = u[1];
+            c[0] = c0.x, c[1] = c0.y, c[2] = c0.z, c[3] = c0.w;
+            c[4] = c1.x, c[5] = c1.y, c[6] = c1.z, c[7] = c1.w;
+            s[0] = s0.x, s[1] = s0.y, s[2] = s0.z, s[3] = s0.w;
+            s[4] = s1.x, s[5] = s1.y, s[6] = s1.z, s[7] = s1.w;
         }
-        const float4* t = reinterpret_cast<const float4*>(a.table + pos * a.rotary + i0);
-        const float4* u = reinterpret_cast<const float4*>(a.table + pos * a.rotary + a.rotary / 2 + i0);
-        const float4 c0 = t[0], c1 = t[1], s0 = u[0], s1 = u[1];
-        c[0] = c0.x, c[1] = c0.y, c[2] = c0.z, c[3] = c0.w;
-        c[4] = c1.x, c[5] = c1.y, c[6] = c1.z, c[7] = c1.w;
-        s[0] = s0.x, s[1] = s0.y, s[2] = s0.z, s[3] = s0.w;
-        s[4] = s1.x, s[5] = s1.y, s[6] = s1.z, s[7] = s1.w;
+        if (a.w[0] != nullptr) {
+            w[0] = load8<kBf16, kVec>(a.w[which], d0);
+            w[1] = load8<kBf16, kVec>(a.w[which], d1);
+        }
     }
-#pragma unroll
-    for (int n = 0; n < kHeads; ++n) {
+    const float inv_dim = 1.f / (float)a.head_dim;
+#pragma unroll 1
+    for (int n = 0; n < tasks.per; ++n) {  // the same count for all lanes of a warp
         float x[16];
-        unpack8<kBf16>(raw[n][0], x);
-        unpack8<kBf16>(raw[n][1], x + 8);
+        if (kVec) {
+            const int ahead = n + kDepth - 1;
+            copy16(&ring[ahead % kDepth][0][tid], x0 + ahead * a.x_head[which] + d0, ahead < count);
+            copy16(&ring[ahead % kDepth][1][tid], x0 + ahead * a.x_head[which] + d1, ahead < count);
+            copies_end_group();
+            copies_wait<kDepth - 1>();
+        }
+        uint4 raw[2] = {};
+        if (n < count) {
+            raw[0] = kVec ? ring[n % kDepth][0][tid] : load8<kBf16, false>(x0 + n * a.x_head[which], d0);
+            raw[1] = kVec ? ring[n % kDepth][1][tid] : load8<kBf16, false>(x0 + n * a.x_head[which], d1);
+        }
+        unpack8<kBf16>(raw[0], x);
+        unpack8<kBf16>(raw[1], x + 8);
         if (a.w[0] != nullptr) {
             float sum = 0.f;
 #pragma unroll
             for (int i = 0; i < 16; ++i) sum = fmaf(x[i], x[i], sum);
 #pragma unroll
             for (int o = kLanes / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            if (have) {
-                const float r = rsqrtf(sum / (float)a.head_dim + a.eps);
-                float w[16];
-                unpack8<kBf16>(load8<kBf16, kVec>(a.w[which[n]], d0), w);
-                unpack8<kBf16>(load8<kBf16, kVec>(a.w[which[n]], d1), w + 8);
+            const float r = rsqrtf(fmaf(sum, inv_dim, a.eps));
+            float f[16];
+            unpack8<kBf16>(w[0], f);
+            unpack8<kBf16>(w[1], f + 8);
 #pragma unroll
-                for (int i = 0; i < 16; ++i) x[i] = x[i] * r * w[i];
+            for (int i = 0; i < 16; ++i) x[i] = x[i] * r * f[i];
+        }
+        if (n >= count) continue;
+        if (turn) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                if (kInterleaved) rotate(x[2 * i], x[2 * i + 1], c[i], s[i]);
+                else rotate(x[i], x[i + 8], c[i], s[i]);
             }
         }
-        if (!have || first + n >= total) continue;
-        if (turn && a.interleaved) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) rotate(x[2 * i], x[2 * i + 1], c[i], s[i]);
-        } else if (turn) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) rotate(x[i], x[i + 8], c[i], s[i]);
-        }
-        const int64_t at = token * a.y_token[which[n]] + head[n] * a.y_head[which[n]];
-        store8<kVec>(a.y[which[n]], at + d0, pack8<kBf16>(x));
-        store8<kVec>(a.y[which[n]], at + d1, pack8<kBf16>(x + 8));
+        store8<kVec>(y0 + n * a.y_head[which], d0, pack8<kBf16>(x));
+        store8<kVec>(y0 + n * a.y_head[which], d1, pack8<kBf16>(x + 8));
     }
 }
 
-using Kernel = void (*)(QkRopeArgs, int);
+using Kernel = void (*)(QkRopeArgs, Tasks);
 
-template <int kLanes>
+template <int kLanes, bool kInterleaved>
 Kernel pick(bool bf16, bool vec) {
-    return bf16 ? (vec ? qknorm_rope_kernel<kLanes, true, true>
-                       : qknorm_rope_kernel<kLanes, true, false>)
-                : (vec ? qknorm_rope_kernel<kLanes, false, true>
-                       : qknorm_rope_kernel<kLanes, false, false>);
+    return bf16 ? (vec ? qknorm_rope_kernel<kLanes, true, true, kInterleaved>
+                       : qknorm_rope_kernel<kLanes, true, false, kInterleaved>)
+                : (vec ? qknorm_rope_kernel<kLanes, false, true, kInterleaved>
+                       : qknorm_rope_kernel<kLanes, false, false, kInterleaved>);
+}
+
+template <bool kInterleaved>
+Kernel pick_lanes(int lanes, bool bf16, bool vec) {
+    return lanes == 4 ? pick<4, kInterleaved>(bf16, vec)
+                      : lanes == 8 ? pick<8, kInterleaved>(bf16, vec)
+                                   : pick<16, kInterleaved>(bf16, vec);
 }
 
 }  // namespace
@@ -140,12 +183,19 @@ cudaError_t launch_qknorm_rope(const QkRopeArgs& a, cudaStream_t stream) {
               (reinterpret_cast<uintptr_t>(a.w[i]) & 15u) == 0;
     const bool bf16 = a.type == kTypeBf16;
     const int lanes = a.head_dim <= 64 ? 4 : a.head_dim <= 128 ? 8 : 16;
-    const Kernel k = lanes == 4 ? pick<4>(bf16, vec) : lanes == 8 ? pick<8>(bf16, vec)
-                                                                  : pick<16>(bf16, vec);
-    const int tasks = (a.heads[0] + a.heads[1] + kHeads - 1) / kHeads;
+    const Kernel k = a.interleaved ? pick_lanes<true>(lanes, bf16, vec)
+                                   : pick_lanes<false>(lanes, bf16, vec);
+    // Heads per task: as many as leave every SM its 32 warps, at most 8.
+    const int64_t rows = a.tokens * (a.heads[0] + a.heads[1]);
+    Tasks t;
+    t.per = 1;
+    while (t.per < 8 && rows * lanes / (2 * t.per) >= (int64_t)148 * 32 * 32) t.per *= 2;
+    t.q_tasks = (a.heads[0] + t.per - 1) / t.per;
+    const int tasks = t.q_tasks + (a.heads[1] + t.per - 1) / t.per;
+    t.tasks = FastDiv((uint32_t)tasks);
     const int64_t threads = a.tokens * tasks * lanes;
     return launch_pdl(k, dim3((unsigned)((threads + kThreads - 1) / kThreads)), dim3(kThreads), 0,
-                      stream, a, tasks);
+                      stream, a, t);
 }
 
 cudaError_t read_qknorm_rope_status(int clear, int* status) {
