@@ -87,17 +87,34 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
     return r;
 }
 
+// K's fields as halves without an arithmetic instruction: the field with its
+// sign bit flipped, u = k + bias (bias 128 or 8), placed in the low bits of a
+// half is the subnormal u 2^-24 (u 2^-20 four bits up), exactly, and the tensor
+// cores take subnormals as they are.  What the bias adds to a score, bias sum_d
+// q_d, is taken off in fp32 with the scales.
+//
+// Bytes 0 and 2 of w as a pair; 1 and 3 are the same of w >> 8.
+__device__ __forceinline__ uint32_t biased_bytes02(uint32_t w) {
+    return lop3_sel_xor_i<0x00FF00FFu, 0x00800080u>(w);
+}
+// Nibbles 0 and 4 (2^-24), and 1 and 5 (2^-20), of w; 2, 6 and 3, 7 are the same of w >> 8.
+__device__ __forceinline__ uint32_t biased_nibbles04(uint32_t w) {
+    return lop3_sel_xor_i<0x000F000Fu, 0x00080008u>(w);
+}
+__device__ __forceinline__ uint32_t biased_nibbles15(uint32_t w) {
+    return lop3_sel_xor_i<0x00F000F0u, 0x00800080u>(w);
+}
+
+// V's fields as themselves: under an exponent of 1024 or 64, less that and the
+// flip of the sign bit.  (Without the subtraction the sum over the tokens would
+// carry the bias times the softmax's denominator, beside which O is small.)
 __device__ __forceinline__ uint32_t h2_add(uint32_t v, unsigned short bias) {
     const __half2 r = __hadd2(u32_as_h2(v), h2_const(bias));
     return *reinterpret_cast<const uint32_t*>(&r);
 }
-
-// Bytes 0 and 2 of w as a pair of halves (two's complement, exact); the pair
-// 1 and 3 is the same of w >> 8.
 __device__ __forceinline__ uint32_t bytes02(uint32_t w) {
     return h2_add(lop3_sel_xor_i<0x00FF00FFu, 0x64806480u>(w), kH_m1152);
 }
-// Nibbles 0 and 4, and 1 and 5, of w; 2, 6 and 3, 7 are the same of w >> 8.
 __device__ __forceinline__ uint32_t nibbles04(uint32_t w) {
     return h2_add(lop3_sel_xor_i<0x000F000Fu, 0x64086408u>(w), kH_m1032);
 }
@@ -509,34 +526,45 @@ __global__ void __launch_bounds__(kThreads, Shape<kDim, kBits, kNB>::kPerSm)
         const int len = chunked ? len0 : s_len[seg.seq];
         const int token0 = first_block(len) * kKvBlock - seg.begin * (kU * kKvBlock);
 
-        // q as B fragments.  bf16 rows are brought into fp16's range by a power
-        // of two (exact; elements 2^14 below their row's largest lose bits that
-        // fp32 sums would not keep either).
+        // q as B fragments.  Rows are brought to [1, 2) by a power of two (exact;
+        // elements 2^14 below their row's largest lose bits that fp32 sums would
+        // not keep either).  int4: the elements that meet nibbles of 2^-24 are
+        // scaled by 2^4, so that all products stand for q k 2^-20 (int8: 2^-24).
+        // rs brings a score to base-2 logits, qc is what the bias adds to it.
         uint32_t qf[kNB][kSteps][2];
-        float rs[kNB][2];
+        float rs[kNB][2], qc[kNB][2];
 #pragma unroll
         for (int n = 0; n < kNB; ++n) {
-            float x[kDim / 4];
+            float x[kDim / 4], top = 0.f, sum = 0.f;
 #pragma unroll
             for (int i = 0; i < kDim / 32; ++i) unpack8<kBf16>(qraw[n][i], x + 8 * i);
+#pragma unroll
+            for (int i = 0; i < kDim / 4; ++i) top = fmaxf(top, fabsf(x[i]));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            const int e = (int)(__float_as_uint(top) >> 23) - 127;
             float unit = a.scale * 1.4426950408889634f;
-            rs[n][0] = rs[n][1] = unit;
-            if (kBf16) {
-                float m = 0.f;
+            // zero, denormal and non-finite rows stay as they are
+            if (e > -126 && e < 127) {
+                const float down = __uint_as_float((uint32_t)(127 - e) << 23);
 #pragma unroll
-                for (int i = 0; i < kDim / 4; ++i) m = fmaxf(m, fabsf(x[i]));
-                m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
-                m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-                const int e = (int)(__float_as_uint(m) >> 23) - 127;
-                // zero, denormal and non-finite rows stay as they are
-                if (e > -126 && e < 127) {
-                    const float down = __uint_as_float((uint32_t)(127 - e) << 23);
+                for (int i = 0; i < kDim / 4; ++i) x[i] *= down;
+                unit *= __uint_as_float((uint32_t)(127 + e) << 23);
+            }
+            // the sum of the elements as the tensor cores get them
 #pragma unroll
-                    for (int i = 0; i < kDim / 4; ++i) x[i] *= down;
-                    unit *= __uint_as_float((uint32_t)(127 + e) << 23);
-                }
-                rs[n][0] = __shfl_sync(0xffffffffu, unit, 8 * t);
-                rs[n][1] = __shfl_sync(0xffffffffu, unit, 8 * t + 4);
+            for (int i = 0; i < kDim / 4; i += 2) {
+                const float2 h = __half22float2(__floats2half2_rn(x[i], x[i + 1]));
+                sum += h.x + h.y;
+            }
+            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+            sum *= (kBits == 8 ? 128.f : 8.f) * unit;
+            unit *= kBits == 8 ? 16777216.f : 1048576.f;  // 2^24, 2^20
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                rs[n][c] = __shfl_sync(0xffffffffu, unit, 8 * t + 4 * c);
+                qc[n][c] = __shfl_sync(0xffffffffu, sum, 8 * t + 4 * c);
             }
 #pragma unroll
             for (int w = 0; w < kKWords; ++w) {
@@ -544,9 +572,9 @@ __global__ void __launch_bounds__(kThreads, Shape<kDim, kBits, kNB>::kPerSm)
                     qf[n][w][0] = pack2<false>(x[4 * w], x[4 * w + 2]);
                     qf[n][w][1] = pack2<false>(x[4 * w + 1], x[4 * w + 3]);
                 } else {
-                    qf[n][2 * w][0] = pack2<false>(x[8 * w], x[8 * w + 4]);
+                    qf[n][2 * w][0] = pack2<false>(16.f * x[8 * w], 16.f * x[8 * w + 4]);
                     qf[n][2 * w][1] = pack2<false>(x[8 * w + 1], x[8 * w + 5]);
-                    qf[n][2 * w + 1][0] = pack2<false>(x[8 * w + 2], x[8 * w + 6]);
+                    qf[n][2 * w + 1][0] = pack2<false>(16.f * x[8 * w + 2], 16.f * x[8 * w + 6]);
                     qf[n][2 * w + 1][1] = pack2<false>(x[8 * w + 3], x[8 * w + 7]);
                 }
             }
@@ -597,17 +625,17 @@ __global__ void __launch_bounds__(kThreads, Shape<kDim, kBits, kNB>::kPerSm)
                         for (int w = 0; w < kKPer; ++w) {
                             const int x = i * kKPer + w;
                             if (kBits == 8) {
-                                const uint32_t f[4] = {bytes02(w0[w]), bytes02(w1[w]),
-                                                       bytes02(w0[w] >> 8), bytes02(w1[w] >> 8)};
+                                const uint32_t f[4] = {biased_bytes02(w0[w]), biased_bytes02(w1[w]),
+                                                       biased_bytes02(w0[w] >> 8), biased_bytes02(w1[w] >> 8)};
 #pragma unroll
                                 for (int n = 0; n < kNB; ++n)
                                     mma_16816(s[k][n], f, qf[n][x][0], qf[n][x][1]);
                             } else {
-                                const uint32_t e[4] = {nibbles04(w0[w]), nibbles04(w1[w]),
-                                                       nibbles15(w0[w]), nibbles15(w1[w])};
+                                const uint32_t e[4] = {biased_nibbles04(w0[w]), biased_nibbles04(w1[w]),
+                                                       biased_nibbles15(w0[w]), biased_nibbles15(w1[w])};
                                 const uint32_t h0 = w0[w] >> 8, h1 = w1[w] >> 8;
-                                const uint32_t f[4] = {nibbles04(h0), nibbles04(h1), nibbles15(h0),
-                                                       nibbles15(h1)};
+                                const uint32_t f[4] = {biased_nibbles04(h0), biased_nibbles04(h1), biased_nibbles15(h0),
+                                                       biased_nibbles15(h1)};
 #pragma unroll
                                 for (int n = 0; n < kNB; ++n) {
                                     mma_16816(s[k][n], e, qf[n][2 * x][0], qf[n][2 * x][1]);
@@ -632,7 +660,8 @@ __global__ void __launch_bounds__(kThreads, Shape<kDim, kBits, kNB>::kPerSm)
                         for (int n = 0; n < kNB; ++n)
 #pragma unroll
                             for (int c = 0; c < 2; ++c)
-                                s[k][n][2 * h + c] = fmaf(s[k][n][2 * h + c], ks * rs[n][c], lv);
+                                s[k][n][2 * h + c] = fmaf(s[k][n][2 * h + c], ks * rs[n][c],
+                                                          fmaf(-ks, qc[n][c], lv));
                     }
                 }
                 const int j0 = cu * (kU * kKvBlock) + token0;
