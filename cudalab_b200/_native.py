@@ -110,7 +110,9 @@ PROTOTYPES = {
     "cl_kvcache_write": (_int, [_vp] * 4 + [ctypes.POINTER(KvCacheDesc), _vp]),
     "cl_kvcache_read": (_int, [_vp] * 4 + [ctypes.POINTER(KvCacheDesc), _vp]),
     "cl_kvattention_workspace": (_int, [ctypes.POINTER(_size)]),
-    "cl_kvattention": (_int, [_vp] * 10 + [ctypes.POINTER(KvAttentionDesc), _vp]),
+    "cl_kvattention_prefix_floats": (_int, [ctypes.POINTER(KvAttentionDesc),
+                                            ctypes.POINTER(_size)]),
+    "cl_kvattention": (_int, [_vp] * 9 + [ctypes.POINTER(KvAttentionDesc), _vp]),
 }
 
 CL_MAX_PEERS = 8

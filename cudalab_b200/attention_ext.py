@@ -284,18 +284,23 @@ class KvAttentionExt(_Ext):
                  and out.device == dev and out.data_ptr() % 16 == 0,
                  f"out must be contiguous {q.dtype} {list(q.shape)} on {dev}, 16-byte aligned")
         lse = torch.empty(q.shape[:-1], dtype=torch.float32, device=dev) if return_lse else None
-        front = front_lse = None
         q4 = q.unsqueeze(1) if q.dim() == 3 else q
-        if prefix_length:
-            if q4.size(0) > 1 and q4.size(1) > 1 and q4.stride(0) != q4.size(1) * q4.stride(1):
-                q4 = q4.contiguous()
-            front = torch.empty(q.shape, dtype=torch.float32, device=dev)
-            front_lse = torch.empty(q.shape[:-1], dtype=torch.float32, device=dev)
+        if prefix_length and q4.size(0) > 1 and q4.size(1) > 1 \
+                and q4.stride(0) != q4.size(1) * q4.stride(1):
+            q4 = q4.contiguous()
         d = nat.KvAttentionDesc(
             pages.size(0), page_table.stride(0), q4.stride(0), q4.stride(1), q4.stride(2),
             q4.size(0), q4.size(1), q4.size(2), pages.size(1), D, bits, page_size,
             page_table.size(1), int(window), _TYPES[q.dtype], int(prefix_length), n_prefix,
             D ** -0.5 if scale is None else float(scale))
+
+        scratch = None
+        if prefix_length:
+            n = ctypes.c_size_t(0)
+            rc = self._lib.cl_kvattention_prefix_floats(ctypes.byref(d), ctypes.byref(n))
+            if rc != nat.CL_OK:
+                raise RuntimeError(f"{self.kind} failed ({rc}): {nat.last_error(self._lib)}")
+            scratch = torch.empty(n.value, dtype=torch.float32, device=dev)
 
         def ptr(x):
             return None if x is None else x.data_ptr()
@@ -303,7 +308,7 @@ class KvAttentionExt(_Ext):
         self._call(self._lib.cl_kvattention, dev, q4.data_ptr(), pages.data_ptr(),
                    page_table.data_ptr(), lengths.data_ptr(),
                    ptr(prefix_pages) if prefix_length else None, out.data_ptr(), ptr(lse),
-                   ptr(front), ptr(front_lse), workspace.data_ptr(), ctypes.byref(d))
+                   ptr(scratch), workspace.data_ptr(), ctypes.byref(d))
         return (out, lse) if return_lse else out
 
     def forward(self, q, pages, page_table, lengths, scale: float | None = None, window: int = 0,

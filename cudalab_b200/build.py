@@ -37,7 +37,7 @@ ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 # template instantiations)
 NVCC_FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "--split-compile", "0"]
 SOURCES = ["gemv_kernels.cu", "gemv_dense.cu", "quantize.cu", "qknorm_rope.cu", "kv_cache.cu",
-           "kv_attention.cu", "capi.cu"]
+           "kv_attention.cu", "kv_prefix.cu", "capi.cu"]
 
 
 def _nvcc() -> str:

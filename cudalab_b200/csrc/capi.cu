@@ -319,7 +319,8 @@ int cl_device_status(int clear, int* status_out) {
     if (!status_out) return fail(CL_ERR_INVALID_ARGUMENT, "status_out is null");
     // one word per translation unit with a status; the first nonzero one is reported
     cudaError_t (*const words[])(int, int*) = {clb::read_device_status,
-                                               clb::read_kv_attention_status, clb::read_kv_status,
+                                               clb::read_kv_attention_status, clb::read_kv_prefix_status,
+                                               clb::read_kv_status,
                                                clb::read_qknorm_rope_status};
     int status = 0;
     for (auto read : words) {
@@ -636,7 +637,7 @@ int type16(int dtype) {
 
 // The cache's format, shared by the cache and the attention calls.
 int check_cache(const char* op, int64_t num_pages, int kv_heads, int head_dim, int bits,
-                int page_size, const void* pages) {
+                int page_size) {
     if (head_dim != 64 && head_dim != 128 && head_dim != 256)
         return bad(op, "head_dim must be 64, 128 or 256");
     if (bits != 8 && bits != 4) return bad(op, "bits must be 8 or 4");
@@ -644,8 +645,6 @@ int check_cache(const char* op, int64_t num_pages, int kv_heads, int head_dim, i
     if (num_pages <= 0 || num_pages > INT32_MAX) return bad(op, "num_pages must be in [1, 2^31)");
     if (page_size <= 0 || page_size % clb::kKvBlock != 0 || page_size > (1 << 20))
         return bad(op, "page_size must be a multiple of 16, at most 2^20");
-    if (!pages) return bad(op, "null device pointer");
-    if (misaligned16(pages)) return bad(op, "pages must be 16-byte aligned");
     return CL_OK;
 }
 
@@ -655,9 +654,10 @@ int cache_args(const char* op, const void* k, const void* v, const void* pages, 
     if (d->tokens < 0) return bad(op, "tokens must be >= 0");
     const int type = type16(d->dtype);
     if (type < 0) return bad(op, "dtype must be CL_DTYPE_F16 or CL_DTYPE_BF16");
-    const int rc = check_cache(op, d->num_pages, d->kv_heads, d->head_dim, d->bits, d->page_size, pages);
+    const int rc = check_cache(op, d->num_pages, d->kv_heads, d->head_dim, d->bits, d->page_size);
     if (rc != CL_OK) return rc;
-    if (d->tokens > 0 && (!k || !v || !slots)) return bad(op, "null device pointer");
+    if (!pages || (d->tokens > 0 && (!k || !v || !slots))) return bad(op, "null device pointer");
+    if (misaligned16(pages)) return bad(op, "pages must be 16-byte aligned");
     if (d->tokens > (((int64_t)1 << 31) - 256) / d->kv_heads)
         return bad(op, "too many tokens for one launch");
     *a = clb::KvCacheArgs{const_cast<uint8_t*>(static_cast<const uint8_t*>(pages)), slots,
@@ -741,15 +741,32 @@ int cl_kvattention_workspace(size_t* bytes) {
     return CL_OK;
 }
 
-int cl_kvattention(const void* q, const uint8_t* pages, const int32_t* page_table,
-                   const int32_t* lengths, const int32_t* prefix_pages, void* out, float* lse,
-                   float* prefix_out, float* prefix_lse, void* workspace,
-                   const cl_kvattention_desc* d, void* stream) {
-    const char* op = "kvattention";
+namespace {
+
+// The launch over the prefix: the whole batch as the new tokens of one
+// sequence that sees all of it.
+clb::KvAttentionArgs prefix_args(const cl_kvattention_desc* d) {
+    clb::KvAttentionArgs f{};
+    f.q_new = d->new_tokens > 1 ? d->q_new : d->q_batch;
+    f.q_head = d->q_head;
+    f.num_pages = d->num_pages;
+    f.max_pages = d->prefix_page_count;
+    f.fixed_length = d->prefix_length;
+    f.batch = 1;
+    f.new_tokens = d->batch * d->new_tokens;
+    f.kv_heads = d->kv_heads;
+    f.group = d->q_heads / d->kv_heads;
+    f.head_dim = d->head_dim;
+    f.bits = d->bits;
+    f.page_size = d->page_size;
+    f.scale = d->scale;
+    return f;
+}
+
+int check_attention(const char* op, const cl_kvattention_desc* d) {
     if (!d) return bad(op, "null descriptor");
-    const int type = type16(d->dtype);
-    if (type < 0) return bad(op, "dtype must be CL_DTYPE_F16 or CL_DTYPE_BF16");
-    int rc = check_cache(op, d->num_pages, d->kv_heads, d->head_dim, d->bits, d->page_size, pages);
+    if (type16(d->dtype) < 0) return bad(op, "dtype must be CL_DTYPE_F16 or CL_DTYPE_BF16");
+    const int rc = check_cache(op, d->num_pages, d->kv_heads, d->head_dim, d->bits, d->page_size);
     if (rc != CL_OK) return rc;
     if (d->batch < 0 || d->batch > 4096) return bad(op, "batch must be in [0, 4096]");
     if (d->new_tokens <= 0 || d->new_tokens > (1 << 20))
@@ -763,11 +780,45 @@ int cl_kvattention(const void* q, const uint8_t* pages, const int32_t* page_tabl
     if (d->max_pages < 0 || (int64_t)d->max_pages * d->page_size > INT32_MAX)
         return bad(op, "max_pages * page_size exceeds 2^31 - 1 tokens");
     if (d->prefix_length < 0 || d->prefix_page_count < 0) return bad(op, "negative prefix");
+    if (d->prefix_length > 0) {
+        if (d->window != 0) return bad(op, "a prefix and a window exclude each other");
+        if ((int64_t)d->prefix_page_count * d->page_size > INT32_MAX)
+            return bad(op, "prefix_page_count * page_size exceeds 2^31 - 1 tokens");
+        if ((int64_t)d->prefix_page_count * d->page_size < d->prefix_length)
+            return bad(op, "prefix_pages hold fewer than prefix_length tokens");
+        if (d->batch > 1 && d->new_tokens > 1 && d->q_batch != d->new_tokens * d->q_new)
+            return bad(op, "with a prefix the q rows must be evenly spaced");
+    }
+    return CL_OK;
+}
+
+}  // namespace
+
+int cl_kvattention_prefix_floats(const cl_kvattention_desc* d, size_t* floats) {
+    const char* op = "kvattention_prefix_floats";
+    if (!floats) return bad(op, "floats is null");
+    const int rc = check_attention(op, d);
+    if (rc != CL_OK) return rc;
+    *floats = 0;
+    if (d->prefix_length == 0 || d->batch == 0) return CL_OK;
+    const clb::KvAttentionArgs f = prefix_args(d);
+    const int parts = clb::kv_prefix_takes(f) ? clb::kv_prefix_parts(f) : 1;
+    *floats = (size_t)parts * d->batch * d->new_tokens * d->q_heads * (d->head_dim + 1);
+    return CL_OK;
+}
+
+int cl_kvattention(const void* q, const uint8_t* pages, const int32_t* page_table,
+                   const int32_t* lengths, const int32_t* prefix_pages, void* out, float* lse,
+                   float* prefix_scratch, void* workspace, const cl_kvattention_desc* d,
+                   void* stream) {
+    const char* op = "kvattention";
+    const int rc = check_attention(op, d);
+    if (rc != CL_OK) return rc;
     if (d->batch == 0) return CL_OK;
-    if (!q || !out || !workspace || !lengths || (d->max_pages > 0 && !page_table))
+    if (!q || !pages || !out || !workspace || !lengths || (d->max_pages > 0 && !page_table))
         return bad(op, "null device pointer");
-    if (misaligned16(out) || misaligned16(workspace))
-        return bad(op, "out and workspace must be 16-byte aligned");
+    if (misaligned16(pages) || misaligned16(out) || misaligned16(workspace))
+        return bad(op, "pages, out and workspace must be 16-byte aligned");
     clb::KvAttentionArgs a{};
     a.q = q;
     a.q_batch = d->q_batch;
@@ -787,51 +838,37 @@ int cl_kvattention(const void* q, const uint8_t* pages, const int32_t* page_tabl
     a.head_dim = d->head_dim;
     a.bits = d->bits;
     a.page_size = d->page_size;
-    a.type = type;
+    a.type = type16(d->dtype);
     a.causal = 1;
     a.window = d->window;
     a.scale = d->scale;
     a.out = out;
     a.lse = lse;
     a.workspace = workspace;
-    const clb::KvAttentionArgs* both[2] = {&a, nullptr};
-    clb::KvAttentionArgs f = a;
+    if (!clb::kv_attention_fits(a))
+        return bad(op, "the page tables span too many blocks for one launch");
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (d->prefix_length > 0) {
-        if (d->window != 0) return bad(op, "a prefix and a window exclude each other");
-        if ((int64_t)d->prefix_page_count * d->page_size > INT32_MAX)
-            return bad(op, "prefix_page_count * page_size exceeds 2^31 - 1 tokens");
-        if ((int64_t)d->prefix_page_count * d->page_size < d->prefix_length)
-            return bad(op, "prefix_pages hold fewer than prefix_length tokens");
-        if (!prefix_pages || !prefix_out || !prefix_lse) return bad(op, "null prefix pointer");
-        if (misaligned16(prefix_out)) return bad(op, "prefix_out must be 16-byte aligned");
-        if (d->batch > 1 && d->new_tokens > 1 && d->q_batch != d->new_tokens * d->q_new)
-            return bad(op, "with a prefix the q rows must be evenly spaced");
-        // the whole batch as the new tokens of one sequence that sees all of it
-        f.q_new = d->new_tokens > 1 ? d->q_new : d->q_batch;
+        if (!prefix_pages || !prefix_scratch) return bad(op, "null prefix pointer");
+        if (misaligned16(prefix_scratch)) return bad(op, "prefix_scratch must be 16-byte aligned");
+        clb::KvAttentionArgs f = prefix_args(d);
+        f.q = q;
+        f.pages = pages;
         f.table = prefix_pages;
-        f.table_stride = 0;
-        f.max_pages = d->prefix_page_count;
-        f.fixed_length = d->prefix_length;
-        f.batch = 1;
-        f.new_tokens = d->batch * d->new_tokens;
-        f.causal = 0;
-        f.out = nullptr;
-        f.out_f32 = prefix_out;
-        f.lse = prefix_lse;
-        a.front = prefix_out;
-        a.front_lse = prefix_lse;
-        both[0] = &f;
-        both[1] = &a;
+        f.type = a.type;
+        f.workspace = workspace;
+        if (!clb::kv_attention_fits(f))
+            return bad(op, "the prefix spans too many blocks for one launch");
+        const bool tensor = clb::kv_prefix_takes(f);
+        a.front_parts = tensor ? clb::kv_prefix_parts(f) : 1;
+        a.front = f.out_f32 = prefix_scratch;
+        a.front_lse = f.lse = prefix_scratch + (size_t)a.front_parts * d->batch * d->new_tokens *
+                                                   d->q_heads * d->head_dim;
+        const cudaError_t e = tensor ? clb::launch_kv_prefix(f, s) : clb::launch_kv_attention(f, s);
+        if (e != cudaSuccess) return cuda_fail(e, "kvattention prefix launch");
     }
-    for (const clb::KvAttentionArgs* one : both) {
-        if (one && !clb::kv_attention_fits(*one))
-            return bad(op, "the page tables span too many blocks for one launch");
-    }
-    for (const clb::KvAttentionArgs* one : both) {
-        if (!one) continue;
-        cudaError_t e = clb::launch_kv_attention(*one, static_cast<cudaStream_t>(stream));
-        if (e != cudaSuccess) return cuda_fail(e, "kvattention launch");
-    }
+    const cudaError_t e = clb::launch_kv_attention(a, s);
+    if (e != cudaSuccess) return cuda_fail(e, "kvattention launch");
     return CL_OK;
 }
 

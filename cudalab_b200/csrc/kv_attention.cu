@@ -319,17 +319,24 @@ __global__ void __launch_bounds__(kThreads, Shape<kDim, kBits, kNB>::kPerSm)
         o.x *= inv, o.y *= inv, o.z *= inv, o.w *= inv;
         if (a.front != nullptr) {
             constexpr float kLog2e = 1.4426950408889634f;
-            const float4 f = __ldcg(reinterpret_cast<const float4*>(a.front + row * kDim + d));
-            const float fl = __ldcg(a.front_lse + row) * kLog2e;
-            const float top = fmaxf(lse2, fl);
-            const float ref = top == -INFINITY ? 0.f : top;
-            const float wo = ex2(lse2 - ref), wf = ex2(fl - ref), sum = wo + wf;
+            const int64_t all = (int64_t)a.batch * a.new_tokens * a.kv_heads * a.group;
+            float sum = lse2 == -INFINITY ? 0.f : 1.f, top = lse2;
+#pragma unroll 4
+            for (int f = 0; f < a.front_parts; ++f) {
+                const int64_t at = f * all + row;
+                const float4 x = __ldcg(reinterpret_cast<const float4*>(a.front + at * kDim + d));
+                const float fl = __ldcg(a.front_lse + at) * kLog2e;
+                const float next = fmaxf(top, fl);
+                const float ref = next == -INFINITY ? 0.f : next;
+                const float wo = ex2(top - ref), wf = ex2(fl - ref);
+                top = next;
+                sum = sum * wo + wf;
+                o.x = o.x * wo + x.x * wf, o.y = o.y * wo + x.y * wf;
+                o.z = o.z * wo + x.z * wf, o.w = o.w * wo + x.w * wf;
+            }
             const float i2 = sum > 0.f ? 1.f / sum : (sum == sum ? 0.f : sum);
-            o.x = (o.x * wo + f.x * wf) * i2;
-            o.y = (o.y * wo + f.y * wf) * i2;
-            o.z = (o.z * wo + f.z * wf) * i2;
-            o.w = (o.w * wo + f.w * wf) * i2;
-            lse2 = sum > 0.f ? ref + lg2(sum) : (sum == sum ? -INFINITY : sum);
+            o.x *= i2, o.y *= i2, o.z *= i2, o.w *= i2;
+            lse2 = sum > 0.f ? top + lg2(sum) : (sum == sum ? -INFINITY : sum);
         }
         if (a.out_f32 != nullptr)
             *reinterpret_cast<float4*>(a.out_f32 + row * kDim + d) = o;

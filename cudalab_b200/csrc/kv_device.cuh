@@ -31,11 +31,14 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
 template <bool kBf16, bool kVec>
 __device__ __forceinline__ uint4 load8(const void* p, int64_t at) {
     const uint16_t* e = static_cast<const uint16_t*>(p) + at;
-    if (kVec) return *reinterpret_cast<const uint4*>(e);
-    uint32_t w[4];
+    if constexpr (kVec) {
+        return *reinterpret_cast<const uint4*>(e);
+    } else {
+        uint32_t w[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = (uint32_t)e[2 * i] | ((uint32_t)e[2 * i + 1] << 16);
-    return make_uint4(w[0], w[1], w[2], w[3]);
+        for (int i = 0; i < 4; ++i) w[i] = (uint32_t)e[2 * i] | ((uint32_t)e[2 * i + 1] << 16);
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    }
 }
 
 template <bool kVec>

@@ -100,8 +100,9 @@ struct KvAttentionArgs {
     void* out;        // [batch, new, heads, head_dim] contiguous (type), or null
     float* out_f32;   // the same in fp32 instead (partial results), or null
     float* lse;       // [batch, new, heads] natural log, or null (required with out_f32)
-    const float* front;      // fp32 result over tokens in front of these, or null
-    const float* front_lse;  // its lse
+    const float* front;      // fp32 results over tokens in front of these, or null:
+    const float* front_lse;  // [front_parts] of them and their lse
+    int front_parts;
     void* workspace;
 };
 // Workspace bytes of a call (zero-filled before its first use).
@@ -110,6 +111,15 @@ size_t kv_attention_workspace();
 // table allows.
 bool kv_attention_fits(const KvAttentionArgs& a);
 cudaError_t launch_kv_attention(const KvAttentionArgs& a, cudaStream_t stream);
+
+// Attention of all rows (new_tokens of one sequence) over fixed_length tokens that
+// every row sees, on the tensor cores (kv_prefix.cu): whether it is the faster
+// kernel for these arguments, the partial results it writes (out_f32 and lse
+// hold that many, one after the other), the launch.
+bool kv_prefix_takes(const KvAttentionArgs& a);
+int kv_prefix_parts(const KvAttentionArgs& a);
+cudaError_t launch_kv_prefix(const KvAttentionArgs& a, cudaStream_t stream);
+cudaError_t read_kv_prefix_status(int clear, int* status);
 
 // Reads (optionally clears) the status word of the cache kernels.
 cudaError_t read_kv_status(int clear, int* status);

@@ -1,0 +1,703 @@
+// Attention of many query rows over one run of cached tokens that all of them
+// see: the prefix that a batch shares (layout of the cache: kv_layout.cuh).
+//
+//   s_j = scale * ks_j * (q . k_j),  o = sum_j e^(s_j) vs_j v_j / sum_j e^(s_j)
+//
+// With a batch's worth of rows per cache head the operation is bound by
+// arithmetic, 4 rows tokens head_dim operations per head against tokens
+// (2 head_dim bits / 8 + 4) bytes, so it runs on the 5th-generation tensor
+// cores.  A CTA takes 128 rows (lanes of Tensor Memory) and a range of tokens,
+// 128 at a time:
+//   * 8 warps expand the tile's 8 cache blocks, one block a warp, to exact fp16
+//     whole values in shared memory (rows of tokens, 64 elements wide, 128-byte
+//     swizzle), read one tile ahead into registers; the scales become three
+//     numbers per token in fp32;
+//   * one thread issues the MMAs (M = N = 128, K = 16, fp32 accumulators): S =
+//     Q K^T with Q in Tensor Memory and K as stored (K-major), O += P V with P in
+//     Tensor Memory and the same layout of V read across (MN-major);
+//   * 4 warps, a row a thread, do the softmax as in kv_attention.cu: weights
+//     w_j = 2^(s_j + log2 vs_j - m) in fp16, the sum of w_j / vs_j in fp32, one
+//     lazy reference m per row, packed fp32 pairs; O is only rescaled when a
+//     score exceeds the reference by more than kSlack.
+// S is double-buffered: the tensor cores compute tile i + 1's S and tile i -
+// 1's O while the softmax of tile i runs.  Tokens past the prefix get a weight
+// of zero from their three numbers, so no tile is special.
+//
+// Tensor Memory (512 columns): S 2 x 128, O head_dim, P 64, Q head_dim / 2.
+// int4: a byte's nibbles leave their word as pairs (0, 4) (1, 5) (2, 6) (3, 7),
+// so K, Q and V all keep that order of the 8 elements of a 16-byte piece; the
+// sum over them does not mind, and O's columns are put back when it is written.
+//
+// The tokens are cut so that heads x row tiles x parts fill the SMs; each part
+// writes a normalised fp32 result and its lse, joined by the launch over the
+// sequences' own tokens.  Every wait is bounded (status 8 on expiry).
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cstdint>
+
+#include "gemv_common.cuh"
+#include "gemv_launch.h"
+#include "kv_device.cuh"
+#include "kv_layout.cuh"
+
+namespace clb {
+namespace {
+
+__device__ int g_kv_prefix_status;
+
+constexpr int kRows = 128, kTile = 128;  // query rows and tokens of a tile
+constexpr int kSoftWarps = 4, kFillWarps = 8;
+constexpr int kMmaWarp = kSoftWarps + kFillWarps;
+constexpr int kThreads = 32 * (kMmaWarp + 1);
+constexpr float kSlack = 8.f;
+constexpr uint32_t kColS = 0, kColO = 256, kColP = 384, kColQ = 448, kColumns = 512;
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float lg2(float x) {
+    float y;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ unsigned long long f2_mul(unsigned long long a, unsigned long long b) {
+    unsigned long long d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+
+__device__ __forceinline__ void fence_before() {
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+}
+__device__ __forceinline__ void fence_after() {
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+}
+__device__ __forceinline__ void wait_st() {
+    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void commit(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
+                     bar)
+                 : "memory");
+}
+
+// D[tmem] (+)= A[tmem] x B[smem].
+__device__ __forceinline__ void mma(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc,
+                                    uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %3, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %4, {%5, %5, %5, %5}, p;\n\t}"
+        ::"r"(d), "r"(a), "l"(b), "r"(accumulate), "r"(idesc), "r"(0u)
+        : "memory");
+}
+
+// Instruction descriptor of kind::f16: D fp32 (bits 4-5 = 1), A and B fp16, A
+// K-major, B K-major or MN-major (bit 16), N >> 3 at bit 17, M >> 4 at bit 24.
+__host__ __device__ constexpr uint32_t instruction(int n, bool b_mn_major) {
+    return (1u << 4) | ((uint32_t)b_mn_major << 16) | ((uint32_t)(n >> 3) << 17) |
+           ((uint32_t)(kRows >> 4) << 24);
+}
+// Shared-memory descriptor of a 128-byte swizzled operand: 8-row groups of 1024
+// bytes (stride 1024 at bit 32), the next 64 columns `wide` bytes on (bit 16;
+// MN-major only), version 1 (bit 46), 128-byte swizzle (2 at bit 61).
+__device__ __forceinline__ uint64_t operand(uint32_t addr, uint32_t wide) {
+    return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)((wide >> 4) & 0x3FFFu) << 16) |
+           ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+
+// 32 columns of this thread's lane: issue, and the wait that makes them valid.
+__device__ __forceinline__ void ld32(uint32_t addr, uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, "
+        "%12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, "
+        "%30, %31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+          "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+          "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]),
+          "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]),
+          "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(addr)
+        : "memory");
+}
+__device__ __forceinline__ void ld_wait(uint32_t (&r)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]),
+                   "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]),
+                   "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]),
+                   "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
+                   "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]),
+                   "+r"(r[30]), "+r"(r[31])
+                 :
+                 : "memory");
+}
+__device__ __forceinline__ void st32(uint32_t addr, const uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, "
+        "%12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, "
+        "%30, %31, %32};" ::"r"(addr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+        "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]),
+        "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]),
+        "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]),
+        "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+__device__ __forceinline__ void st16(uint32_t addr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, "
+        "%12, %13, %14, %15, %16};" ::"r"(addr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+        "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]),
+        "r"(r[15])
+        : "memory");
+}
+
+struct PrefixParams {
+    KvAttentionArgs a;
+    FastDiv group, page_blocks;
+    int rows;        // per cache head
+    int row_tiles, parts, part_tiles, tiles;
+    int q_vec;
+    long long wait_cycles;
+};
+
+template <int kDim, int kBits>
+struct PrefixShape {
+    static constexpr int kRow = kDim * kBits / 8;
+    static constexpr int kBlockBytes = kv_block_bytes(kRow);
+    static constexpr int kHalves = kDim / 64;             // 64-element columns of an operand
+    static constexpr int kHalfBytes = kTile * 128;
+    static constexpr int kOperandBytes = kHalves * kHalfBytes;
+    static constexpr int kLoads = kRow / 32;              // 16-byte pieces per lane of a part
+    static constexpr int kOutStride = kDim * 4 + 16;      // bytes of a staged output row
+    // K and V twice each (the output is staged there at the end), per-token
+    // numbers, barriers; at least 120 KB, so that one CTA has an SM and its
+    // Tensor Memory.
+    static constexpr int kNumbers = 4 * kOperandBytes;
+    static constexpr int kBars = kNumbers + 2 * 3 * kTile * 4;
+    static constexpr int kSmem = (kBars + 128 < 120 * 1024 ? 120 * 1024 : kBars + 128) + 1024;
+    static_assert(kRows * kOutStride <= 4 * kOperandBytes, "room for the output");
+};
+
+// The 16-byte piece of a part that a lane holds in load `i`: its token row and
+// logical piece.  The lanes that store together (8) then fall on different
+// banks: int8 on two rows, int4 on four.
+template <int kBits>
+__device__ __forceinline__ void piece(int i, int lane, int* row, int* chunk, int halves) {
+    if (kBits == 8) {
+        *row = 8 * (i / halves) + (lane >> 2);
+        *chunk = 4 * (i % halves) + (lane & 3);
+    } else {
+        *row = lane >> 1;
+        *chunk = 2 * i + (lane & 1);
+    }
+}
+
+// One 16-byte piece of whole values -> 2 (int8) or 4 (int4) 16-byte pieces of
+// halves in the operand's row `token`.
+template <int kBits>
+__device__ __forceinline__ void expand(const uint4 raw, uint8_t* operand_base, int half_bytes,
+                                       int token, int chunk) {
+    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+    constexpr int kOut = 16 / kBits;  // pieces out
+    const int first = kOut * chunk;
+    uint8_t* row = operand_base + (first >> 3) * half_bytes + token * 128;
+#pragma unroll
+    for (int s = 0; s < kOut; ++s) {
+        __half2 q[4];
+        if (kBits == 8) {
+            __half2 lo[2], hi[2];
+            int8x4_to_h2(w[2 * s], lo);
+            int8x4_to_h2(w[2 * s + 1], hi);
+            q[0] = lo[0], q[1] = lo[1], q[2] = hi[0], q[3] = hi[1];
+        } else {
+            const uint32_t up = w[s] >> 8;
+            q[0] = __hadd2(u32_as_h2(lop3_sel_xor_i<0x000F000Fu, 0x64086408u>(w[s])), h2_const(kH_m1032));
+            q[1] = __hadd2(u32_as_h2(lop3_sel_xor_i<0x00F000F0u, 0x54805480u>(w[s])), h2_const(kH_m72));
+            q[2] = __hadd2(u32_as_h2(lop3_sel_xor_i<0x000F000Fu, 0x64086408u>(up)), h2_const(kH_m1032));
+            q[3] = __hadd2(u32_as_h2(lop3_sel_xor_i<0x00F000F0u, 0x54805480u>(up)), h2_const(kH_m72));
+        }
+        *reinterpret_cast<uint4*>(row + (((first + s) & 7) ^ (token & 7)) * 16) =
+            *reinterpret_cast<const uint4*>(q);
+    }
+}
+
+template <int kDim, int kBits, bool kBf16>
+__global__ void __launch_bounds__(kThreads, 1) kv_prefix_kernel(const PrefixParams p) {
+    using S = PrefixShape<kDim, kBits>;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>(
+        (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+    uint8_t* kbuf = smem;                          // [2] K operands
+    uint8_t* vbuf = smem + 2 * S::kOperandBytes;   // [2] V operands
+    float* numbers = reinterpret_cast<float*>(smem + S::kNumbers);  // [2][3][kTile]
+    const uint32_t bars = smem_u32(smem + S::kBars);
+    const uint32_t kfull = bars, vfull = bars + 16, kempty = bars + 32, vempty = bars + 48,
+                   sfull = bars + 64, pfull = bars + 80;
+    volatile uint32_t* s_tmem = reinterpret_cast<volatile uint32_t*>(smem + S::kBars + 96);
+    volatile int* s_fail = reinterpret_cast<volatile int*>(smem + S::kBars + 100);
+
+    const KvAttentionArgs& a = p.a;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int part = (int)blockIdx.x % p.parts, rest = (int)blockIdx.x / p.parts;
+    const int head = rest % a.kv_heads, row0 = rest / a.kv_heads * kRows;
+    const int tile0 = part * p.part_tiles;
+    const int tiles = min(p.part_tiles, p.tiles - tile0);
+    const int length = a.fixed_length;
+
+    pdl_allow_dependents();
+    if (tid == 0) {
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(kfull + 8 * i, kFillWarps);
+            mbar_init(vfull + 8 * i, kFillWarps);
+            mbar_init(kempty + 8 * i, 1);
+            mbar_init(vempty + 8 * i, 1);
+            mbar_init(sfull + 8 * i, 1);
+        }
+        mbar_init(pfull, kSoftWarps);
+        *s_fail = 0;
+        fence_barrier_init();
+    }
+    pdl_wait_prior_grids();
+    if (warp == 0) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                         smem_u32(const_cast<uint32_t*>(s_tmem))),
+                     "r"(kColumns)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = *s_tmem;
+
+    // A bounded wait; false (for the whole warp or the one thread) once any
+    // role has given up.
+    auto wait = [&](uint32_t bar, int phase) -> bool {
+        bool ok = *s_fail == 0 && mbar_wait_bounded(bar, (uint32_t)phase & 1u, p.wait_cycles);
+        if (!ok && *s_fail == 0) {
+            atomicCAS(&g_kv_prefix_status, 0, kStatusTimeoutKv);
+            *s_fail = 1;
+        }
+        return ok;
+    };
+
+    float sum_l = 0.f, ref = 0.f;  // of this thread's row
+    bool finished = false;         // softmax warps: all tiles done
+
+    if (warp < kSoftWarps) {
+        // ---------------- softmax: one row a thread ----------------
+        const uint32_t lane_base = tmem + ((uint32_t)(32 * warp) << 16);
+        const int r = row0 + 32 * warp + lane;
+        float unit = 1.f;  // what the row was divided by (a power of two)
+        {
+            const int i0 = p.group.div(r);
+            const uint16_t* src = static_cast<const uint16_t*>(a.q) + i0 * a.q_new +
+                                  ((head - i0) * a.group + r) * a.q_head;
+            auto load = [&](int d) {
+                if (r >= p.rows) return make_uint4(0, 0, 0, 0);
+                return p.q_vec ? load8<kBf16, true>(src, d) : load8<kBf16, false>(src, d);
+            };
+            // bf16 rows that fp16 would not hold are scaled into its range
+            float down = 1.f;
+            if (kBf16) {
+                float top = 0.f;
+#pragma unroll 1
+                for (int d = 0; d < kDim; d += 8) {
+                    float x[8];
+                    unpack8<kBf16>(load(d), x);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[i]));
+                }
+                const int e = (int)(__float_as_uint(top) >> 23) - 127;
+                if ((e >= 15 || e < -6) && e > -126 && e < 127) {
+                    down = __uint_as_float((uint32_t)(127 - e) << 23);
+                    unit = __uint_as_float((uint32_t)(127 + e) << 23);
+                }
+            }
+#pragma unroll 1
+            for (int d = 0; d < kDim; d += 32) {
+                uint32_t packed[16];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    float x[8];
+                    unpack8<kBf16>(load(d + 8 * c), x);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) x[i] *= down;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        packed[4 * c + i] = kBits == 8 ? pack2<false>(x[2 * i], x[2 * i + 1])
+                                                       : pack2<false>(x[i], x[i + 4]);
+                }
+                st16(lane_base + kColQ + d / 2, packed);
+            }
+            wait_st();
+            fence_before();
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(pfull);  // phase 0: Q is there
+
+        const bool scaled = __any_sync(0xffffffffu, unit != 1.f);
+        const unsigned long long unit2 = f2_pack(unit, unit);
+        unsigned long long l2 = f2_pack(0.f, 0.f);
+        bool ok = true;
+        for (int i = 0; i < tiles && ok; ++i) {
+            const int b = i & 1;
+            ok = wait(sfull + 8 * b, i >> 1) && wait(vfull + 8 * b, i >> 1);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            fence_after();
+            const uint32_t s_at = lane_base + kColS + 128 * b;
+            const float* num = numbers + b * 3 * kTile;
+            // z of 4 columns, less the reference
+            auto logits = [&](const uint32_t* s, int col, float nref, unsigned long long& z0,
+                              unsigned long long& z1) {
+                const ulonglong2 ks = *reinterpret_cast<const ulonglong2*>(num + col);
+                const ulonglong2 lv = *reinterpret_cast<const ulonglong2*>(num + kTile + col);
+                unsigned long long x0 = f2_pack(__uint_as_float(s[0]), __uint_as_float(s[1]));
+                unsigned long long x1 = f2_pack(__uint_as_float(s[2]), __uint_as_float(s[3]));
+                if (scaled) x0 = f2_mul(x0, unit2), x1 = f2_mul(x1, unit2);
+                const unsigned long long n2 = f2_pack(nref, nref);
+                z0 = f2_fma(x0, ks.x, f2_add(lv.x, n2));
+                z1 = f2_fma(x1, ks.y, f2_add(lv.y, n2));
+            };
+            // The reference from the tile's own scores: at the start, and when
+            // a score has outgrown it.
+            auto new_reference = [&]() {
+                float top = -INFINITY;
+#pragma unroll 1
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t s[32];
+                    ld32(s_at + 32 * c, s);
+                    ld_wait(s);
+#pragma unroll
+                    for (int j = 0; j < 32; j += 4) {
+                        unsigned long long z0, z1;
+                        float x, y, z, w;
+                        logits(s + j, 32 * c + j, 0.f, z0, z1);
+                        f2_unpack(z0, x, y);
+                        f2_unpack(z1, z, w);
+                        top = fmaxf(fmaxf(fmaxf(top, x), y), fmaxf(z, w));
+                    }
+                }
+                return top;
+            };
+            bool waited = false;  // for the MMAs of tile i - 1, which read P and write O
+            auto previous_done = [&]() {
+                if (!waited && i > 0) {
+                    ok = wait(vempty + 8 * ((i - 1) & 1), (i - 1) >> 1);
+                    ok = __all_sync(0xffffffffu, ok);
+                    fence_after();
+                }
+                waited = true;
+                return ok;
+            };
+            if (i == 0) {
+                const float top = new_reference();
+                ref = top == -INFINITY ? 0.f : top;  // only a NaN row has no largest score
+            }
+            for (;;) {
+                unsigned long long try_l = l2;
+                float most = -INFINITY;
+                uint32_t s[2][32];
+                ld32(s_at, s[0]);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t(&cur)[32] = s[c & 1];
+                    ld_wait(cur);
+                    if (c < 3) ld32(s_at + 32 * (c + 1), s[(c + 1) & 1]);
+                    uint32_t packed[16];
+#pragma unroll
+                    for (int j = 0; j < 32; j += 4) {
+                        unsigned long long z0, z1;
+                        float x, y, z, w;
+                        logits(cur + j, 32 * c + j, -ref, z0, z1);
+                        f2_unpack(z0, x, y);
+                        f2_unpack(z1, z, w);
+                        most = fmaxf(fmaxf(fmaxf(most, x), y), fmaxf(z, w));
+                        x = ex2(x), y = ex2(y), z = ex2(z), w = ex2(w);
+                        const ulonglong2 iv = *reinterpret_cast<const ulonglong2*>(
+                            num + 2 * kTile + 32 * c + j);
+                        try_l = f2_fma(f2_pack(x, y), iv.x, try_l);
+                        try_l = f2_fma(f2_pack(z, w), iv.y, try_l);
+                        packed[j / 2] = pack2<false>(x, y);
+                        packed[j / 2 + 1] = pack2<false>(z, w);
+                    }
+                    if (c == 0 && !previous_done()) break;
+                    st16(lane_base + kColP + 16 * c, packed);
+                }
+                if (!ok) break;
+                if (!__any_sync(0xffffffffu, most > kSlack)) {
+                    l2 = try_l;
+                    break;
+                }
+                // rescale what there is and take the tile again
+                wait_st();
+                const float top = fmaxf(ref, new_reference());
+                const float f = ex2(ref - top);
+                ref = top;
+                l2 = f2_mul(l2, f2_pack(f, f));
+                if (i > 0) {
+#pragma unroll 1
+                    for (int c = 0; c < kDim; c += 32) {
+                        uint32_t o[32];
+                        ld32(lane_base + kColO + c, o);
+                        ld_wait(o);
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+                        st32(lane_base + kColO + c, o);
+                    }
+                    wait_st();
+                }
+            }
+            if (!ok) break;
+            wait_st();
+            fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(pfull);
+        }
+        if (ok && __all_sync(0xffffffffu, wait(vempty + 8 * ((tiles - 1) & 1), (tiles - 1) >> 1))) {
+            fence_after();
+            finished = true;
+            float x, y;
+            f2_unpack(l2, x, y);
+            sum_l = x + y;
+        }
+        // nothing of this thread is in flight when the memory is freed
+        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+        wait_st();
+    } else if (warp < kMmaWarp) {
+        // ---------------- expansion: one cache block a warp ----------------
+        const int w = warp - kSoftWarps;
+        uint32_t where = 0xffffffffu;  // lane i: the block of the 32-tile batch's i-th tile
+        uint4 raw[2][S::kLoads];
+        __half scale = __half(0.f);
+        bool there = false;
+        auto fetch = [&](int i) {  // tile i's block into registers
+            if ((i & 31) == 0) {
+                const int blk = (tile0 + i + lane) * 8 + w;
+                where = 0xffffffffu;
+                if (i + lane < tiles && blk * kKvBlock < length) {
+                    const int index = p.page_blocks.div(blk);
+                    const int page = __ldg(a.table + index);
+                    if (page >= 0 && page < a.num_pages)
+                        where = ((uint32_t)page * a.kv_heads + head) * p.page_blocks.d +
+                                (blk - index * p.page_blocks.d);
+                    else
+                        atomicCAS(&g_kv_prefix_status, 0, kStatusKvIndex);
+                }
+            }
+            const uint32_t at = __shfl_sync(0xffffffffu, where, i & 31);
+            there = at != 0xffffffffu;
+            if (!there) {
+#pragma unroll
+                for (int x = 0; x < 2; ++x)
+#pragma unroll
+                    for (int n = 0; n < S::kLoads; ++n) raw[x][n] = make_uint4(0, 0, 0, 0);
+                scale = __half(0.f);
+                return;
+            }
+            const uint8_t* block = a.pages + (int64_t)at * S::kBlockBytes;
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+#pragma unroll
+                for (int n = 0; n < S::kLoads; ++n) {
+                    int row, chunk;
+                    piece<kBits>(n, lane, &row, &chunk, S::kHalves);
+                    raw[x][n] = __ldg(reinterpret_cast<const uint4*>(
+                        block + x * kKvBlock * S::kRow + kv_offset<S::kRow>(row, 16 * chunk)));
+                }
+            scale = reinterpret_cast<const __half*>(block + 2 * kKvBlock * S::kRow)[lane];
+        };
+        auto store = [&](int x, uint8_t* to) {
+#pragma unroll
+            for (int n = 0; n < S::kLoads; ++n) {
+                int row, chunk;
+                piece<kBits>(n, lane, &row, &chunk, S::kHalves);
+                expand<kBits>(raw[x][n], to, S::kHalfBytes, kKvBlock * w + row, chunk);
+            }
+        };
+        auto arrive = [&](uint32_t bar) {
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar);
+        };
+        const float log2_scale = a.scale * 1.4426950408889634f;
+        fetch(0);
+        for (int i = 0; i < tiles; ++i) {
+            const int b = i & 1;
+            if (i >= 2 && !__all_sync(0xffffffffu, wait(kempty + 8 * b, (i - 2) >> 1))) break;
+            store(0, kbuf + b * S::kOperandBytes);
+            arrive(kfull + 8 * b);
+            if (i >= 2 && !__all_sync(0xffffffffu, wait(vempty + 8 * b, (i - 2) >> 1))) break;
+            store(1, vbuf + b * S::kOperandBytes);
+            // K's scale (lanes 0-15) and V's (16-31) of token lane & 15
+            {
+                const int j = kKvBlock * w + (lane & 15);
+                const bool seen = there && (tile0 + i) * kTile + j < length;
+                const float s = __half2float(scale);
+                float* num = numbers + b * 3 * kTile + j;
+                if (lane < 16) {
+                    num[0] = seen ? s * log2_scale : 0.f;
+                } else {
+                    // a zero scale has all-zero values: any log will do
+                    const float lv = fmaxf(lg2(s), -24.f);
+                    num[kTile] = seen ? lv : -INFINITY;
+                    num[2 * kTile] = seen ? ex2(-lv) : 0.f;
+                }
+            }
+            if (i + 1 < tiles) fetch(i + 1);
+            arrive(vfull + 8 * b);
+        }
+    } else if (lane == 0) {
+        // ---------------- MMAs ----------------
+        constexpr uint32_t kIdescS = instruction(kTile, false), kIdescO = instruction(kDim, true);
+        int committed = 0;
+        bool ok = wait(pfull, 0);  // Q
+        for (int i = 0; i <= tiles && ok; ++i) {
+            if (i < tiles) {
+                const int b = i & 1;
+                ok = wait(kfull + 8 * b, i >> 1);
+                if (!ok) break;
+                fence_after();
+                const uint32_t kb = smem_u32(kbuf) + b * S::kOperandBytes;
+#pragma unroll
+                for (int k = 0; k < kDim / 16; ++k)
+                    mma(tmem + kColS + 128 * b, tmem + kColQ + 8 * k,
+                        operand(kb + (k >> 2) * S::kHalfBytes + (k & 3) * 32, 16), kIdescS, k > 0);
+                commit(sfull + 8 * b);
+                commit(kempty + 8 * b);
+            }
+            if (i > 0) {
+                const int b = (i - 1) & 1;
+                ok = wait(pfull, i) && wait(vfull + 8 * b, (i - 1) >> 1);
+                if (!ok) break;
+                fence_after();
+                const uint32_t vb = smem_u32(vbuf) + b * S::kOperandBytes;
+#pragma unroll
+                for (int k = 0; k < kTile / 16; ++k)
+                    mma(tmem + kColO, tmem + kColP + 8 * k, operand(vb + k * 2048, S::kHalfBytes),
+                        kIdescO, i > 1 || k > 0);
+                commit(vempty + 8 * b);
+                committed = i;
+            }
+        }
+        if (!ok && committed > 0) {
+            // the MMAs issued so far end before the memory they use is given up
+            mbar_wait_bounded(vempty + 8 * ((committed - 1) & 1), (uint32_t)(committed - 1) >> 1 & 1u,
+                              p.wait_cycles);
+        }
+    }
+
+    __syncthreads();
+    fence_after();
+    // ---------------- the output, through shared memory ----------------
+    if (finished) {
+        const uint32_t lane_base = tmem + ((uint32_t)(32 * warp) << 16);
+        const float inv = sum_l > 0.f ? 1.f / sum_l : sum_l;  // 0 cannot be; NaN stays
+        float* row = reinterpret_cast<float*>(smem + (32 * warp + lane) * S::kOutStride);
+#pragma unroll 1
+        for (int c = 0; c < kDim; c += 32) {
+            uint32_t o[32];
+            ld32(lane_base + kColO + c, o);
+            ld_wait(o);
+#pragma unroll
+            for (int j = 0; j < 32; j += 4) {
+                // int4: columns (0..7) hold elements 0 4 1 5 2 6 3 7
+                const int g8 = j & ~7, odd = (j >> 2) & 1;
+                float v[4];
+#pragma unroll
+                for (int x = 0; x < 4; ++x)
+                    v[x] = __uint_as_float(kBits == 8 ? o[j + x] : o[g8 + 2 * x + odd]) * inv;
+                *reinterpret_cast<float4*>(row + c + j) = make_float4(v[0], v[1], v[2], v[3]);
+            }
+        }
+        row[kDim] = (ref + lg2(sum_l)) * 0.6931471805599453f;
+    }
+    fence_before();
+    __syncthreads();
+    if (warp == 0) {
+        fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kColumns)
+                     : "memory");
+    }
+    if (*s_fail) return;
+    const int heads = a.kv_heads * a.group;
+    const int64_t all = (int64_t)(p.rows / a.group) * heads;  // rows of one part's result
+    const int valid = min(kRows, p.rows - row0);
+    for (int i = tid; i < valid * (kDim / 4); i += kThreads) {
+        const int rr = i / (kDim / 4), d = i % (kDim / 4) * 4;
+        const int i0 = p.group.div(row0 + rr);
+        const int64_t at = part * all + (int64_t)i0 * heads + (head - i0) * a.group + row0 + rr;
+        const float* row = reinterpret_cast<const float*>(smem + rr * S::kOutStride);
+        *reinterpret_cast<float4*>(a.out_f32 + at * kDim + d) = *reinterpret_cast<const float4*>(row + d);
+        if (d == 0) a.lse[at] = row[kDim];
+    }
+}
+
+template <int kDim, int kBits, bool kBf16>
+cudaError_t run(const PrefixParams& p, cudaStream_t stream) {
+    using S = PrefixShape<kDim, kBits>;
+    const auto kernel = kv_prefix_kernel<kDim, kBits, kBf16>;
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
+    if (e != cudaSuccess) return e;
+    return launch_pdl(kernel, dim3((unsigned)(p.a.kv_heads * p.row_tiles * p.parts)), dim3(kThreads),
+                      S::kSmem, stream, p);
+}
+
+// Parts of the tokens: the cut that needs the fewest tile times, with a CTA's
+// set-up and output at about kSetUp tiles and one CTA per SM.
+int cut(int items, int tiles) {
+    constexpr int kSetUp = 5, kSms = 148, kMostParts = 16;
+    int best = 1, cost = INT32_MAX;
+    for (int parts = 1; parts <= std::min(kMostParts, tiles); ++parts) {
+        const int per = (tiles + parts - 1) / parts, used = (tiles + per - 1) / per;
+        const int waves = (items * used + kSms - 1) / kSms;
+        if (waves * (per + kSetUp) < cost) cost = waves * (per + kSetUp), best = used;
+    }
+    return best;
+}
+
+}  // namespace
+
+bool kv_prefix_takes(const KvAttentionArgs& a) {
+    return a.head_dim <= 128 && (int64_t)a.new_tokens * a.group >= 32 &&
+           (int64_t)a.new_tokens * a.group < (1 << 24);
+}
+
+int kv_prefix_parts(const KvAttentionArgs& a) {
+    const int rows = a.new_tokens * a.group, row_tiles = (rows + kRows - 1) / kRows;
+    return cut(a.kv_heads * row_tiles, (a.fixed_length + kTile - 1) / kTile);
+}
+
+cudaError_t launch_kv_prefix(const KvAttentionArgs& a, cudaStream_t stream) {
+    PrefixParams p{};
+    p.a = a;
+    p.group = FastDiv((uint32_t)a.group);
+    p.page_blocks = FastDiv((uint32_t)(a.page_size / kKvBlock));
+    p.rows = a.new_tokens * a.group;
+    p.row_tiles = (p.rows + kRows - 1) / kRows;
+    p.tiles = (a.fixed_length + kTile - 1) / kTile;
+    p.parts = kv_prefix_parts(a);
+    p.part_tiles = (p.tiles + p.parts - 1) / p.parts;
+    p.q_vec = aligned16(a.q, a.q_new, a.q_head);
+    p.wait_cycles = wait_budget();
+    const bool bf16 = a.type == kTypeBf16;
+    if (a.head_dim == 64)
+        return a.bits == 8 ? (bf16 ? run<64, 8, true>(p, stream) : run<64, 8, false>(p, stream))
+                           : (bf16 ? run<64, 4, true>(p, stream) : run<64, 4, false>(p, stream));
+    return a.bits == 8 ? (bf16 ? run<128, 8, true>(p, stream) : run<128, 8, false>(p, stream))
+                       : (bf16 ? run<128, 4, true>(p, stream) : run<128, 4, false>(p, stream));
+}
+
+cudaError_t read_kv_prefix_status(int clear, int* status) {
+    return read_status_symbol(g_kv_prefix_status, clear, status);
+}
+
+}  // namespace clb

@@ -256,22 +256,22 @@ py::object kvattention(const at::Tensor& q, const at::Tensor& pages, const at::T
     desc.scale = static_cast<float>(default_scale ? 1.0 / std::sqrt(static_cast<double>(D)) : scale);
     c10::cuda::OptionalCUDAGuard guard;
     void* st = begin(d, &guard);
-    at::Tensor out = at::empty(q.sizes(), q.options()), lse, front;
+    at::Tensor out = at::empty(q.sizes(), q.options()), lse, scratch;
     const auto f32 = q.options().dtype(at::kFloat);
     if (return_lse) lse = at::empty(q.sizes().slice(0, last), f32);
-    float *po = nullptr, *pl = nullptr;
     if (shared) {
         desc.prefix_length = static_cast<int32_t>(prefix_length);
         desc.prefix_page_count = static_cast<int32_t>(prefix->size(0));
-        front = at::empty({B * new_tokens * H * (D + 1)}, f32);
-        po = front.data_ptr<float>();
-        pl = po + B * new_tokens * H * D;
+        size_t floats = 0;
+        if (cl_kvattention_prefix_floats(&desc, &floats) != CL_OK) return py::none();
+        scratch = at::empty({static_cast<int64_t>(floats)}, f32);
     }
     if (cl_kvattention(q.data_ptr(), static_cast<const uint8_t*>(pages.data_ptr()),
                        table.data_ptr<int32_t>(), lengths.data_ptr<int32_t>(),
                        shared ? prefix->data_ptr<int32_t>() : nullptr, out.data_ptr(),
-                       return_lse ? lse.data_ptr<float>() : nullptr, po, pl, workspace.data_ptr(),
-                       &desc, st) != CL_OK)
+                       return_lse ? lse.data_ptr<float>() : nullptr,
+                       shared ? scratch.data_ptr<float>() : nullptr, workspace.data_ptr(), &desc,
+                       st) != CL_OK)
         return py::none();
     if (return_lse) return py::cast(Pair(out, lse));
     return py::cast(out);

@@ -362,11 +362,12 @@ int cl_kvcache_read(const uint8_t* pages, const int64_t* slots, void* k, void* v
  * With prefix_pages (int32 [prefix_page_count]) and prefix_length > 0 the
  * tokens of those pages stand in front of every sequence's own (length counts
  * the own ones) and are read once for the whole batch: one launch over the
- * prefix, then one over the sequences that joins the two.  prefix_out (fp32
- * [batch, new_tokens, q_heads, head_dim], 16-byte aligned) and prefix_lse
- * (fp32 [batch, new_tokens, q_heads]) are scratch of the call.  The q rows
- * must then be evenly spaced (q_batch == new_tokens * q_new when both batch
- * and new_tokens exceed 1) and window must be 0.
+ * prefix (on the 5th-generation tensor cores where the batch has the rows for
+ * them), then one over the sequences that joins the two.  prefix_scratch:
+ * cl_kvattention_prefix_floats floats for the same descriptor, 16-byte
+ * aligned, used within the call.  The q rows must then be evenly spaced
+ * (q_batch == new_tokens * q_new when both batch and new_tokens exceed 1) and
+ * window must be 0.
  *
  * workspace: cl_kvattention_workspace bytes, 16-byte aligned, zero-filled
  * once before its first use and again only after a launch that failed; each
@@ -380,10 +381,11 @@ typedef struct cl_kvattention_desc {
     float scale;
 } cl_kvattention_desc;
 int cl_kvattention_workspace(size_t* bytes);
+int cl_kvattention_prefix_floats(const cl_kvattention_desc* desc, size_t* floats);
 int cl_kvattention(const void* q, const uint8_t* pages, const int32_t* page_table,
                    const int32_t* lengths, const int32_t* prefix_pages, void* out, float* lse,
-                   float* prefix_out, float* prefix_lse, void* workspace,
-                   const cl_kvattention_desc* desc, void* stream);
+                   float* prefix_scratch, void* workspace, const cl_kvattention_desc* desc,
+                   void* stream);
 
 #ifdef __cplusplus
 } /* extern "C" */

@@ -78,7 +78,7 @@ def test_attention_descriptor(lib):
     ok = nat.KvAttentionDesc(num_pages=4, batch=2, new_tokens=1, q_heads=8, kv_heads=2,
                              head_dim=128, bits=8, page_size=64, max_pages=2,
                              dtype=nat.CL_DTYPE_F16, scale=0.1)
-    args = [FAKE] * 10
+    args = [FAKE] * 9
 
     def call(a=args, **kw):
         return lib.cl_kvattention(*a, _with(ok, **kw), None)
@@ -95,11 +95,18 @@ def test_attention_descriptor(lib):
                      (dict(prefix_length=10, prefix_page_count=1, new_tokens=2, q_batch=3, q_new=1),
                       "evenly")):
         assert call(**kw) == BAD and text in nat.last_error(lib), (kw, nat.last_error(lib))
-    for i in (0, 1, 2, 3, 5, 9):
+    for i in (0, 1, 2, 3, 5, 8):
         assert call(args[:i] + [None] + args[i + 1:]) == BAD
-    for i in (1, 5, 9):
+    for i in (1, 5, 8):
         assert call(args[:i] + [FAKE + 2] + args[i + 1:]) == BAD and "aligned" in nat.last_error(lib)
-    assert call([FAKE, FAKE] + [None] * 8, batch=0) == nat.CL_OK
+    assert call([FAKE, FAKE] + [None] * 7, batch=0) == nat.CL_OK
+    n = ctypes.c_size_t(0)
+    assert lib.cl_kvattention_prefix_floats(_with(ok), ctypes.byref(n)) == nat.CL_OK and n.value == 0
+    assert lib.cl_kvattention_prefix_floats(_with(ok, prefix_length=10, prefix_page_count=1),
+                                            ctypes.byref(n)) == nat.CL_OK
+    assert n.value >= 2 * 8 * 129 and n.value % (2 * 8 * 129) == 0
+    assert call(prefix_length=10, prefix_page_count=1, a=args[:7] + [None] + args[8:]) == BAD
+    assert call(prefix_length=10, prefix_page_count=1, a=args[:7] + [FAKE + 4] + args[8:]) == BAD
 
 
 def _rej(fn, text):
