@@ -57,6 +57,11 @@ constexpr int kWarps = 4, kThreads = 32 * kWarps;
 constexpr int kMaxBatch = 4096;  // lengths and their running sum are kept in shared memory
 constexpr int kMaxGrid = 148 * 5;
 constexpr int kFan = 16;         // partial results added by one CTA at a time
+// What a CTA pays for a segment besides its units (loading q, joining its
+// warps' results, latencies), in units: about 4000 cycles against 400 to 700 a
+// unit.  Without it the CTA that gets the shortest sequences of a ragged batch
+// ends last (64 sequences of 1 to 1024 tokens: 91 us).
+constexpr int kSegmentCost = 8;
 constexpr float kSlack = 8.f;    // weights stay below 2^8, far inside fp16
 constexpr int kPartialFloats = 16 * 128 + 2 * 16;  // O, m and l of one partial result
 constexpr size_t kCounterBytes = (size_t)kMaxGrid * 3 * sizeof(int);
@@ -150,6 +155,13 @@ __device__ __forceinline__ int ceil_div(int n, float inv) {
     return __float2int_ru(((float)n - 0.5f) * inv);
 }
 
+// n / d for quotients below 2^21: an estimate, right to one, and its correction.
+__device__ __forceinline__ int quotient(int n, int d) {
+    int q = __float2int_rz(__fdividef((float)n, (float)d));
+    const int r = n - q * d;
+    return q - (r < 0) + (r >= d);
+}
+
 struct Params {
     KvAttentionArgs a;
     float* partial;
@@ -208,6 +220,7 @@ __global__ void __launch_bounds__(kThreads, Shape<kDim, kBits, kNB>::kPerSm)
     int* flag = reinterpret_cast<int*>(bars + kWarps * kStages);
     int* s_len = flag + 4;                 // [batch]
     int* s_cum = s_len + p.a.batch;        // [batch + 1] cells in front of a sequence
+    int* s_cost = s_cum + p.a.batch + 1;   // [batch + 1] the same with kSegmentCost a segment
 
     const KvAttentionArgs& a = p.a;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -261,13 +274,15 @@ __global__ void __launch_bounds__(kThreads, Shape<kDim, kBits, kNB>::kPerSm)
             units = __reduce_add_sync(0xffffffffu, units) * heads_tiles;
             segments = __reduce_add_sync(0xffffffffu, segments) * heads_tiles;
             // equal ranges of the line (the estimate may be short on very long ones)
-            share = max(p.min_units, ceil_div(units, p.inv_grid));
-            if (share * (int64_t)grid < units) share += 1 + (share >> 20);
+            const int cost = units + kSegmentCost * segments;
+            share = max(p.min_units, ceil_div(cost, p.inv_grid));
+            if (share * (int64_t)grid < cost) share += 1 + (share >> 20);
             if (2 * segments <= grid && p.may_chunk) {
                 // Few segments: each is cut into chunks of its own, one per CTA,
                 // so that a CTA works on one segment.  Eight sizes between the
                 // equal range and the one that must fit, four lanes on each; the
                 // smallest with which the grid holds all chunks is taken.
+                share = max(p.min_units, ceil_div(units, p.inv_grid));
                 const int more = max(0, ceil_div(units, __fdividef(1.f, (float)(grid - segments))) + 1 - share);
                 const int mine = share + (more * (lane >> 2) * 37 >> 8);  // 37/256 > 1/7
                 const float inv = __fdividef(1.f, (float)mine);
@@ -280,21 +295,31 @@ __global__ void __launch_bounds__(kThreads, Shape<kDim, kBits, kNB>::kPerSm)
                 share = 1;
             }
             const float inv = __fdividef(1.f, (float)cell);
-            int before = 0;
+            int before = 0, filled = 0;
             for (int b0 = 0; b0 < a.batch; b0 += 32) {
                 const int b = b0 + lane;
                 int n = b < a.batch ? units_of(s_len[b]) : 0;
                 if (cell > 1) n = ceil_div(n, inv);
+                const uint32_t some = __ballot_sync(0xffffffffu, n > 0);
                 int scan = n;
 #pragma unroll
                 for (int o = 1; o < 32; o <<= 1) {
                     const int v = __shfl_up_sync(0xffffffffu, scan, o);
                     if (lane >= o) scan += v;
                 }
-                if (b < a.batch) s_cum[b] = before + scan - n;
+                if (b < a.batch) {
+                    s_cum[b] = before + scan - n;
+                    s_cost[b] = before + scan - n +
+                                kSegmentCost * (filled + __popc(some & ((1u << lane) - 1)));
+                }
                 before += __shfl_sync(0xffffffffu, scan, 31);
+                filled += __popc(some);
             }
-            if (lane == 0) s_cum[a.batch] = before, flag[1] = cell, flag[2] = share;
+            if (lane == 0) {
+                s_cum[a.batch] = before;
+                s_cost[a.batch] = before + kSegmentCost * filled;
+                flag[1] = cell, flag[2] = share;
+            }
         }
         if (few) {
             __syncwarp();
@@ -365,7 +390,7 @@ __global__ void __launch_bounds__(kThreads, Shape<kDim, kBits, kNB>::kPerSm)
     if (p.every_chunk) {
         const int segment = p.seg_chunks.div((int)blockIdx.x);
         c0 = segment * (int)p.seg_chunks.d;
-        start.seq = (int)((unsigned)segment / (unsigned)heads_tiles);
+        start.seq = quotient(segment, heads_tiles);
         start.part = segment - start.seq * heads_tiles;
         len0 = length_of(start.seq);
         start.begin = 0;
@@ -379,21 +404,44 @@ __global__ void __launch_bounds__(kThreads, Shape<kDim, kBits, kNB>::kPerSm)
             return;
         }
     } else {
-        for (int b = blockIdx.x; b < a.batch; b += grid)
-            if (s_cum[b + 1] == s_cum[b]) write_empty(b, 0, a.kv_heads);
-        const int total = s_cum[a.batch] * heads_tiles;
-        const int x0 = (int)min((int64_t)total, (int64_t)blockIdx.x * share);
-        u0 = x0;
-        u1 = min(total, x0 + share);
-        if (u0 >= u1) return;
-        int lo = 0, hi = a.batch;  // last sequence whose cells begin at or before x0
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (s_cum[mid] * heads_tiles <= x0) lo = mid; else hi = mid;
+        for (int i = blockIdx.x; i < a.batch * a.kv_heads; i += grid) {
+            const int b = i / a.kv_heads, h = i - b * a.kv_heads;
+            if (s_cum[b + 1] == s_cum[b]) write_empty(b, h, h + 1);
         }
-        const int cells = s_cum[lo + 1] - s_cum[lo], in = x0 - s_cum[lo] * heads_tiles;
+        // last sequence whose cells (`sums`) begin at or before x, by the whole warp
+        auto find = [&](const int* sums, int x) {
+            int count = 0;
+            for (int b0 = 0; b0 < a.batch; b0 += 32) {
+                const int b = b0 + lane;
+                const uint32_t at_or_before =
+                    __ballot_sync(0xffffffffu, b < a.batch && sums[min(b, a.batch)] * heads_tiles <= x);
+                count += __popc(at_or_before);
+                if (at_or_before != 0xffffffffu) break;
+            }
+            return count - 1;
+        };
+        // Equal ranges are cut in cost; the unit at which a cost begins:
+        const int total_cost = s_cost[a.batch] * heads_tiles;
+        auto unit_at = [&](int cost) {
+            if (cost >= total_cost) return s_cum[a.batch] * heads_tiles;
+            const int b = find(s_cost, cost);
+            const int n = s_cum[b + 1] - s_cum[b], in = cost - s_cost[b] * heads_tiles;
+            const int part = quotient(in, n + kSegmentCost);
+            return s_cum[b] * heads_tiles + part * n + min(n, in - part * (n + kSegmentCost));
+        };
+        const int64_t x0 = (int64_t)blockIdx.x * share;
+        if (chunked) {
+            u0 = (int)min(x0, (int64_t)s_cum[a.batch] * heads_tiles);
+            u1 = min(u0 + 1, s_cum[a.batch] * heads_tiles);
+        } else {
+            u0 = unit_at((int)min(x0, (int64_t)total_cost));
+            u1 = unit_at((int)min(x0 + share, (int64_t)total_cost));
+        }
+        if (u0 >= u1) return;
+        const int lo = find(s_cum, u0);
+        const int cells = s_cum[lo + 1] - s_cum[lo], in = u0 - s_cum[lo] * heads_tiles;
         start.seq = lo;
-        start.part = (int)((unsigned)in / (unsigned)cells);
+        start.part = quotient(in, cells);
         start.units = cells;
         start.begin = s_cum[lo] * heads_tiles + start.part * cells;
         len0 = s_len[lo];
@@ -456,14 +504,11 @@ __global__ void __launch_bounds__(kThreads, Shape<kDim, kBits, kNB>::kPerSm)
         if (u >= u1) return;
         int part = start.part, in = u;
         if (!chunked) {
-            int hi = a.batch;
-            while (hi - seq > 1) {
-                const int mid = (seq + hi) >> 1;
-                if (s_cum[mid] * heads_tiles <= u) seq = mid; else hi = mid;
-            }
-            const int units = s_cum[seq + 1] - s_cum[seq];
+            int next = s_cum[seq + 1];
+            while (next * heads_tiles <= u) next = s_cum[++seq + 1];
+            const int units = next - s_cum[seq];
             in = u - s_cum[seq] * heads_tiles;
-            part = in / units;
+            part = quotient(in, units);
             in -= part * units;
         }
         const int len = chunked ? len0 : s_len[seq];
@@ -859,8 +904,9 @@ __global__ void __launch_bounds__(kThreads, Shape<kDim, kBits, kNB>::kPerSm)
 
         if (!whole) {
             if (!chunked) {
-                c0 = now.begin / share;
-                parts = (now.begin + now.units - 1) / share - c0 + 1;
+                const int cost = s_cost[now.seq] * heads_tiles + now.part * (now.units + kSegmentCost);
+                c0 = quotient(cost, share);
+                parts = quotient(cost + now.units - 1, share) - c0 + 1;
             }
             const int me = (int)blockIdx.x - c0;
             auto slot_of = [&](int i) {  // of the segment's i-th CTA
@@ -976,8 +1022,8 @@ cudaError_t run(Params& p, cudaStream_t stream) {
     const KvAttentionArgs& a = p.a;
     const size_t fixed = S::kRingBytes + S::kRedBytes + S::kStatBytes +
                          kWarps * S::kStages * 8 + 16;
-    const size_t smem = fixed + (2 * (size_t)a.batch + 1) * sizeof(int);
-    const size_t smem_max = fixed + (2 * (size_t)kMaxBatch + 1) * sizeof(int);
+    const size_t smem = fixed + (3 * (size_t)a.batch + 2) * sizeof(int);
+    const size_t smem_max = fixed + (3 * (size_t)kMaxBatch + 2) * sizeof(int);
     static std::atomic<int> resident[64];  // CTAs the device holds at once, 0: not asked yet
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
@@ -1007,8 +1053,8 @@ cudaError_t run(Params& p, cudaStream_t stream) {
     p.every_chunk = grid == segments * per;
     p.seg_chunks = FastDiv((uint32_t)per);
     p.min_chunk = FastDiv((uint32_t)p.min_units);
-    // blocks of all segments below 2^22: every count that the plan divides is
-    p.may_chunk = line < (int64_t)1 << 22;
+    // blocks of all segments below 2^21: every count that the plan divides is
+    p.may_chunk = line < (int64_t)1 << 21;
     p.inv_grid = 1.f / (float)grid;
     return launch_pdl(kernel, dim3((unsigned)grid), dim3(kThreads), smem, stream, p);
 }
@@ -1031,7 +1077,9 @@ size_t kv_attention_workspace() {
 bool kv_attention_fits(const KvAttentionArgs& a) {
     const int64_t rows = (int64_t)a.new_tokens * a.group;
     const int64_t per = a.page_size / kKvBlock;
-    return longest_line(a, (rows + 7) / 8) < ((int64_t)1 << 31) - ((int64_t)1 << 21) &&
+    return longest_line(a, (rows + 7) / 8) +
+                   (int64_t)kSegmentCost * a.batch * a.kv_heads * ((rows + 7) / 8) <
+               ((int64_t)1 << 31) - ((int64_t)1 << 21) &&
            a.num_pages * a.kv_heads * per < ((int64_t)1 << 32) - 2;  // blocks are numbered
 }
 

@@ -10,18 +10,18 @@
 // 128 at a time:
 //   * 8 warps expand the tile's 8 cache blocks, one block a warp, to exact fp16
 //     whole values in shared memory (rows of tokens, 64 elements wide, 128-byte
-//     swizzle), read one tile ahead into registers; the scales become three
+//     swizzle), read a tile ahead into registers; the scales become two
 //     numbers per token in fp32;
 //   * one thread issues the MMAs (M = N = 128, K = 16, fp32 accumulators): S =
 //     Q K^T with Q in Tensor Memory and K as stored (K-major), O += P V with P in
 //     Tensor Memory and the same layout of V read across (MN-major);
-//   * 4 warps, a row a thread, do the softmax as in kv_attention.cu: weights
-//     w_j = 2^(s_j + log2 vs_j - m) in fp16, the sum of w_j / vs_j in fp32, one
-//     lazy reference m per row, packed fp32 pairs; O is only rescaled when a
-//     score exceeds the reference by more than kSlack.
+//   * 8 warps, half a row's tokens a thread, do the softmax as in
+//     kv_attention.cu: p_j = 2^(s_j - m) summed in fp32, weights p_j vs_j in
+//     fp16, one lazy reference m per row near the maximum of s_j + log2 vs_j,
+//     packed fp32 pairs; O is only rescaled when a weight exceeds kMostWeight,
+//     which the two warps of a row find out with one barrier a tile.
 // S is double-buffered: the tensor cores compute tile i + 1's S and tile i -
-// 1's O while the softmax of tile i runs.  Tokens past the prefix get a weight
-// of zero from their three numbers, so no tile is special.
+// 1's O while the softmax of tile i runs.
 //
 // Tensor Memory (512 columns): S 2 x 128, O head_dim, P 64, Q head_dim / 2.
 // int4: a byte's nibbles leave their word as pairs (0, 4) (1, 5) (2, 6) (3, 7),
@@ -49,10 +49,10 @@ namespace {
 __device__ int g_kv_prefix_status;
 
 constexpr int kRows = 128, kTile = 128;  // query rows and tokens of a tile
-constexpr int kSoftWarps = 4, kFillWarps = 8;
+constexpr int kSoftWarps = 8, kFillWarps = 8;
 constexpr int kMmaWarp = kSoftWarps + kFillWarps;
 constexpr int kThreads = 32 * (kMmaWarp + 1);
-constexpr float kSlack = 8.f;
+constexpr float kMostWeight = 256.f;  // far inside fp16
 constexpr uint32_t kColS = 0, kColO = 256, kColP = 384, kColQ = 448, kColumns = 512;
 
 __device__ __forceinline__ float ex2(float x) {
@@ -111,6 +111,15 @@ __device__ __forceinline__ uint64_t operand(uint32_t addr, uint32_t wide) {
            ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
 }
 
+// 16 bytes of the cache, asked for here and not where they are used (a plain
+// load may be moved down to its use, which costs the whole latency).
+__device__ __forceinline__ uint4 load_now(const uint8_t* p) {
+    uint4 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+
 // 32 columns of this thread's lane: issue, and the wait that makes them valid.
 __device__ __forceinline__ void ld32(uint32_t addr, uint32_t (&r)[32]) {
     asm volatile(
@@ -136,6 +145,24 @@ __device__ __forceinline__ void ld_wait(uint32_t (&r)[32]) {
                  :
                  : "memory");
 }
+__device__ __forceinline__ void ld16(uint32_t addr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, "
+        "%12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+          "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+          "=r"(r[14]), "=r"(r[15])
+        : "r"(addr)
+        : "memory");
+}
+__device__ __forceinline__ void ld_wait(uint32_t (&r)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]),
+                   "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]),
+                   "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+                 :
+                 : "memory");
+}
 __device__ __forceinline__ void st32(uint32_t addr, const uint32_t (&r)[32]) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, "
@@ -156,6 +183,18 @@ __device__ __forceinline__ void st16(uint32_t addr, const uint32_t (&r)[16]) {
         "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]),
         "r"(r[15])
         : "memory");
+}
+
+// Barrier of the 64 threads that share 32 rows, and whether any of them says so.
+__device__ __forceinline__ bool any_of_rows(int id, bool say) {
+    uint32_t r;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.u32 p, %1, 0;\n\t"
+        "barrier.cta.red.or.pred q, %2, 64, p;\n\t"
+        "selp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(r) : "r"((uint32_t)say), "r"(id) : "memory");
+    return r != 0;
 }
 
 struct PrefixParams {
@@ -180,7 +219,8 @@ struct PrefixShape {
     // numbers, barriers; at least 120 KB, so that one CTA has an SM and its
     // Tensor Memory.
     static constexpr int kNumbers = 4 * kOperandBytes;
-    static constexpr int kBars = kNumbers + 2 * 3 * kTile * 4;
+    static constexpr int kTops = kNumbers + 4 * 2 * kTile * 4;  // [2][kRows] exchanged by row halves
+    static constexpr int kBars = kTops + 2 * kRows * 4;
     static constexpr int kSmem = (kBars + 128 < 120 * 1024 ? 120 * 1024 : kBars + 128) + 1024;
     static_assert(kRows * kOutStride <= 4 * kOperandBytes, "room for the output");
 };
@@ -236,12 +276,13 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prefix_kernel(const PrefixPara
         (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
     uint8_t* kbuf = smem;                          // [2] K operands
     uint8_t* vbuf = smem + 2 * S::kOperandBytes;   // [2] V operands
-    float* numbers = reinterpret_cast<float*>(smem + S::kNumbers);  // [2][3][kTile]
+    float* numbers = reinterpret_cast<float*>(smem + S::kNumbers);  // [4][2][kTile]
+    float* tops = reinterpret_cast<float*>(smem + S::kTops);
     const uint32_t bars = smem_u32(smem + S::kBars);
     const uint32_t kfull = bars, vfull = bars + 16, kempty = bars + 32, vempty = bars + 48,
-                   sfull = bars + 64, pfull = bars + 80;
-    volatile uint32_t* s_tmem = reinterpret_cast<volatile uint32_t*>(smem + S::kBars + 96);
-    volatile int* s_fail = reinterpret_cast<volatile int*>(smem + S::kBars + 100);
+                   sfull = bars + 64, pfull = bars + 80, nfull = bars + 88;
+    volatile uint32_t* s_tmem = reinterpret_cast<volatile uint32_t*>(smem + S::kBars + 120);
+    volatile int* s_fail = reinterpret_cast<volatile int*>(smem + S::kBars + 124);
 
     const KvAttentionArgs& a = p.a;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -260,6 +301,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prefix_kernel(const PrefixPara
             mbar_init(vempty + 8 * i, 1);
             mbar_init(sfull + 8 * i, 1);
         }
+        for (int i = 0; i < 4; ++i) mbar_init(nfull + 8 * i, kFillWarps);
         mbar_init(pfull, kSoftWarps);
         *s_fail = 0;
         fence_barrier_init();
@@ -288,13 +330,14 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prefix_kernel(const PrefixPara
         return ok;
     };
 
-    float sum_l = 0.f, ref = 0.f;  // of this thread's row
-    bool finished = false;         // softmax warps: all tiles done
+    float sum_l = 0.f, ref = -INFINITY;  // of this thread's row (and half of the tokens)
+    bool finished = false;               // softmax warps: all tiles done
+    const int quarter = warp & 3, half = warp >> 2 & 1;  // of the softmax warps
+    const uint32_t lane_base = tmem + ((uint32_t)(32 * quarter) << 16);
 
     if (warp < kSoftWarps) {
-        // ---------------- softmax: one row a thread ----------------
-        const uint32_t lane_base = tmem + ((uint32_t)(32 * warp) << 16);
-        const int r = row0 + 32 * warp + lane;
+        // ---------------- softmax: half a row's tokens a thread ----------------
+        const int in_tile = 32 * quarter + lane, r = row0 + in_tile;
         float unit = 1.f;  // what the row was divided by (a power of two)
         {
             const int i0 = p.group.div(r);
@@ -308,7 +351,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prefix_kernel(const PrefixPara
             float down = 1.f;
             if (kBf16) {
                 float top = 0.f;
-#pragma unroll 1
+#pragma unroll 4
                 for (int d = 0; d < kDim; d += 8) {
                     float x[8];
                     unpack8<kBf16>(load(d), x);
@@ -322,7 +365,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prefix_kernel(const PrefixPara
                 }
             }
 #pragma unroll 1
-            for (int d = 0; d < kDim; d += 32) {
+            for (int d = half * (kDim / 2); d < (half + 1) * (kDim / 2); d += 32) {
                 uint32_t packed[16];
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
@@ -349,103 +392,129 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prefix_kernel(const PrefixPara
         bool ok = true;
         for (int i = 0; i < tiles && ok; ++i) {
             const int b = i & 1;
-            ok = wait(sfull + 8 * b, i >> 1) && wait(vfull + 8 * b, i >> 1);
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) break;
+            bool good = __all_sync(0xffffffffu, wait(nfull + 8 * (i & 3), i >> 2) &&
+                                                    wait(sfull + 8 * b, i >> 1));
             fence_after();
-            const uint32_t s_at = lane_base + kColS + 128 * b;
-            const float* num = numbers + b * 3 * kTile;
-            // z of 4 columns, less the reference
-            auto logits = [&](const uint32_t* s, int col, float nref, unsigned long long& z0,
-                              unsigned long long& z1) {
+            const uint32_t s_at = lane_base + kColS + 128 * b + 64 * half;
+            const float* num = numbers + (i & 3) * 2 * kTile + 64 * half;
+            // columns of this half that hold tokens
+            const int live = length - (tile0 + i) * kTile - 64 * half;
+            // 16 columns of S have come; columns past the end at -inf
+            auto take_s = [&](int c, uint32_t (&s)[16]) {
+                ld_wait(s);
+                if (live < 16 * c + 16) {
+#pragma unroll
+                    for (int j = 0; j < 16; ++j)
+                        if (16 * c + j >= live) s[j] = 0xff800000u;
+                }
+            };
+            // base-2 logits of 4 columns, less the reference
+            auto logits = [&](const uint32_t* s, int col, unsigned long long nref,
+                              unsigned long long& z0, unsigned long long& z1) {
                 const ulonglong2 ks = *reinterpret_cast<const ulonglong2*>(num + col);
-                const ulonglong2 lv = *reinterpret_cast<const ulonglong2*>(num + kTile + col);
                 unsigned long long x0 = f2_pack(__uint_as_float(s[0]), __uint_as_float(s[1]));
                 unsigned long long x1 = f2_pack(__uint_as_float(s[2]), __uint_as_float(s[3]));
-                if (scaled) x0 = f2_mul(x0, unit2), x1 = f2_mul(x1, unit2);
-                const unsigned long long n2 = f2_pack(nref, nref);
-                z0 = f2_fma(x0, ks.x, f2_add(lv.x, n2));
-                z1 = f2_fma(x1, ks.y, f2_add(lv.y, n2));
+                if (kBf16 && scaled) x0 = f2_mul(x0, unit2), x1 = f2_mul(x1, unit2);
+                z0 = f2_fma(x0, ks.x, nref);
+                z1 = f2_fma(x1, ks.y, nref);
             };
-            // The reference from the tile's own scores: at the start, and when
-            // a score has outgrown it.
-            auto new_reference = [&]() {
-                float top = -INFINITY;
-#pragma unroll 1
-                for (int c = 0; c < 4; ++c) {
-                    uint32_t s[32];
-                    ld32(s_at + 32 * c, s);
-                    ld_wait(s);
-#pragma unroll
-                    for (int j = 0; j < 32; j += 4) {
-                        unsigned long long z0, z1;
-                        float x, y, z, w;
-                        logits(s + j, 32 * c + j, 0.f, z0, z1);
-                        f2_unpack(z0, x, y);
-                        f2_unpack(z1, z, w);
-                        top = fmaxf(fmaxf(fmaxf(top, x), y), fmaxf(z, w));
-                    }
-                }
-                return top;
-            };
-            bool waited = false;  // for the MMAs of tile i - 1, which read P and write O
+            bool waited = i == 0;  // for the MMAs of tile i - 1, which read P and write O
             auto previous_done = [&]() {
-                if (!waited && i > 0) {
-                    ok = wait(vempty + 8 * ((i - 1) & 1), (i - 1) >> 1);
-                    ok = __all_sync(0xffffffffu, ok);
+                if (!waited) {
+                    good = __all_sync(0xffffffffu, wait(vempty + 8 * ((i - 1) & 1), (i - 1) >> 1));
                     fence_after();
                 }
                 waited = true;
-                return ok;
+                return good;
             };
-            if (i == 0) {
-                const float top = new_reference();
-                ref = top == -INFINITY ? 0.f : top;  // only a NaN row has no largest score
-            }
-            for (;;) {
+            // Until the weights fit the reference: usually once.  The first tile
+            // has none yet.  What the two warps of a row do next is decided by
+            // their barrier alone, so neither can wait for the other in vain.
+            bool fresh = i == 0;
+            for (int tries = 0;; ++tries, fresh = false) {
                 unsigned long long try_l = l2;
-                float most = -INFINITY;
-                uint32_t s[2][32];
-                ld32(s_at, s[0]);
+                __half2 most = __half2half2(__half(0.f));
+                if (good && !fresh) {
+                    const unsigned long long nref = f2_pack(-ref, -ref);
+                    uint32_t s[2][16], packed[16];
+                    ld16(s_at, s[0]);
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    uint32_t(&cur)[32] = s[c & 1];
-                    ld_wait(cur);
-                    if (c < 3) ld32(s_at + 32 * (c + 1), s[(c + 1) & 1]);
-                    uint32_t packed[16];
+                    for (int c = 0; c < 4; ++c) {
+                        take_s(c, s[c & 1]);
+                        if (c < 3) ld16(s_at + 16 * (c + 1), s[(c + 1) & 1]);  // under the arithmetic
 #pragma unroll
-                    for (int j = 0; j < 32; j += 4) {
-                        unsigned long long z0, z1;
-                        float x, y, z, w;
-                        logits(cur + j, 32 * c + j, -ref, z0, z1);
-                        f2_unpack(z0, x, y);
-                        f2_unpack(z1, z, w);
-                        most = fmaxf(fmaxf(fmaxf(most, x), y), fmaxf(z, w));
-                        x = ex2(x), y = ex2(y), z = ex2(z), w = ex2(w);
-                        const ulonglong2 iv = *reinterpret_cast<const ulonglong2*>(
-                            num + 2 * kTile + 32 * c + j);
-                        try_l = f2_fma(f2_pack(x, y), iv.x, try_l);
-                        try_l = f2_fma(f2_pack(z, w), iv.y, try_l);
-                        packed[j / 2] = pack2<false>(x, y);
-                        packed[j / 2 + 1] = pack2<false>(z, w);
+                        for (int j = 0; j < 16; j += 4) {
+                            unsigned long long z0, z1;
+                            float x, y, z, w;
+                            logits(s[c & 1] + j, 16 * c + j, nref, z0, z1);
+                            f2_unpack(z0, x, y);
+                            f2_unpack(z1, z, w);
+                            z0 = f2_pack(ex2(x), ex2(y));
+                            z1 = f2_pack(ex2(z), ex2(w));
+                            try_l = f2_add(try_l, f2_add(z0, z1));
+                            const ulonglong2 vs = *reinterpret_cast<const ulonglong2*>(
+                                num + kTile + 16 * c + j);
+                            f2_unpack(f2_mul(z0, vs.x), x, y);
+                            f2_unpack(f2_mul(z1, vs.y), z, w);
+                            uint32_t* to = packed + 8 * (c & 1) + j / 2;
+                            to[0] = pack2<false>(x, y);
+                            to[1] = pack2<false>(z, w);
+                            most = __hmax2(most, __hmax2(u32_as_h2(to[0]), u32_as_h2(to[1])));
+                        }
+                        if (c & 1) {
+                            if (c == 1 && !previous_done()) break;
+                            st16(lane_base + kColP + 32 * half + 8 * (c - 1), packed);
+                        }
                     }
-                    if (c == 0 && !previous_done()) break;
-                    st16(lane_base + kColP + 16 * c, packed);
                 }
-                if (!ok) break;
-                if (!__any_sync(0xffffffffu, most > kSlack)) {
+                const float2 m2 = __half22float2(most);
+                // (a second reference always fits; the bound is for the loop's sake)
+                const bool over = fresh || (tries < 3 && fmaxf(m2.x, m2.y) > kMostWeight);
+                if (!any_of_rows(1 + quarter, over || !good)) {
                     l2 = try_l;
                     break;
                 }
-                // rescale what there is and take the tile again
+                if (any_of_rows(1 + quarter, !good)) {
+                    ok = false;
+                    break;
+                }
+                // The reference from the tile's own scores, under which what there
+                // is of O is rescaled; then the tile again.
+                float top = -INFINITY;
+#pragma unroll 1
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t s[16];
+                    ld16(s_at + 16 * c, s);
+                    take_s(c, s);
+#pragma unroll
+                    for (int j = 0; j < 16; j += 4) {
+                        unsigned long long z0, z1;
+                        float x, y, z, w;
+                        logits(s + j, 16 * c + j, f2_pack(0.f, 0.f), z0, z1);
+                        f2_unpack(z0, x, y);
+                        f2_unpack(z1, z, w);
+                        // a zero scale has all-zero values: any log will do
+                        const float4 vs = *reinterpret_cast<const float4*>(num + kTile + 16 * c + j);
+                        x += fmaxf(lg2(vs.x), -24.f), y += fmaxf(lg2(vs.y), -24.f);
+                        z += fmaxf(lg2(vs.z), -24.f), w += fmaxf(lg2(vs.w), -24.f);
+                        top = fmaxf(fmaxf(fmaxf(top, x), y), fmaxf(z, w));
+                    }
+                }
+                tops[half * kRows + in_tile] = top;
                 wait_st();
-                const float top = fmaxf(ref, new_reference());
+                if (any_of_rows(1 + quarter, !previous_done())) {
+                    ok = false;
+                    break;
+                }
+                top = fmaxf(top, tops[(half ^ 1) * kRows + in_tile]);
+                top = fmaxf(top, ref);
+                if (top == -INFINITY) top = 0.f;  // a row of NaN has no largest score
                 const float f = ex2(ref - top);
                 ref = top;
                 l2 = f2_mul(l2, f2_pack(f, f));
                 if (i > 0) {
 #pragma unroll 1
-                    for (int c = 0; c < kDim; c += 32) {
+                    for (int c = half * (kDim / 2); c < (half + 1) * (kDim / 2); c += 32) {
                         uint32_t o[32];
                         ld32(lane_base + kColO + c, o);
                         ld_wait(o);
@@ -468,6 +537,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prefix_kernel(const PrefixPara
             float x, y;
             f2_unpack(l2, x, y);
             sum_l = x + y;
+            tops[half * kRows + in_tile] = sum_l;
         }
         // nothing of this thread is in flight when the memory is freed
         asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
@@ -476,44 +546,44 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prefix_kernel(const PrefixPara
         // ---------------- expansion: one cache block a warp ----------------
         const int w = warp - kSoftWarps;
         uint32_t where = 0xffffffffu;  // lane i: the block of the 32-tile batch's i-th tile
-        uint4 raw[2][S::kLoads];
+        uint4 raw[2][S::kLoads];       // a block's K and V on their way
         __half scale = __half(0.f);
-        bool there = false;
-        auto fetch = [&](int i) {  // tile i's block into registers
+        uint32_t at = 0xffffffffu;
+        auto find = [&](int i) {  // tile i's block
+            if (i >= tiles) return;
             if ((i & 31) == 0) {
                 const int blk = (tile0 + i + lane) * 8 + w;
                 where = 0xffffffffu;
                 if (i + lane < tiles && blk * kKvBlock < length) {
                     const int index = p.page_blocks.div(blk);
-                    const int page = __ldg(a.table + index);
-                    if (page >= 0 && page < a.num_pages)
-                        where = ((uint32_t)page * a.kv_heads + head) * p.page_blocks.d +
-                                (blk - index * p.page_blocks.d);
-                    else
+                    int page = __ldg(a.table + index);
+                    if (page < 0 || page >= a.num_pages) {  // recorded; page 0 is read
                         atomicCAS(&g_kv_prefix_status, 0, kStatusKvIndex);
+                        page = 0;
+                    }
+                    where = ((uint32_t)page * a.kv_heads + head) * p.page_blocks.d +
+                            (blk - index * p.page_blocks.d);
                 }
             }
-            const uint32_t at = __shfl_sync(0xffffffffu, where, i & 31);
-            there = at != 0xffffffffu;
-            if (!there) {
+            at = __shfl_sync(0xffffffffu, where, i & 31);
+        };
+        auto fetch = [&](int x, int i) {  // its K (0, with the scales) or V (1)
+            if (i >= tiles) return;
+            if (at == 0xffffffffu) {
 #pragma unroll
-                for (int x = 0; x < 2; ++x)
-#pragma unroll
-                    for (int n = 0; n < S::kLoads; ++n) raw[x][n] = make_uint4(0, 0, 0, 0);
-                scale = __half(0.f);
+                for (int n = 0; n < S::kLoads; ++n) raw[x][n] = make_uint4(0, 0, 0, 0);
+                if (x == 0) scale = __half(0.f);
                 return;
             }
             const uint8_t* block = a.pages + (int64_t)at * S::kBlockBytes;
 #pragma unroll
-            for (int x = 0; x < 2; ++x)
-#pragma unroll
-                for (int n = 0; n < S::kLoads; ++n) {
-                    int row, chunk;
-                    piece<kBits>(n, lane, &row, &chunk, S::kHalves);
-                    raw[x][n] = __ldg(reinterpret_cast<const uint4*>(
-                        block + x * kKvBlock * S::kRow + kv_offset<S::kRow>(row, 16 * chunk)));
-                }
-            scale = reinterpret_cast<const __half*>(block + 2 * kKvBlock * S::kRow)[lane];
+            for (int n = 0; n < S::kLoads; ++n) {
+                int row, chunk;
+                piece<kBits>(n, lane, &row, &chunk, S::kHalves);
+                raw[x][n] = load_now(block + x * kKvBlock * S::kRow +
+                                     kv_offset<S::kRow>(row, 16 * chunk));
+            }
+            if (x == 0) scale = reinterpret_cast<const __half*>(block + 2 * kKvBlock * S::kRow)[lane];
         };
         auto store = [&](int x, uint8_t* to) {
 #pragma unroll
@@ -529,31 +599,28 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prefix_kernel(const PrefixPara
             if (lane == 0) mbar_arrive(bar);
         };
         const float log2_scale = a.scale * 1.4426950408889634f;
-        fetch(0);
+        find(0);
+        fetch(0, 0);
+        fetch(1, 0);
         for (int i = 0; i < tiles; ++i) {
             const int b = i & 1;
             if (i >= 2 && !__all_sync(0xffffffffu, wait(kempty + 8 * b, (i - 2) >> 1))) break;
+            // K's scale (lanes 0-15) and V's (16-31) of token lane & 15, 0 past
+            // the end; that S(i - 2) is done says that softmax i - 4 is
+            const bool seen = at != 0xffffffffu &&
+                              (tile0 + i) * kTile + kKvBlock * w + (lane & 15) < length;
+            const float s = seen ? __half2float(scale) : 0.f;
+            numbers[(i & 3) * 2 * kTile + (lane >> 4) * kTile + kKvBlock * w + (lane & 15)] =
+                lane < 16 ? (seen ? s * log2_scale : 1.f) : s;
             store(0, kbuf + b * S::kOperandBytes);
             arrive(kfull + 8 * b);
+            if (lane == 0) mbar_arrive(nfull + 8 * (i & 3));
+            find(i + 1);
+            fetch(0, i + 1);
             if (i >= 2 && !__all_sync(0xffffffffu, wait(vempty + 8 * b, (i - 2) >> 1))) break;
             store(1, vbuf + b * S::kOperandBytes);
-            // K's scale (lanes 0-15) and V's (16-31) of token lane & 15
-            {
-                const int j = kKvBlock * w + (lane & 15);
-                const bool seen = there && (tile0 + i) * kTile + j < length;
-                const float s = __half2float(scale);
-                float* num = numbers + b * 3 * kTile + j;
-                if (lane < 16) {
-                    num[0] = seen ? s * log2_scale : 0.f;
-                } else {
-                    // a zero scale has all-zero values: any log will do
-                    const float lv = fmaxf(lg2(s), -24.f);
-                    num[kTile] = seen ? lv : -INFINITY;
-                    num[2 * kTile] = seen ? ex2(-lv) : 0.f;
-                }
-            }
-            if (i + 1 < tiles) fetch(i + 1);
             arrive(vfull + 8 * b);
+            fetch(1, i + 1);
         }
     } else if (lane == 0) {
         // ---------------- MMAs ----------------
@@ -599,11 +666,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prefix_kernel(const PrefixPara
     fence_after();
     // ---------------- the output, through shared memory ----------------
     if (finished) {
-        const uint32_t lane_base = tmem + ((uint32_t)(32 * warp) << 16);
+        sum_l += tops[(half ^ 1) * kRows + 32 * quarter + lane];
         const float inv = sum_l > 0.f ? 1.f / sum_l : sum_l;  // 0 cannot be; NaN stays
-        float* row = reinterpret_cast<float*>(smem + (32 * warp + lane) * S::kOutStride);
+        float* row = reinterpret_cast<float*>(smem + (32 * quarter + lane) * S::kOutStride);
 #pragma unroll 1
-        for (int c = 0; c < kDim; c += 32) {
+        for (int c = half * (kDim / 2); c < (half + 1) * (kDim / 2); c += 32) {
             uint32_t o[32];
             ld32(lane_base + kColO + c, o);
             ld_wait(o);
@@ -618,7 +685,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prefix_kernel(const PrefixPara
                 *reinterpret_cast<float4*>(row + c + j) = make_float4(v[0], v[1], v[2], v[3]);
             }
         }
-        row[kDim] = (ref + lg2(sum_l)) * 0.6931471805599453f;
+        if (half == 0) row[kDim] = (ref + lg2(sum_l)) * 0.6931471805599453f;
     }
     fence_before();
     __syncthreads();
