@@ -649,9 +649,9 @@ __global__ void __launch_bounds__(kThreads, Shape<kDim, kBits, kNB>::kPerSm)
 #pragma unroll 1
         for (; cu < sb; cu += kWarps) {
             // every lane leaves the wait with the same answer
-            if (!failed && !__all_sync(0xffffffffu, mbar_try_wait(my_bars + 8 * stage, phase >> stage & 1u))) {
+            if (!failed && !__all_sync(0xffffffffu, mbar_try_wait_held(my_bars + 8 * stage, phase >> stage & 1u, kHoldNs))) {
                 const long long t0 = clock64();
-                while (!__all_sync(0xffffffffu, mbar_try_wait(my_bars + 8 * stage, phase >> stage & 1u))) {
+                while (!__all_sync(0xffffffffu, mbar_try_wait_held(my_bars + 8 * stage, phase >> stage & 1u, kHoldNs))) {
                     failed = __any_sync(0xffffffffu, clock64() - t0 > p.wait_cycles);
                     if (failed) break;
                 }
@@ -1002,7 +1002,7 @@ __global__ void __launch_bounds__(kThreads, Shape<kDim, kBits, kNB>::kPerSm)
         // the units issued and not done are in the next stages of the ring.
         for (int i = 0; i < min(issued, mine) - done; ++i) {
             const int at_stage = (done + i) % kStages;
-            mbar_wait_bounded(my_bars + 8 * at_stage, phase >> at_stage & 1u, p.wait_cycles);
+            mbar_wait_held(my_bars + 8 * at_stage, phase >> at_stage & 1u, p.wait_cycles);
         }
     }
 }

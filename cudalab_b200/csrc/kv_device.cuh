@@ -9,6 +9,8 @@
 
 #include <cstdint>
 
+#include "gemv_common.cuh"
+
 namespace clb {
 
 template <bool kBf16>
@@ -103,6 +105,33 @@ struct FastDiv {
 // Rows of 16-bit elements that 16-byte accesses may be used on.
 inline bool aligned16(const void* p, int64_t stride0, int64_t stride1) {
     return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && stride0 % 8 == 0 && stride1 % 8 == 0;
+}
+
+// One poll of an mbarrier phase that the hardware may hold for up to `hold_ns`
+// before it answers no: a warp that waits then issues next to nothing (plain
+// polls took half of the issue slots of the prefix kernel).
+__device__ __forceinline__ bool mbar_try_wait_held(uint32_t bar, uint32_t parity, uint32_t hold_ns) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity), "r"(hold_ns)
+        : "memory");
+    return ok != 0;
+}
+constexpr uint32_t kHoldNs = 20000;
+
+// Bounded wait on one phase, at most `budget` SM cycles and one poll more.
+__device__ __forceinline__ bool mbar_wait_held(uint32_t bar, uint32_t parity, long long budget) {
+    if (mbar_try_wait_held(bar, parity, kHoldNs)) return true;
+    const long long t0 = clock64();
+#pragma unroll 1
+    while (!mbar_try_wait_held(bar, parity, kHoldNs)) {
+        if (clock64() - t0 > budget) return false;
+    }
+    return true;
 }
 
 // Programmatic dependent launch: the kernel waits (griddepcontrol.wait) before

@@ -18,7 +18,7 @@
 //   * 8 warps, half a row's tokens a thread, do the softmax as in
 //     kv_attention.cu: p_j = 2^(s_j - m) summed in fp32, weights p_j vs_j in
 //     fp16, one lazy reference m per row near the maximum of s_j + log2 vs_j,
-//     packed fp32 pairs; O is only rescaled when a weight exceeds kMostWeight,
+//     O is only rescaled when a weight exceeds kMostWeight,
 //     which the two warps of a row find out with one barrier a tile.
 // S is double-buffered: the tensor cores compute tile i + 1's S and tile i -
 // 1's O while the softmax of tile i runs.
@@ -65,12 +65,6 @@ __device__ __forceinline__ float lg2(float x) {
     asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-__device__ __forceinline__ unsigned long long f2_mul(unsigned long long a, unsigned long long b) {
-    unsigned long long d;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-    return d;
-}
-
 __device__ __forceinline__ void fence_before() {
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
 }
@@ -210,9 +204,8 @@ template <int kDim, int kBits>
 struct PrefixShape {
     static constexpr int kRow = kDim * kBits / 8;
     static constexpr int kBlockBytes = kv_block_bytes(kRow);
-    static constexpr int kHalves = kDim / 64;             // 64-element columns of an operand
-    static constexpr int kHalfBytes = kTile * 128;
-    static constexpr int kOperandBytes = kHalves * kHalfBytes;
+    static constexpr int kHalfBytes = kTile * 128;        // 64 elements wide
+    static constexpr int kOperandBytes = kDim / 64 * kHalfBytes;
     static constexpr int kLoads = kRow / 32;              // 16-byte pieces per lane of a part
     static constexpr int kOutStride = kDim * 4 + 16;      // bytes of a staged output row
     // K and V twice each (the output is staged there at the end), per-token
@@ -225,47 +218,49 @@ struct PrefixShape {
     static_assert(kRows * kOutStride <= 4 * kOperandBytes, "room for the output");
 };
 
-// The 16-byte piece of a part that a lane holds in load `i`: its token row and
-// logical piece.  The lanes that store together (8) then fall on different
-// banks: int8 on two rows, int4 on four.
-template <int kBits>
-__device__ __forceinline__ void piece(int i, int lane, int* row, int* chunk, int halves) {
-    if (kBits == 8) {
-        *row = 8 * (i / halves) + (lane >> 2);
-        *chunk = 4 * (i % halves) + (lane & 3);
-    } else {
-        *row = lane >> 1;
-        *chunk = 2 * i + (lane & 1);
+// The 16-byte pieces of a block's part that a lane expands: load n is of token
+// row 8 (n / halves) + lane / 4 (int8) or lane / 2 (int4), and lanes that store
+// together (8) fall on different banks.  Both swizzles are exclusive ors of
+// address bits that the loads do not carry into, so a place is one number per
+// lane, exclusive or a constant, plus a constant:
+template <int kDim, int kBits>
+struct Pieces {
+    static constexpr int kRow = kDim * kBits / 8, kHalves = kDim / 64;
+    int from, to;  // place of piece 0 in the cache's part and in the operand
+    __device__ explicit Pieces(int lane) {
+        const int row = kBits == 8 ? lane >> 2 : lane >> 1, piece = kBits == 8 ? lane & 3 : lane & 1;
+        from = kv_offset<kRow>(row, 16 * piece);
+        to = row * 128 + (((kBits == 8 ? 2 : 4) * piece) ^ (row & 7)) * 16;
     }
-}
+    // load n: 64 elements on (another half of the operand), or 8 rows on (int8)
+    __device__ static constexpr int column(int n) { return n % kHalves; }
+    __device__ static constexpr int rows(int n) { return n / kHalves * 8; }
+    __device__ int source(int n) const {  // `from` of a half: kRow / kHalves bytes on
+        return (from ^ (column(n) * (kRow / kHalves))) + rows(n) * kRow;
+    }
+    __device__ int target(int n, int s) const {
+        return (to ^ (16 * s)) + column(n) * (kTile * 128) + rows(n) * 128;
+    }
+};
 
-// One 16-byte piece of whole values -> 2 (int8) or 4 (int4) 16-byte pieces of
-// halves in the operand's row `token`.
+// One 16-byte piece of whole values -> output piece s of 2 (int8) or 4 (int4).
 template <int kBits>
-__device__ __forceinline__ void expand(const uint4 raw, uint8_t* operand_base, int half_bytes,
-                                       int token, int chunk) {
+__device__ __forceinline__ uint4 expand(const uint4& raw, int s) {
     const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-    constexpr int kOut = 16 / kBits;  // pieces out
-    const int first = kOut * chunk;
-    uint8_t* row = operand_base + (first >> 3) * half_bytes + token * 128;
-#pragma unroll
-    for (int s = 0; s < kOut; ++s) {
-        __half2 q[4];
-        if (kBits == 8) {
-            __half2 lo[2], hi[2];
-            int8x4_to_h2(w[2 * s], lo);
-            int8x4_to_h2(w[2 * s + 1], hi);
-            q[0] = lo[0], q[1] = lo[1], q[2] = hi[0], q[3] = hi[1];
-        } else {
-            const uint32_t up = w[s] >> 8;
-            q[0] = __hadd2(u32_as_h2(lop3_sel_xor_i<0x000F000Fu, 0x64086408u>(w[s])), h2_const(kH_m1032));
-            q[1] = __hadd2(u32_as_h2(lop3_sel_xor_i<0x00F000F0u, 0x54805480u>(w[s])), h2_const(kH_m72));
-            q[2] = __hadd2(u32_as_h2(lop3_sel_xor_i<0x000F000Fu, 0x64086408u>(up)), h2_const(kH_m1032));
-            q[3] = __hadd2(u32_as_h2(lop3_sel_xor_i<0x00F000F0u, 0x54805480u>(up)), h2_const(kH_m72));
-        }
-        *reinterpret_cast<uint4*>(row + (((first + s) & 7) ^ (token & 7)) * 16) =
-            *reinterpret_cast<const uint4*>(q);
+    __half2 q[4];
+    if (kBits == 8) {
+        __half2 lo[2], hi[2];
+        int8x4_to_h2(w[2 * s], lo);
+        int8x4_to_h2(w[2 * s + 1], hi);
+        q[0] = lo[0], q[1] = lo[1], q[2] = hi[0], q[3] = hi[1];
+    } else {
+        const uint32_t up = w[s] >> 8;
+        q[0] = __hadd2(u32_as_h2(lop3_sel_xor_i<0x000F000Fu, 0x64086408u>(w[s])), h2_const(kH_m1032));
+        q[1] = __hadd2(u32_as_h2(lop3_sel_xor_i<0x00F000F0u, 0x54805480u>(w[s])), h2_const(kH_m72));
+        q[2] = __hadd2(u32_as_h2(lop3_sel_xor_i<0x000F000Fu, 0x64086408u>(up)), h2_const(kH_m1032));
+        q[3] = __hadd2(u32_as_h2(lop3_sel_xor_i<0x00F000F0u, 0x54805480u>(up)), h2_const(kH_m72));
     }
+    return *reinterpret_cast<const uint4*>(q);
 }
 
 template <int kDim, int kBits, bool kBf16>
@@ -319,15 +314,19 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prefix_kernel(const PrefixPara
     fence_after();
     const uint32_t tmem = *s_tmem;
 
-    // A bounded wait; false (for the whole warp or the one thread) once any
-    // role has given up.
+    // A bounded wait; false once it or any other of the CTA has run out.
     auto wait = [&](uint32_t bar, int phase) -> bool {
-        bool ok = *s_fail == 0 && mbar_wait_bounded(bar, (uint32_t)phase & 1u, p.wait_cycles);
-        if (!ok && *s_fail == 0) {
-            atomicCAS(&g_kv_prefix_status, 0, kStatusTimeoutKv);
-            *s_fail = 1;
+        if (mbar_try_wait_held(bar, (uint32_t)phase & 1u, kHoldNs)) return true;
+        const long long t0 = clock64();
+        while (!mbar_try_wait_held(bar, (uint32_t)phase & 1u, kHoldNs)) {
+            if (*s_fail) return false;
+            if (clock64() - t0 > p.wait_cycles) {
+                atomicCAS(&g_kv_prefix_status, 0, kStatusTimeoutKv);
+                *s_fail = 1;
+                return false;
+            }
         }
-        return ok;
+        return true;
     };
 
     float sum_l = 0.f, ref = -INFINITY;  // of this thread's row (and half of the tokens)
@@ -387,8 +386,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prefix_kernel(const PrefixPara
         if (lane == 0) mbar_arrive(pfull);  // phase 0: Q is there
 
         const bool scaled = __any_sync(0xffffffffu, unit != 1.f);
-        const unsigned long long unit2 = f2_pack(unit, unit);
-        unsigned long long l2 = f2_pack(0.f, 0.f);
+        float l2[2] = {0.f, 0.f};
         bool ok = true;
         for (int i = 0; i < tiles && ok; ++i) {
             const int b = i & 1;
@@ -402,21 +400,21 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prefix_kernel(const PrefixPara
             // 16 columns of S have come; columns past the end at -inf
             auto take_s = [&](int c, uint32_t (&s)[16]) {
                 ld_wait(s);
-                if (live < 16 * c + 16) {
+                if (kBf16 && scaled) {
 #pragma unroll
-                    for (int j = 0; j < 16; ++j)
-                        if (16 * c + j >= live) s[j] = 0xff800000u;
+                    for (int j = 0; j < 16; ++j) s[j] = __float_as_uint(__uint_as_float(s[j]) * unit);
+                }
+                if (live < 16 * c + 16) {
+#pragma unroll 1
+                    for (int j = max(0, live - 16 * c); j < 16; ++j)
+#pragma unroll
+                        for (int x = 0; x < 16; ++x)
+                            if (x == j) s[x] = 0xff800000u;
                 }
             };
-            // base-2 logits of 4 columns, less the reference
-            auto logits = [&](const uint32_t* s, int col, unsigned long long nref,
-                              unsigned long long& z0, unsigned long long& z1) {
-                const ulonglong2 ks = *reinterpret_cast<const ulonglong2*>(num + col);
-                unsigned long long x0 = f2_pack(__uint_as_float(s[0]), __uint_as_float(s[1]));
-                unsigned long long x1 = f2_pack(__uint_as_float(s[2]), __uint_as_float(s[3]));
-                if (kBf16 && scaled) x0 = f2_mul(x0, unit2), x1 = f2_mul(x1, unit2);
-                z0 = f2_fma(x0, ks.x, nref);
-                z1 = f2_fma(x1, ks.y, nref);
+            // base-2 logit of a column, less the reference
+            auto logit = [&](uint32_t s, float ks, float nref) {
+                return fmaf(__uint_as_float(s), ks, nref);
             };
             bool waited = i == 0;  // for the MMAs of tile i - 1, which read P and write O
             auto previous_done = [&]() {
@@ -432,10 +430,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prefix_kernel(const PrefixPara
             // their barrier alone, so neither can wait for the other in vain.
             bool fresh = i == 0;
             for (int tries = 0;; ++tries, fresh = false) {
-                unsigned long long try_l = l2;
+                float try_l[2] = {l2[0], l2[1]};
                 __half2 most = __half2half2(__half(0.f));
                 if (good && !fresh) {
-                    const unsigned long long nref = f2_pack(-ref, -ref);
                     uint32_t s[2][16], packed[16];
                     ld16(s_at, s[0]);
 #pragma unroll
@@ -444,21 +441,15 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prefix_kernel(const PrefixPara
                         if (c < 3) ld16(s_at + 16 * (c + 1), s[(c + 1) & 1]);  // under the arithmetic
 #pragma unroll
                         for (int j = 0; j < 16; j += 4) {
-                            unsigned long long z0, z1;
-                            float x, y, z, w;
-                            logits(s[c & 1] + j, 16 * c + j, nref, z0, z1);
-                            f2_unpack(z0, x, y);
-                            f2_unpack(z1, z, w);
-                            z0 = f2_pack(ex2(x), ex2(y));
-                            z1 = f2_pack(ex2(z), ex2(w));
-                            try_l = f2_add(try_l, f2_add(z0, z1));
-                            const ulonglong2 vs = *reinterpret_cast<const ulonglong2*>(
-                                num + kTile + 16 * c + j);
-                            f2_unpack(f2_mul(z0, vs.x), x, y);
-                            f2_unpack(f2_mul(z1, vs.y), z, w);
+                            const uint32_t* t = s[c & 1] + j;
+                            const float4 ks = *reinterpret_cast<const float4*>(num + 16 * c + j);
+                            const float4 vs = *reinterpret_cast<const float4*>(num + kTile + 16 * c + j);
+                            const float x = ex2(logit(t[0], ks.x, -ref)), y = ex2(logit(t[1], ks.y, -ref));
+                            const float z = ex2(logit(t[2], ks.z, -ref)), w = ex2(logit(t[3], ks.w, -ref));
+                            try_l[0] += x, try_l[1] += y, try_l[0] += z, try_l[1] += w;
                             uint32_t* to = packed + 8 * (c & 1) + j / 2;
-                            to[0] = pack2<false>(x, y);
-                            to[1] = pack2<false>(z, w);
+                            to[0] = pack2<false>(x * vs.x, y * vs.y);
+                            to[1] = pack2<false>(z * vs.z, w * vs.w);
                             most = __hmax2(most, __hmax2(u32_as_h2(to[0]), u32_as_h2(to[1])));
                         }
                         if (c & 1) {
@@ -471,7 +462,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prefix_kernel(const PrefixPara
                 // (a second reference always fits; the bound is for the loop's sake)
                 const bool over = fresh || (tries < 3 && fmaxf(m2.x, m2.y) > kMostWeight);
                 if (!any_of_rows(1 + quarter, over || !good)) {
-                    l2 = try_l;
+                    l2[0] = try_l[0], l2[1] = try_l[1];
                     break;
                 }
                 if (any_of_rows(1 + quarter, !good)) {
@@ -488,15 +479,13 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prefix_kernel(const PrefixPara
                     take_s(c, s);
 #pragma unroll
                     for (int j = 0; j < 16; j += 4) {
-                        unsigned long long z0, z1;
-                        float x, y, z, w;
-                        logits(s + j, 16 * c + j, f2_pack(0.f, 0.f), z0, z1);
-                        f2_unpack(z0, x, y);
-                        f2_unpack(z1, z, w);
-                        // a zero scale has all-zero values: any log will do
+                        const float4 ks = *reinterpret_cast<const float4*>(num + 16 * c + j);
                         const float4 vs = *reinterpret_cast<const float4*>(num + kTile + 16 * c + j);
-                        x += fmaxf(lg2(vs.x), -24.f), y += fmaxf(lg2(vs.y), -24.f);
-                        z += fmaxf(lg2(vs.z), -24.f), w += fmaxf(lg2(vs.w), -24.f);
+                        // a zero scale has all-zero values: any log will do
+                        const float x = logit(s[j], ks.x, fmaxf(lg2(vs.x), -24.f));
+                        const float y = logit(s[j + 1], ks.y, fmaxf(lg2(vs.y), -24.f));
+                        const float z = logit(s[j + 2], ks.z, fmaxf(lg2(vs.z), -24.f));
+                        const float w = logit(s[j + 3], ks.w, fmaxf(lg2(vs.w), -24.f));
                         top = fmaxf(fmaxf(fmaxf(top, x), y), fmaxf(z, w));
                     }
                 }
@@ -511,7 +500,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prefix_kernel(const PrefixPara
                 if (top == -INFINITY) top = 0.f;  // a row of NaN has no largest score
                 const float f = ex2(ref - top);
                 ref = top;
-                l2 = f2_mul(l2, f2_pack(f, f));
+                l2[0] *= f, l2[1] *= f;
                 if (i > 0) {
 #pragma unroll 1
                     for (int c = half * (kDim / 2); c < (half + 1) * (kDim / 2); c += 32) {
@@ -534,9 +523,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prefix_kernel(const PrefixPara
         if (ok && __all_sync(0xffffffffu, wait(vempty + 8 * ((tiles - 1) & 1), (tiles - 1) >> 1))) {
             fence_after();
             finished = true;
-            float x, y;
-            f2_unpack(l2, x, y);
-            sum_l = x + y;
+            sum_l = l2[0] + l2[1];
             tops[half * kRows + in_tile] = sum_l;
         }
         // nothing of this thread is in flight when the memory is freed
@@ -546,6 +533,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prefix_kernel(const PrefixPara
         // ---------------- expansion: one cache block a warp ----------------
         const int w = warp - kSoftWarps;
         uint32_t where = 0xffffffffu;  // lane i: the block of the 32-tile batch's i-th tile
+        const Pieces<kDim, kBits> pieces(lane);
         uint4 raw[2][S::kLoads];       // a block's K and V on their way
         __half scale = __half(0.f);
         uint32_t at = 0xffffffffu;
@@ -577,21 +565,17 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prefix_kernel(const PrefixPara
             }
             const uint8_t* block = a.pages + (int64_t)at * S::kBlockBytes;
 #pragma unroll
-            for (int n = 0; n < S::kLoads; ++n) {
-                int row, chunk;
-                piece<kBits>(n, lane, &row, &chunk, S::kHalves);
-                raw[x][n] = load_now(block + x * kKvBlock * S::kRow +
-                                     kv_offset<S::kRow>(row, 16 * chunk));
-            }
+            for (int n = 0; n < S::kLoads; ++n)
+                raw[x][n] = load_now(block + x * kKvBlock * S::kRow + pieces.source(n));
             if (x == 0) scale = reinterpret_cast<const __half*>(block + 2 * kKvBlock * S::kRow)[lane];
         };
         auto store = [&](int x, uint8_t* to) {
 #pragma unroll
-            for (int n = 0; n < S::kLoads; ++n) {
-                int row, chunk;
-                piece<kBits>(n, lane, &row, &chunk, S::kHalves);
-                expand<kBits>(raw[x][n], to, S::kHalfBytes, kKvBlock * w + row, chunk);
-            }
+            for (int n = 0; n < S::kLoads; ++n)
+#pragma unroll
+                for (int o = 0; o < 16 / kBits; ++o)
+                    *reinterpret_cast<uint4*>(to + kKvBlock * w * 128 + pieces.target(n, o)) =
+                        expand<kBits>(raw[x][n], o);
         };
         auto arrive = [&](uint32_t bar) {
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -657,7 +641,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prefix_kernel(const PrefixPara
         }
         if (!ok && committed > 0) {
             // the MMAs issued so far end before the memory they use is given up
-            mbar_wait_bounded(vempty + 8 * ((committed - 1) & 1), (uint32_t)(committed - 1) >> 1 & 1u,
+            mbar_wait_held(vempty + 8 * ((committed - 1) & 1), (uint32_t)(committed - 1) >> 1 & 1u,
                               p.wait_cycles);
         }
     }
