@@ -861,6 +861,7 @@ int cl_kvattention(const void* q, const uint8_t* pages, const int32_t* page_tabl
             return bad(op, "the prefix spans too many blocks for one launch");
         const bool tensor = clb::kv_prefix_takes(f);
         a.front_parts = tensor ? clb::kv_prefix_parts(f) : 1;
+        a.front_by_tensor_cores = tensor;
         a.front = f.out_f32 = prefix_scratch;
         a.front_lse = f.lse = prefix_scratch + (size_t)a.front_parts * d->batch * d->new_tokens *
                                                    d->q_heads * d->head_dim;

@@ -235,7 +235,15 @@ __global__ void __launch_bounds__(kThreads, Shape<kDim, kBits, kNB>::kPerSm)
         for (int i = 0; i < kStages; ++i) mbar_init(my_bars + 8 * i, 1);
         fence_barrier_init();
     }
-    pdl_wait_prior_grids();
+    // Over a prefix's tensor-core launch everything up to the first result runs
+    // beside it: that launch lets this one begin only after the kernel before
+    // it has completed, and writes nothing but what `front` points to.  Before
+    // a result is written (and the front read, or the workspace used by a
+    // launch further back) `settle` waits for it.
+    if (!a.front_by_tensor_cores) pdl_wait_prior_grids();
+    auto settle = [&]() {
+        if (a.front_by_tensor_cores) pdl_wait_prior_grids();
+    };
 
     // Units of each sequence (a window drops the blocks in front of the first
     // token that any row sees), and how the line of all segments is cut.
@@ -373,6 +381,7 @@ __global__ void __launch_bounds__(kThreads, Shape<kDim, kBits, kNB>::kPerSm)
 
     // Sequences with nothing to read (their rows see no cached token).
     auto write_empty = [&](int b, int part0, int part1) {
+        settle();
         const int n = rows * (kDim / 4);
         for (int h = part0; h < part1; ++h)
             for (int i = tid; i < n; i += kThreads) {
@@ -846,6 +855,7 @@ __global__ void __launch_bounds__(kThreads, Shape<kDim, kBits, kNB>::kPerSm)
         // ---- the segment's end: the warps' results meet in shared memory ----
         // Value v of a lane: 4 elements of row 2t + v / (kSteps / 2) (+ 8 n),
         // stored lane by lane; warp w joins and writes the values w, w + 4, ...
+        settle();
         const Segment now = seg;
         next_segment(seg);
         const bool whole = sa == now.begin && sb == now.begin + now.units;

@@ -103,6 +103,7 @@ struct KvAttentionArgs {
     const float* front;      // fp32 results over tokens in front of these, or null:
     const float* front_lse;  // [front_parts] of them and their lse
     int front_parts;
+    int front_by_tensor_cores;  // written by the launch just before (launch_kv_prefix)
     void* workspace;
 };
 // Workspace bytes of a call (zero-filled before its first use).

@@ -267,8 +267,9 @@ template <int kDim, int kBits, bool kBf16>
 __global__ void __launch_bounds__(kThreads, 1) kv_prefix_kernel(const PrefixParams p) {
     using S = PrefixShape<kDim, kBits>;
     extern __shared__ uint8_t smem_raw[];
-    uint8_t* smem = reinterpret_cast<uint8_t*>(
-        (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+    // aligned for the swizzle by an offset, so that the compiler still knows the
+    // accesses for shared memory
+    uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     uint8_t* kbuf = smem;                          // [2] K operands
     uint8_t* vbuf = smem + 2 * S::kOperandBytes;   // [2] V operands
     float* numbers = reinterpret_cast<float*>(smem + S::kNumbers);  // [4][2][kTile]
@@ -287,7 +288,6 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prefix_kernel(const PrefixPara
     const int tiles = min(p.part_tiles, p.tiles - tile0);
     const int length = a.fixed_length;
 
-    pdl_allow_dependents();
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) {
             mbar_init(kfull + 8 * i, kFillWarps);
@@ -301,7 +301,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prefix_kernel(const PrefixPara
         *s_fail = 0;
         fence_barrier_init();
     }
+    // The launch over the sequences' own tokens may begin once every CTA here has
+    // seen the preceding kernel complete: it then waits for this grid only
+    // before it joins the results (KvAttentionArgs::front_by_tensor_cores).
     pdl_wait_prior_grids();
+    pdl_allow_dependents();
     if (warp == 0) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
                          smem_u32(const_cast<uint32_t*>(s_tmem))),
@@ -339,37 +343,45 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prefix_kernel(const PrefixPara
         const int in_tile = 32 * quarter + lane, r = row0 + in_tile;
         float unit = 1.f;  // what the row was divided by (a power of two)
         {
+            // this half of the row, all of it on its way at once
             const int i0 = p.group.div(r);
             const uint16_t* src = static_cast<const uint16_t*>(a.q) + i0 * a.q_new +
-                                  ((head - i0) * a.group + r) * a.q_head;
-            auto load = [&](int d) {
-                if (r >= p.rows) return make_uint4(0, 0, 0, 0);
-                return p.q_vec ? load8<kBf16, true>(src, d) : load8<kBf16, false>(src, d);
-            };
+                                  ((head - i0) * a.group + r) * a.q_head + half * (kDim / 2);
+            uint4 raw[kDim / 16];
+#pragma unroll
+            for (int c = 0; c < kDim / 16; ++c) {
+                raw[c] = make_uint4(0, 0, 0, 0);
+                if (r < p.rows)
+                    raw[c] = p.q_vec ? load8<kBf16, true>(src, 8 * c) : load8<kBf16, false>(src, 8 * c);
+            }
             // bf16 rows that fp16 would not hold are scaled into its range
             float down = 1.f;
             if (kBf16) {
                 float top = 0.f;
-#pragma unroll 4
-                for (int d = 0; d < kDim; d += 8) {
+#pragma unroll
+                for (int c = 0; c < kDim / 16; ++c) {
                     float x[8];
-                    unpack8<kBf16>(load(d), x);
+                    unpack8<kBf16>(raw[c], x);
 #pragma unroll
                     for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[i]));
                 }
+                tops[half * kRows + in_tile] = top;
+                any_of_rows(1 + quarter, false);
+                top = fmaxf(top, tops[(half ^ 1) * kRows + in_tile]);
+                any_of_rows(1 + quarter, false);  // read before it is written again
                 const int e = (int)(__float_as_uint(top) >> 23) - 127;
                 if ((e >= 15 || e < -6) && e > -126 && e < 127) {
                     down = __uint_as_float((uint32_t)(127 - e) << 23);
                     unit = __uint_as_float((uint32_t)(127 + e) << 23);
                 }
             }
-#pragma unroll 1
-            for (int d = half * (kDim / 2); d < (half + 1) * (kDim / 2); d += 32) {
+#pragma unroll
+            for (int d = 0; d < kDim / 2; d += 32) {
                 uint32_t packed[16];
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
                     float x[8];
-                    unpack8<kBf16>(load(d + 8 * c), x);
+                    unpack8<kBf16>(raw[d / 8 + c], x);
 #pragma unroll
                     for (int i = 0; i < 8; ++i) x[i] *= down;
 #pragma unroll
@@ -377,7 +389,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prefix_kernel(const PrefixPara
                         packed[4 * c + i] = kBits == 8 ? pack2<false>(x[2 * i], x[2 * i + 1])
                                                        : pack2<false>(x[i], x[i + 4]);
                 }
-                st16(lane_base + kColQ + d / 2, packed);
+                st16(lane_base + kColQ + (half * (kDim / 2) + d) / 2, packed);
             }
             wait_st();
             fence_before();
@@ -718,8 +730,12 @@ int cut(int items, int tiles) {
 }  // namespace
 
 bool kv_prefix_takes(const KvAttentionArgs& a) {
-    return a.head_dim <= 128 && (int64_t)a.new_tokens * a.group >= 32 &&
-           (int64_t)a.new_tokens * a.group < (1 << 24);
+    // Measured with 8 heads of 128 (int8), both kernels with the launch that
+    // joins them, us at 128 / 512 / 2048 / 8192 tokens: 32 rows 15.0 15.7 19.6
+    // 26.4 here, 14.4 18.3 19.8 32.1 on the register-fed kernel; 256 rows 17.0
+    // 18.3 21.6 35.8 against 16.1 20.0 32.1 72.1.
+    const int64_t rows = (int64_t)a.new_tokens * a.group;
+    return a.head_dim <= 128 && rows >= 32 && rows < (1 << 24) && a.fixed_length >= 512;
 }
 
 int kv_prefix_parts(const KvAttentionArgs& a) {
