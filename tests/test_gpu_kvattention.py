@@ -69,7 +69,7 @@ def _check(out, lse, q, c, scale, window=0, prefix=None):
         assert np.array_equal(np.isinf(rl), np.isinf(lse[b])), (b, n)
         fin = np.isfinite(rl)
         ltol = oa.lse_tolerance(rl, mag, tokens, q.shape[-1])
-        assert (np.abs(lse[b] - rl)[fin] <= ltol[fin]).all(), (b, n)
+        assert (np.abs(lse[b][fin] - rl[fin]) <= ltol[fin]).all(), (b, n)
     assert nat.device_status(clear=True) == 0
 
 
@@ -191,6 +191,95 @@ def test_shared_prefix(prefix, D, bits, group, n, dtype):
     _check(out, lse, q, c, D ** -0.5, prefix=p)
     none = att.forward_shared(q, pages, prefix_pages, 0, c.table, c.len_tensor())
     assert torch.equal(none, att.forward(q, pages, c.table, c.len_tensor()))
+
+
+# The tensor-core prefix kernel (from 32 rows and 512 tokens): rows around its
+# 128-row tiles, lengths around its 128-token tiles and the parts they are cut
+# into, every format, one and several new tokens.
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=str)
+@pytest.mark.parametrize("D,bits", [(64, 8), (64, 4), (128, 8), (128, 4)])
+@pytest.mark.parametrize("batch,n,group,prefix", [(32, 1, 1, 512), (16, 1, 8, 513), (43, 1, 3, 640),
+                                                  (9, 3, 5, 1000), (65, 1, 4, 2049)])
+def test_shared_prefix_on_tensor_cores(batch, n, group, prefix, D, bits, dtype):
+    p = Cache([prefix], 1, D, bits, 48, seed=prefix, spread=1.0, scales=1.0)
+    c = Cache([i % 4 for i in range(batch)], 1, D, bits, 48, seed=prefix + 1)
+    pages = torch.cat((c.pages, p.pages))
+    q = _q(batch, n, group, D, dtype, seed=prefix + 2, scale=2.0)
+    att = build("kvattention")
+    out, lse = att.forward_shared(q, pages, p.table[0] + c.pages.shape[0], prefix, c.table,
+                                  c.len_tensor(), workspace=att.workspace(), return_lse=True)
+    _check(out, lse, q, c, D ** -0.5, prefix=p)
+
+
+def test_shared_prefix_large_and_small_queries():
+    """bf16 rows outside fp16's range, rows of zeros and a NaN, beside ordinary ones."""
+    p = Cache([600], 1, 128, 8, 64, seed=31)
+    c = Cache([2] * 40, 1, 128, 8, 64, seed=32)
+    pages = torch.cat((c.pages, p.pages))
+    q = _q(40, 1, 2, 128, BF16, seed=33)
+    q[1], q[2], q[3] = q[1] * 1e30, q[2] * 1e-30, 0
+    att = build("kvattention")
+    args = (pages, p.table[0] + c.pages.shape[0], 600, c.table, c.len_tensor())
+    scale = 1e-30  # the large rows then have ordinary scores, the others none to speak of
+    out, lse = att.forward_shared(q, *args, scale=scale, return_lse=True)
+    _check(out, lse, q, c, scale, prefix=p)
+    q = _q(40, 1, 2, 128, BF16, seed=34)
+    clean = att.forward_shared(q, *args)
+    q[7, 0, 1, 5] = float("nan")
+    out = att.forward_shared(q, *args)
+    bad = torch.isnan(out).any(-1)
+    assert bad.sum() == 1 and bad[7, 0, 1] and torch.equal(out[~bad], clean[~bad])
+
+
+def test_shared_prefix_rising_scores():
+    """Scores that grow along the prefix move the softmax reference at every tile, and one
+    late token outweighs all before it."""
+    n, D = 1300, 128
+    p = Cache([n], 1, D, 8, 64, seed=41)
+    c = Cache([1] * 33, 1, D, 8, 64, seed=42)
+    g = torch.Generator().manual_seed(43)
+    d = torch.randn(D, generator=g)
+    k = torch.randn(n, 1, D, generator=g) * 0.1 + d * torch.linspace(-1, 1, n)[:, None, None]
+    k[1200] = 6 * d
+    j = torch.arange(n)
+    slots = p.table[0].cpu().long()[j // 64] * 64 + j % 64
+    p.ext.write(k.half().cuda(), torch.from_numpy(p.v[0]).half().cuda(), p.pages, slots.cuda())
+    qk, s = oa.quantise(k.half().float().numpy(), 8)
+    p.k[0] = qk.astype(np.float64) * s.astype(np.float64)[..., None]
+    qv, s = oa.quantise(torch.from_numpy(p.v[0]).half().float().numpy(), 8)
+    p.v[0] = qv.astype(np.float64) * s.astype(np.float64)[..., None]
+    pages = torch.cat((c.pages, p.pages))
+    q = (d + 0.3 * torch.randn(33, 1, 4, D, generator=g)).half().cuda()
+    att = build("kvattention")
+    out, lse = att.forward_shared(q, pages, p.table[0] + c.pages.shape[0], n, c.table,
+                                  c.len_tensor(), scale=0.4, return_lse=True)
+    _check(out, lse, q, c, 0.4, prefix=p)
+
+
+def test_shared_prefix_in_a_graph_and_on_another_stream():
+    p = Cache([700], 2, 128, 4, 32, seed=51)
+    c = Cache([i % 50 for i in range(24)], 2, 128, 4, 32, seed=52)
+    pages = torch.cat((c.pages, p.pages))
+    q = _q(24, 1, 8, 128, F16, seed=53)
+    att = build("kvattention")
+    ws = att.workspace()
+    args = (pages, p.table[0] + c.pages.shape[0], 700, c.table, c.len_tensor())
+    ref = att.forward_shared(q, *args, workspace=ws)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=s):
+            # q written by the kernel before: the launches must wait for it
+            q2 = q * 1.0
+            out = att.forward_shared(q2, *args, workspace=ws)
+        for _ in range(5):
+            q.neg_()
+            graph.replay()
+        q.neg_()
+        graph.replay()
+    s.synchronize()
+    assert torch.equal(out, ref)
 
 
 def test_index_errors_are_recorded():
