@@ -1017,11 +1017,13 @@ __global__ void __launch_bounds__(kThreads, Shape<kDim, kBits, kNB>::kPerSm)
     }
 }
 
-// Blocks of all segments if every sequence were as long as its page table.
+// Blocks of all segments if every sequence were as long as its page table (or
+// reached back as far as the window lets its rows see).
 int64_t longest_line(const KvAttentionArgs& a, int64_t row_tiles) {
-    const int64_t blocks = a.fixed_length >= 0
-                               ? (a.fixed_length + kKvBlock - 1) / kKvBlock
-                               : (int64_t)a.max_pages * (a.page_size / kKvBlock);
+    int64_t blocks = a.fixed_length >= 0 ? (a.fixed_length + kKvBlock - 1) / kKvBlock
+                                         : (int64_t)a.max_pages * (a.page_size / kKvBlock);
+    if (a.window > 0)
+        blocks = std::min(blocks, ((int64_t)a.window + a.new_tokens - 2) / kKvBlock + 2);
     return blocks * a.batch * a.kv_heads * row_tiles;
 }
 
