@@ -126,7 +126,8 @@ def _binding_cmd(out: Path) -> list[str]:
              f"-DTORCH_EXTENSION_NAME={BINDING_NAME}", "-DTORCH_API_INCLUDE_EXTENSION_H",
              f"-D_GLIBCXX_USE_CXX11_ABI={abi}"]
             + [f"-I{p}" for p in inc]
-            + [f"-L{torch_lib}", "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_python",
+            + [f"-L{torch_lib}", "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_cuda",
+               "-ltorch_python",
                f"-L{LIB_DIR}", "-lcudalab_gemv", "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{torch_lib}"])
 
 
