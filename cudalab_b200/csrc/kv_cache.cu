@@ -29,7 +29,7 @@ namespace {
 
 __device__ int g_kv_status;
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 128;
 
 // Place of a slot: its page's block, and the token's row j in the block.
 struct Place {

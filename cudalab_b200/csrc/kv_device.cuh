@@ -107,6 +107,20 @@ inline bool aligned16(const void* p, int64_t stride0, int64_t stride1) {
     return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && stride0 % 8 == 0 && stride1 % 8 == 0;
 }
 
+// 16-byte asynchronous copies to shared memory, in groups.
+__device__ __forceinline__ void copy16(void* to, const void* from, bool go) {
+    if (go)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(to)), "l"(from)
+                     : "memory");
+}
+__device__ __forceinline__ void copies_end_group() {
+    asm volatile("cp.async.commit_group;" ::: "memory");
+}
+template <int kLeft>
+__device__ __forceinline__ void copies_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory");
+}
+
 // One poll of an mbarrier phase that the hardware may hold for up to `hold_ns`
 // before it answers no: a warp that waits then issues next to nothing (plain
 // polls took half of the issue slots of the prefix kernel).

@@ -94,6 +94,16 @@ def test_zero_rows_empty_and_extremes():
     assert bad.sum() == 1 and bad[1, 1]
 
 
+def test_infinity_past_the_rotation_stays_alone():
+    q, k, _, _, table, pos = _case(3, 2, 1, 128, 32, torch.float16, seed=11)
+    q = q.contiguous()
+    q[1, 0, 70] = float("inf")
+    for interleaved in (False, True):
+        y, _ = build("qknorm_rope").forward(q, k, None, None, table, pos, interleaved=interleaved)
+        assert torch.equal(y[..., 32:], q[..., 32:])
+        assert torch.isfinite(y).sum() == y.numel() - 1
+
+
 def test_position_outside_the_table_is_recorded():
     q, k, qw, kw, table, pos = _case(2, 2, 1, 64, 64, torch.float16, seed=7)
     pos[1] = table.shape[0]
