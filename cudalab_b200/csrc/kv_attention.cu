@@ -92,21 +92,23 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
     return r;
 }
 
-// K's fields as halves without an arithmetic instruction: the field with its
-// sign bit flipped, u = k + bias (bias 128 or 8), placed in the low bits of a
-// half is the subnormal u 2^-24 (u 2^-20 four bits up), exactly, and the tensor
-// cores take subnormals as they are.  What the bias adds to a score, bias sum_d
-// q_d, is taken off in fp32 with the scales.
+// K's fields as halves without a conversion: the field with its sign bit
+// flipped, u = k + bias (bias 128 or 8), placed in the mantissa of a half whose
+// exponent is zero is the subnormal u 2^-22 (int8, bits 2 to 9) or u 2^-20
+// (int4, bits 4 to 7), exactly, and the tensor cores take subnormals as they
+// are.  What the bias adds to a score, bias sum_d q_d, is taken off in fp32 with
+// the scales.  The place matters: the tensor cores line products up by their
+// operands' exponents and drop what falls below, so a field in the lowest bits
+// loses as many bits of the sum as there are zeros above it.  One place for all
+// fields costs one more shift a word of int8, two of int4, than the lowest bits
+// (the log-sum-exp of some ten tokens of int4 was 1.8e-6 of itself off there).
 //
-// Bytes 0 and 2 of w as a pair; 1 and 3 are the same of w >> 8.
-__device__ __forceinline__ uint32_t biased_bytes02(uint32_t w) {
-    return lop3_sel_xor_i<0x00FF00FFu, 0x00800080u>(w);
+// Bytes 0 and 2 of w << 2 or, of w >> 6, bytes 1 and 3 of w.
+__device__ __forceinline__ uint32_t biased_bytes(uint32_t w) {
+    return lop3_sel_xor_i<0x03FC03FCu, 0x02000200u>(w);
 }
-// Nibbles 0 and 4 (2^-24), and 1 and 5 (2^-20), of w; 2, 6 and 3, 7 are the same of w >> 8.
-__device__ __forceinline__ uint32_t biased_nibbles04(uint32_t w) {
-    return lop3_sel_xor_i<0x000F000Fu, 0x00080008u>(w);
-}
-__device__ __forceinline__ uint32_t biased_nibbles15(uint32_t w) {
+// Nibbles 1 and 5 of w; of w << 4, w >> 4, w >> 8: 0 and 4, 2 and 6, 3 and 7.
+__device__ __forceinline__ uint32_t biased_nibbles(uint32_t w) {
     return lop3_sel_xor_i<0x00F000F0u, 0x00800080u>(w);
 }
 
@@ -589,9 +591,7 @@ __global__ void __launch_bounds__(kThreads, Shape<kDim, kBits, kNB>::kPerSm)
 
         // q as B fragments.  Rows are brought to [1, 2) by a power of two (exact;
         // elements 2^14 below their row's largest lose bits that fp32 sums would
-        // not keep either).  int4: the elements that meet nibbles of 2^-24 are
-        // scaled by 2^4, so that all products stand for q k 2^-20 (int8: 2^-24).
-        // rs brings a score to base-2 logits, qc is what the bias adds to it.
+        // not keep either).  rs brings a score to base-2 logits, qc is what the bias adds to it.
         uint32_t qf[kNB][kSteps][2];
         float rs[kNB][2], qc[kNB][2];
 #pragma unroll
@@ -621,7 +621,7 @@ __global__ void __launch_bounds__(kThreads, Shape<kDim, kBits, kNB>::kPerSm)
             sum += __shfl_xor_sync(0xffffffffu, sum, 1);
             sum += __shfl_xor_sync(0xffffffffu, sum, 2);
             sum *= (kBits == 8 ? 128.f : 8.f) * unit;
-            unit *= kBits == 8 ? 16777216.f : 1048576.f;  // 2^24, 2^20
+            unit *= kBits == 8 ? 4194304.f : 1048576.f;  // 2^22, 2^20
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 rs[n][c] = __shfl_sync(0xffffffffu, unit, 8 * t + 4 * c);
@@ -633,9 +633,9 @@ __global__ void __launch_bounds__(kThreads, Shape<kDim, kBits, kNB>::kPerSm)
                     qf[n][w][0] = pack2<false>(x[4 * w], x[4 * w + 2]);
                     qf[n][w][1] = pack2<false>(x[4 * w + 1], x[4 * w + 3]);
                 } else {
-                    qf[n][2 * w][0] = pack2<false>(16.f * x[8 * w], 16.f * x[8 * w + 4]);
+                    qf[n][2 * w][0] = pack2<false>(x[8 * w], x[8 * w + 4]);
                     qf[n][2 * w][1] = pack2<false>(x[8 * w + 1], x[8 * w + 5]);
-                    qf[n][2 * w + 1][0] = pack2<false>(16.f * x[8 * w + 2], 16.f * x[8 * w + 6]);
+                    qf[n][2 * w + 1][0] = pack2<false>(x[8 * w + 2], x[8 * w + 6]);
                     qf[n][2 * w + 1][1] = pack2<false>(x[8 * w + 3], x[8 * w + 7]);
                 }
             }
@@ -682,27 +682,37 @@ __global__ void __launch_bounds__(kThreads, Shape<kDim, kBits, kNB>::kPerSm)
                         uint32_t w0[kKPer], w1[kKPer];
                         lds_words<kKPer>(kb, w0);
                         lds_words<kKPer>(kb + 8 * kRow, w1);
+                        // The tensor cores cut a sum off where they add to it.  With 16 of them
+                        // in a row, each on a sum that the bias makes large, that showed (1.6e-6
+                        // of the log-sum-exp of one token); so every access starts from zero there.
+                        constexpr bool kFresh = kBits == 8 && kDim == 256;
+                        float fresh[kNB][4] = {};
 #pragma unroll
                         for (int w = 0; w < kKPer; ++w) {
                             const int x = i * kKPer + w;
                             if (kBits == 8) {
-                                const uint32_t f[4] = {biased_bytes02(w0[w]), biased_bytes02(w1[w]),
-                                                       biased_bytes02(w0[w] >> 8), biased_bytes02(w1[w] >> 8)};
+                                const uint32_t f[4] = {biased_bytes(w0[w] << 2), biased_bytes(w1[w] << 2),
+                                                       biased_bytes(w0[w] >> 6), biased_bytes(w1[w] >> 6)};
 #pragma unroll
                                 for (int n = 0; n < kNB; ++n)
-                                    mma_16816(s[k][n], f, qf[n][x][0], qf[n][x][1]);
+                                    mma_16816(kFresh ? fresh[n] : s[k][n], f, qf[n][x][0], qf[n][x][1]);
                             } else {
-                                const uint32_t e[4] = {biased_nibbles04(w0[w]), biased_nibbles04(w1[w]),
-                                                       biased_nibbles15(w0[w]), biased_nibbles15(w1[w])};
-                                const uint32_t h0 = w0[w] >> 8, h1 = w1[w] >> 8;
-                                const uint32_t f[4] = {biased_nibbles04(h0), biased_nibbles04(h1), biased_nibbles15(h0),
-                                                       biased_nibbles15(h1)};
+                                const uint32_t e[4] = {biased_nibbles(w0[w] << 4), biased_nibbles(w1[w] << 4),
+                                                       biased_nibbles(w0[w]), biased_nibbles(w1[w])};
+                                const uint32_t f[4] = {biased_nibbles(w0[w] >> 4), biased_nibbles(w1[w] >> 4),
+                                                       biased_nibbles(w0[w] >> 8), biased_nibbles(w1[w] >> 8)};
 #pragma unroll
                                 for (int n = 0; n < kNB; ++n) {
                                     mma_16816(s[k][n], e, qf[n][2 * x][0], qf[n][2 * x][1]);
                                     mma_16816(s[k][n], f, qf[n][2 * x + 1][0], qf[n][2 * x + 1][1]);
                                 }
                             }
+                        }
+                        if (kFresh) {
+#pragma unroll
+                            for (int n = 0; n < kNB; ++n)
+#pragma unroll
+                                for (int c = 0; c < 4; ++c) s[k][n][c] += fresh[n][c];
                         }
                     }
                 // Scores of tokens j0 + g (0, 1) and j0 + g + 8 (2, 3) of each block,

@@ -92,6 +92,25 @@ def test_lengths_and_formats(group, D, bits, dtype):
         _check(out[:, None], lse[:, None], q, c, D ** -0.5)
 
 
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("lengths", [[1] * 8, list(range(1, 10))], ids=["one", "few"])
+def test_log_sum_exp_of_few_tokens(lengths, D, bits):
+    """Few tokens, so nothing averages out: the log-sum-exp over all rows is
+    within 1e-6 of itself.  Some ten roundings to 24 bits (the products' sum, the
+    bias taken off, the scales' logarithm and its power, the sum, its logarithm)
+    of numbers up to 8, each 8 2^-24 / sqrt(3) on average, are 0.9e-6 together,
+    beside values of root mean square 1 and more."""
+    c = Cache(lengths, 4, D, bits, 16, seed=D + bits, spread=0.0, scales=0.0)
+    q = _q(len(lengths), 1, 32, D, F16, seed=D)
+    out, lse = build("kvattention").forward(q, c.pages, c.table, c.len_tensor(), return_lse=True)
+    _check(out, lse, q, c, D ** -0.5)
+    ref = np.stack([oa.attention(q[b].double().cpu().numpy(), c.k[b], c.v[b], n, D ** -0.5, 0, 0)[1]
+                    for b, n in enumerate(lengths)])
+    off = lse.double().cpu().numpy() - ref
+    assert np.linalg.norm(off) <= 1e-6 * np.linalg.norm(ref)
+
+
 @pytest.mark.parametrize("n,window", [(2, 0), (5, 0), (1, 16), (1, 1), (4, 7), (8, 100), (3, 5000)])
 @pytest.mark.parametrize("D,bits,page", [(64, 8, 16), (128, 4, 64), (256, 8, 48)])
 def test_new_tokens_and_windows(D, bits, page, n, window):
