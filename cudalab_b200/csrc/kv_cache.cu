@@ -41,14 +41,14 @@ struct Place {
     int j;
 };
 
-__device__ __forceinline__ bool find_slot(const KvCacheArgs& a, int64_t slot, int head,
-                                          int block_bytes, Place* p) {
+__device__ __forceinline__ bool find_slot(const KvCacheArgs& a, const FastDiv& page_size,
+                                          int64_t slot, int head, int block_bytes, Place* p) {
     if (slot < 0) return false;
     int64_t page;
     int off;
     if (slot <= 0x7fffffff) {
-        page = (unsigned)slot / (unsigned)a.page_size;
-        off = (int)((unsigned)slot % (unsigned)a.page_size);
+        page = page_size.div((int)slot);
+        off = page_size.mod((int)slot);
     } else {
         page = slot / a.page_size;
         off = (int)(slot % a.page_size);
@@ -57,43 +57,69 @@ __device__ __forceinline__ bool find_slot(const KvCacheArgs& a, int64_t slot, in
         atomicCAS(&g_kv_status, 0, kStatusKvIndex);
         return false;
     }
-    const int64_t blocks = a.page_size / kKvBlock;
+    const int blocks = a.page_size / kKvBlock;
     p->block = a.pages + ((page * a.kv_heads + head) * blocks + off / kKvBlock) * block_bytes;
     p->j = off % kKvBlock;
     return true;
 }
 
-// Largest magnitude of 16 elements, NaN if one of them is.
-__device__ __forceinline__ float max16(const float (&x)[16]) {
-    float m = 0.f;
-#pragma unroll
-    for (int i = 0; i < 16; ++i)
-        asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(m), "f"(fabsf(x[i])));
-    return m;
+// Two elements' larger magnitudes, NaN where one is.
+template <bool kBf16>
+__device__ __forceinline__ uint32_t larger2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    b &= 0x7fff7fffu;
+    if (kBf16)
+        asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    else
+        asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
 }
 
-// rint(x * inv) within +-top as two's complement fields.  Adding 1.5 * 2^23
-// rounds to the nearest even integer and leaves it in the low bits, without
-// the quarter-rate conversion.
+// Largest magnitude of 16 elements, NaN if one of them is.
+template <bool kBf16>
+__device__ __forceinline__ float max16(const uint32_t (&w)[8]) {
+    uint32_t m = w[0] & 0x7fff7fffu;
+#pragma unroll
+    for (int i = 1; i < 8; ++i) m = larger2<kBf16>(m, w[i]);
+    const float2 f = unpack2<kBf16>(m);
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(f.x), "f"(f.y));
+    return r;
+}
+
+// m / kTop, correctly rounded, for m of a 16-bit type: the product with the
+// rounded reciprocal and one step on its remainder, which is exact (Markstein,
+// IBM J. Res. Dev. 34, 1990).  A general division is three times as long.
+template <int kTop>
+__device__ __forceinline__ float over_top(float m) {
+    constexpr float top = kTop, inv = 1.f / top;
+    const float q = __fmul_rn(m, inv);
+    return fmaf(fmaf(-q, top, m), inv, q);
+}
+
+// rint(x * inv) as two's complement fields, for |x * inv| < top + 1/2.  Adding
+// 1.5 * 2^23 rounds to the nearest even integer and leaves it in the low bits,
+// without the quarter-rate conversion.
 template <int kBits>
 __device__ __forceinline__ void quantise16(const float (&x)[16], float inv, uint32_t* out) {
-    constexpr float kTop = kBits == 8 ? 127.f : 7.f;
     uint32_t q[16];
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
-        q[i] = __float_as_uint(fminf(fmaxf(__fmul_rn(x[i], inv), -kTop), kTop) + 12582912.f);
+    for (int i = 0; i < 16; ++i) q[i] = __float_as_uint(__fmul_rn(x[i], inv) + 12582912.f);
     if (kBits == 8) {
 #pragma unroll
         for (int w = 0; w < 4; ++w)
             out[w] = prmt_i<0x5410u>(prmt_i<0x0040u>(q[4 * w], q[4 * w + 1]),
                                      prmt_i<0x0040u>(q[4 * w + 2], q[4 * w + 3]));
     } else {
+        // sum_i 16^i (q_i + 8), whose digits 1 to 15 do not carry; then the
+        // sign bit of every digit flipped back
+        constexpr uint32_t kMagic = 0x4b400000u, kDigits = 0x11111111u;
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
-            uint32_t r = 0;
+            uint32_t r = q[8 * w + 7];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) r |= (q[8 * w + i] & 15u) << (4 * i);
-            out[w] = r;
+            for (int i = 6; i >= 0; --i) r = 16u * r + q[8 * w + i];
+            out[w] = (r + kDigits * (8u - kMagic)) ^ 0x88888888u;
         }
     }
 }
@@ -120,8 +146,9 @@ __device__ __forceinline__ void expand16(const uint32_t (&raw)[4], float (&x)[16
 }
 
 template <int kDim, int kBits, bool kBf16, bool kVec>
-__global__ void __launch_bounds__(kThreads) kv_write_kernel(const KvCacheArgs a, const FastDiv heads) {
-    constexpr int kRow = kDim * kBits / 8, kLanes = kDim / 16;
+__global__ void __launch_bounds__(kThreads) kv_write_kernel(const KvCacheArgs a, const FastDiv heads,
+                                                            const FastDiv page_size) {
+    constexpr int kRow = kDim * kBits / 8, kLanes = kDim / 16, kTop = kBits == 8 ? 127 : 7;
     constexpr int kBlockBytes = kv_block_bytes(kRow);
     pdl_allow_dependents();
     pdl_wait_prior_grids();
@@ -131,29 +158,56 @@ __global__ void __launch_bounds__(kThreads) kv_write_kernel(const KvCacheArgs a,
     const int head = heads.mod(row);
     const bool in = token < a.tokens;
     const int64_t slot = in ? a.slots[token] : -1;
-    float x[2][16];
+    uint32_t w[2][8] = {};
     if (in) {
-        load16<kBf16, kVec>(a.k, token * a.k_token + head * a.k_head + 16 * l, x[0]);
-        load16<kBf16, kVec>(a.v, token * a.v_token + head * a.v_head + 16 * l, x[1]);
+#pragma unroll
+        for (int part = 0; part < 2; ++part) {
+            const void* from = part ? a.v : a.k;
+            const int64_t at = 16 * l + (part ? token * a.v_token + head * a.v_head
+                                              : token * a.k_token + head * a.k_head);
+            const uint4 x = load8<kBf16, kVec>(from, at), y = load8<kBf16, kVec>(from, at + 8);
+            w[part][0] = x.x, w[part][1] = x.y, w[part][2] = x.z, w[part][3] = x.w;
+            w[part][4] = y.x, w[part][5] = y.y, w[part][6] = y.z, w[part][7] = y.w;
+        }
     }
     Place p;
-    const bool put = find_slot(a, slot, head, kBlockBytes, &p);
+    const bool put = find_slot(a, page_size, slot, head, kBlockBytes, &p);
 #pragma unroll
     for (int part = 0; part < 2; ++part) {
-        float m = in ? max16(x[part]) : 0.f;
+        float m = max16<kBf16>(w[part]);
         if (!(m == m)) {  // NaN is stored as 0
 #pragma unroll
-            for (int i = 0; i < 16; ++i) x[part][i] = x[part][i] == x[part][i] ? x[part][i] : 0.f;
-            m = max16(x[part]);
+            for (int i = 0; i < 8; ++i) {
+                const float2 f = unpack2<kBf16>(w[part][i]);
+                w[part][i] &= (f.x == f.x ? 0xffffu : 0u) | (f.y == f.y ? 0xffff0000u : 0u);
+            }
+            m = max16<kBf16>(w[part]);
         }
 #pragma unroll
         for (int o = kLanes / 2; o > 0; o >>= 1)
             m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-        const float top = kBits == 8 ? 127.f : 7.f;
-        const __half s = __float2half_rn(fminf(__fdiv_rn(m, top), 65504.f));
+        // at most 65504 = 2^16 - 32 with m limited to kTop of it
+        const __half s = __float2half_rn(over_top<kTop>(fminf(m, 65504.f * kTop)));
         if (!put) continue;
+        float x[16];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float2 f = unpack2<kBf16>(w[part][i]);
+            x[2 * i] = f.x;
+            x[2 * i + 1] = f.y;
+        }
+        const uint32_t bits = __half_as_ushort(s);
+        float inv = bits ? __frcp_rn(__half2float(s)) : 0.f;
+        // A normal s is within 2^-11 of m / kTop, so |x / s| < kTop + 1/2; one
+        // that is subnormal or at its limit need not be.
+        if (bits - 1u < 0x3ffu || bits >= 0x7bffu) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                x[i] = fminf(fmaxf(__fmul_rn(x[i], inv), -(float)kTop), (float)kTop);
+            inv = 1.f;
+        }
         uint32_t q[4];
-        quantise16<kBits>(x[part], __hgt(s, __half(0.f)) ? __frcp_rn(__half2float(s)) : 0.f, q);
+        quantise16<kBits>(x, inv, q);
         uint8_t* rows = const_cast<uint8_t*>(p.block) + part * kKvBlock * kRow;
         if (kBits == 8)
             *reinterpret_cast<uint4*>(rows + kv_offset<kRow>(p.j, 16 * l)) =
@@ -167,7 +221,8 @@ __global__ void __launch_bounds__(kThreads) kv_write_kernel(const KvCacheArgs a,
 }
 
 template <int kDim, int kBits, bool kBf16, bool kVec>
-__global__ void __launch_bounds__(kThreads) kv_read_kernel(const KvCacheArgs a, const FastDiv heads) {
+__global__ void __launch_bounds__(kThreads) kv_read_kernel(const KvCacheArgs a, const FastDiv heads,
+                                                           const FastDiv page_size) {
     constexpr int kRow = kDim * kBits / 8, kLanes = kDim / 16;
     constexpr int kBlockBytes = kv_block_bytes(kRow);
     pdl_allow_dependents();
@@ -178,7 +233,7 @@ __global__ void __launch_bounds__(kThreads) kv_read_kernel(const KvCacheArgs a, 
     const int head = heads.mod(row);
     if (token >= a.tokens) return;
     Place p;
-    const bool have = find_slot(a, a.slots[token], head, kBlockBytes, &p);
+    const bool have = find_slot(a, page_size, a.slots[token], head, kBlockBytes, &p);
     uint32_t raw[2][4] = {};
     float s[2] = {0.f, 0.f};
     if (have) {
@@ -209,7 +264,7 @@ __global__ void __launch_bounds__(kThreads) kv_read_kernel(const KvCacheArgs a, 
     }
 }
 
-using Kernel = void (*)(KvCacheArgs, FastDiv);
+using Kernel = void (*)(KvCacheArgs, FastDiv, FastDiv);
 
 template <bool kWrite, int kDim, int kBits>
 Kernel pick(bool bf16, bool vec) {
@@ -239,7 +294,7 @@ cudaError_t launch(const KvCacheArgs& a, cudaStream_t stream) {
         k = a.bits == 8 ? pick<kWrite, 256, 8>(bf16, vec) : pick<kWrite, 256, 4>(bf16, vec);
     const int64_t threads = a.tokens * a.kv_heads * (a.head_dim / 16);
     return launch_pdl(k, dim3((unsigned)((threads + kThreads - 1) / kThreads)), dim3(kThreads), 0,
-                      stream, a, FastDiv((uint32_t)a.kv_heads));
+                      stream, a, FastDiv((uint32_t)a.kv_heads), FastDiv((uint32_t)a.page_size));
 }
 
 }  // namespace

@@ -76,13 +76,6 @@ __device__ __forceinline__ uint4 pack8(const float* x) {
 }
 
 template <bool kBf16, bool kVec>
-__device__ __forceinline__ void load16(const void* p, int64_t at, float (&x)[16]) {
-    const uint4 a = load8<kBf16, kVec>(p, at), b = load8<kBf16, kVec>(p, at + 8);
-    unpack8<kBf16>(a, x);
-    unpack8<kBf16>(b, x + 8);
-}
-
-template <bool kBf16, bool kVec>
 __device__ __forceinline__ void store16(void* p, int64_t at, const float (&x)[16]) {
     store8<kVec>(p, at, pack8<kBf16>(x));
     store8<kVec>(p, at + 8, pack8<kBf16>(x + 8));

@@ -76,6 +76,23 @@ def test_special_values(bits):
     assert torch.isfinite(rk).all() and torch.equal(rk, rv)
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("bits", [8, 4])
+def test_every_largest_value(bits, dtype):
+    """Every magnitude that the type has as a row's largest: the scale and all
+    fields, byte for byte."""
+    D, T = 64, 1 << 15
+    top = torch.arange(T, dtype=torch.int32).to(torch.int16).view(dtype).float()
+    x = (top[:, None] * torch.linspace(1, -1, D)[None]).to(dtype).view(T, 1, D)
+    k, v = x.cuda(), x.flip(-1).contiguous().cuda()
+    ext = build("kvcache")
+    pages = ext.empty(T // 16, 1, D, bits, 16)
+    ref = pages.cpu().numpy().copy()
+    ext.write(k, v, pages, torch.arange(T, device="cuda"))
+    oa.write(ref, 16, range(T), k.float().cpu().numpy(), v.float().cpu().numpy(), bits)
+    assert np.array_equal(pages.cpu().numpy(), ref)
+
+
 def test_strided_inputs_and_outputs():
     """k and v as slices of a fused projection, rows with an odd stride, and a
     strided destination give the contiguous call's bytes."""
