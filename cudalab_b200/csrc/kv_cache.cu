@@ -11,13 +11,14 @@
 // of the middle between two steps, where both are as near.
 //
 // Both kernels are bound by memory: the write reads 2 B and writes bits / 8 B
-// per element, the read the reverse.  A lane holds 16 elements (two 16-byte
-// loads, one 16- or 8-byte store of a chunk), head_dim / 16 lanes share a
-// row, and the same lanes take K and V so that four loads are in flight.  Reading
-// 32768 tokens of 8 heads of 128, int8: 37 us, 5.5 TB/s, 0.84 of a copy; writing
-// 8192 of them as int4 and reading them back: 21 us, 4.0 TB/s, the write (14 us)
-// bound by its instructions: 0.70 a cycle and scheduler, for 16 elements a
-// largest value, 16 products, roundings and packings.
+// per element, the read the reverse.  head_dim / 16 lanes share a row; a lane
+// holds 8 elements in each half of it, so that the lanes touch the 16-bit
+// elements in whole lines (with 16 neighbours a lane every access was one of
+// half sectors: 37 us for the 33 below), and takes K and V, so that four
+// loads are in flight.  8 heads of 128: reading 32768 tokens, int8, 33 us, 6.1
+// TB/s, 0.94 of a copy; writing 8192 tokens as int4 and reading them back 17 us, 4.9
+// TB/s, for two kernels of 6.5 us' bytes each and their ramps.  (The write's
+// instructions show as well: 16 for each element 21 us, 12 of them 20.)
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -163,9 +164,10 @@ __global__ void __launch_bounds__(kThreads) kv_write_kernel(const KvCacheArgs a,
 #pragma unroll
         for (int part = 0; part < 2; ++part) {
             const void* from = part ? a.v : a.k;
-            const int64_t at = 16 * l + (part ? token * a.v_token + head * a.v_head
-                                              : token * a.k_token + head * a.k_head);
-            const uint4 x = load8<kBf16, kVec>(from, at), y = load8<kBf16, kVec>(from, at + 8);
+            const int64_t at = 8 * l + (part ? token * a.v_token + head * a.v_head
+                                             : token * a.k_token + head * a.k_head);
+            const uint4 x = load8<kBf16, kVec>(from, at);
+            const uint4 y = load8<kBf16, kVec>(from, at + kDim / 2);
             w[part][0] = x.x, w[part][1] = x.y, w[part][2] = x.z, w[part][3] = x.w;
             w[part][4] = y.x, w[part][5] = y.y, w[part][6] = y.z, w[part][7] = y.w;
         }
@@ -209,11 +211,14 @@ __global__ void __launch_bounds__(kThreads) kv_write_kernel(const KvCacheArgs a,
         uint32_t q[4];
         quantise16<kBits>(x, inv, q);
         uint8_t* rows = const_cast<uint8_t*>(p.block) + part * kKvBlock * kRow;
-        if (kBits == 8)
-            *reinterpret_cast<uint4*>(rows + kv_offset<kRow>(p.j, 16 * l)) =
-                make_uint4(q[0], q[1], q[2], q[3]);
-        else
-            *reinterpret_cast<uint2*>(rows + kv_offset<kRow>(p.j, 8 * l)) = make_uint2(q[0], q[1]);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            uint8_t* to = rows + kv_offset<kRow>(p.j, kBits * l + i * (kRow / 2));
+            if (kBits == 8)
+                *reinterpret_cast<uint2*>(to) = make_uint2(q[2 * i], q[2 * i + 1]);
+            else
+                *reinterpret_cast<uint32_t*>(to) = q[i];
+        }
         if (l == 0)
             reinterpret_cast<__half*>(const_cast<uint8_t*>(p.block) +
                                       2 * kKvBlock * kRow)[part * kKvBlock + p.j] = s;
@@ -240,12 +245,15 @@ __global__ void __launch_bounds__(kThreads) kv_read_kernel(const KvCacheArgs a, 
 #pragma unroll
         for (int part = 0; part < 2; ++part) {
             const uint8_t* rows = p.block + part * kKvBlock * kRow;
-            if (kBits == 8) {
-                const uint4 r = *reinterpret_cast<const uint4*>(rows + kv_offset<kRow>(p.j, 16 * l));
-                raw[part][0] = r.x, raw[part][1] = r.y, raw[part][2] = r.z, raw[part][3] = r.w;
-            } else {
-                const uint2 r = *reinterpret_cast<const uint2*>(rows + kv_offset<kRow>(p.j, 8 * l));
-                raw[part][0] = r.x, raw[part][1] = r.y;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const uint8_t* from = rows + kv_offset<kRow>(p.j, kBits * l + i * (kRow / 2));
+                if (kBits == 8) {
+                    const uint2 r = *reinterpret_cast<const uint2*>(from);
+                    raw[part][2 * i] = r.x, raw[part][2 * i + 1] = r.y;
+                } else {
+                    raw[part][i] = *reinterpret_cast<const uint32_t*>(from);
+                }
             }
             s[part] = __half2float(reinterpret_cast<const __half*>(
                 p.block + 2 * kKvBlock * kRow)[part * kKvBlock + p.j]);
@@ -260,7 +268,8 @@ __global__ void __launch_bounds__(kThreads) kv_read_kernel(const KvCacheArgs a, 
         void* y = part ? a.v : a.k;
         const int64_t at = part ? token * a.v_token + head * a.v_head
                                 : token * a.k_token + head * a.k_head;
-        store16<kBf16, kVec>(y, at + 16 * l, x);
+        store8<kVec>(y, at + 8 * l, pack8<kBf16>(x));
+        store8<kVec>(y, at + 8 * l + kDim / 2, pack8<kBf16>(x + 8));
     }
 }
 

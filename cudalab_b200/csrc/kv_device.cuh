@@ -75,12 +75,6 @@ __device__ __forceinline__ uint4 pack8(const float* x) {
                       pack2<kBf16>(x[4], x[5]), pack2<kBf16>(x[6], x[7]));
 }
 
-template <bool kBf16, bool kVec>
-__device__ __forceinline__ void store16(void* p, int64_t at, const float (&x)[16]) {
-    store8<kVec>(p, at, pack8<kBf16>(x));
-    store8<kVec>(p, at + 8, pack8<kBf16>(x + 8));
-}
-
 // n / d for 0 <= n < 2^31 by a multiplication, d fixed at launch.
 struct FastDiv {
     uint32_t d, mul, shift;
