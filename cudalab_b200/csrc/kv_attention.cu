@@ -39,10 +39,10 @@
 // Measured (8 heads of 128): 64 sequences of 4096 to 8192 tokens, 64 query
 // heads, int4 97 us = 4.3 TB/s, 0.65 of a copy; 16 ragged sequences to 4096,
 // int8 21 us, of which the bytes are 10.5; one sequence of 77 tokens 4.8 us.  The
-// long case is neither DRAM- nor issue-bound (0.56 instructions a cycle and
-// scheduler with the three warps that 158 registers allow): the latencies along
-// a block's chain K -> S -> weights -> O are what is left, and more warps of
-// fewer registers spill.  The short ones are the launch and a cold start.
+// long case is held by the logic instructions that expand the fields, which
+// come in bursts to one pipe: its copies alone take 70 us, all but V's
+// expansion 89, while HADD2, MMAs and shared-memory reads cost nothing beside
+// them.  The short ones are launch, plan, first bytes and join in a row.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
