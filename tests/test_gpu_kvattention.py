@@ -347,3 +347,30 @@ def test_empty_batch():
     q = torch.empty(0, 2, 64, dtype=F16, device="cuda")
     out = build("kvattention").forward(q, c.pages, c.table[:0], c.len_tensor()[:0])
     assert out.shape == (0, 2, 64)
+
+
+def test_cache_beyond_32_bits():
+    """A cache of more than 4 GiB gives its far pages' tokens the bits that the
+    same pages give in a small one: written, read, attended to, and shared."""
+    H, D, page = 8, 128, 64
+    c = Cache([700, 130], H, D, 8, page, seed=61)
+    first = 40000 - c.pages.shape[0]
+    far = c.ext.empty(40000, H, D, 8, page)
+    assert first * far[0].numel() > 1 << 32
+    slots = (c.table[0].long()[:, None] * page + torch.arange(page, device="cuda")).flatten()[:700]
+    k, v = c.ext.read(c.pages, slots, D)
+    c.ext.write(k, v, far, slots + first * page)
+    for x, y in zip(c.ext.read(far, slots + first * page, D), c.ext.read(c.pages, slots, D)):
+        assert torch.equal(x, y)
+    far[first:] = c.pages
+    q = _q(2, 1, 64, D, F16, seed=62)
+    att = build("kvattention")
+    args = (c.len_tensor(),)
+    assert torch.equal(att.forward(q, far, c.table + first, *args),
+                       att.forward(q, c.pages, c.table, *args))
+    q = _q(8, 1, 64, D, F16, seed=63)  # 64 rows a head: the tensor-core prefix kernel
+    lens = torch.tensor([0, 1, 17, 64, 100, 3, 5, 64], dtype=torch.int32, device="cuda")
+    table = c.table[1:].expand(8, -1).contiguous()
+    assert torch.equal(att.forward_shared(q, far, c.table[0] + first, 700, table + first, lens),
+                       att.forward_shared(q, c.pages, c.table[0], 700, table, lens))
+    assert nat.device_status(clear=True) == 0
