@@ -146,9 +146,11 @@ __device__ __forceinline__ void expand16(const uint32_t (&raw)[4], float (&x)[16
     }
 }
 
+// 12 CTAs an SM, 40 registers (17.2 us for the 8192 tokens above, by 10 17.7, by
+// 16 18.3).
 template <int kDim, int kBits, bool kBf16, bool kVec>
-__global__ void __launch_bounds__(kThreads) kv_write_kernel(const KvCacheArgs a, const FastDiv heads,
-                                                            const FastDiv page_size) {
+__global__ void __launch_bounds__(kThreads, 12)
+    kv_write_kernel(const KvCacheArgs a, const FastDiv heads, const FastDiv page_size) {
     constexpr int kRow = kDim * kBits / 8, kLanes = kDim / 16, kTop = kBits == 8 ? 127 : 7;
     constexpr int kBlockBytes = kv_block_bytes(kRow);
     pdl_allow_dependents();
