@@ -389,16 +389,16 @@ __global__ void __launch_bounds__(kThreads, Shape<kDim, kBits, kNB>::kPerSm)
         if (first && a.lse != nullptr) a.lse[row] = lse2 * 0.6931471805599453f;
     };
 
-    // Sequences with nothing to read (their rows see no cached token).
-    auto write_empty = [&](int b, int part0, int part1) {
+    // A row tile with nothing to read (its rows see no cached token).
+    auto write_empty = [&](int b, int part) {
         settle();
-        const int n = rows * (kDim / 4);
-        for (int h = part0; h < part1; ++h)
-            for (int i = tid; i < n; i += kThreads) {
-                const int d = i % (kDim / 4) * 4;
-                write_out(out_row(b, h, i / (kDim / 4)), d, make_float4(0.f, 0.f, 0.f, 0.f),
-                          -INFINITY, 0.f, d == 0);
-            }
+        const int h = p.row_tiles.div(part), r0 = p.row_tiles.mod(part) * S::kCols;
+        const int n = min(S::kCols, rows - r0) * (kDim / 4);
+        for (int i = tid; i < n; i += kThreads) {
+            const int d = i % (kDim / 4) * 4;
+            write_out(out_row(b, h, r0 + i / (kDim / 4)), d, make_float4(0.f, 0.f, 0.f, 0.f),
+                      -INFINITY, 0.f, d == 0);
+        }
     };
 
     // The CTA's range [u0, u1) and its first segment.  Chunked, the line is the
@@ -418,14 +418,13 @@ __global__ void __launch_bounds__(kThreads, Shape<kDim, kBits, kNB>::kPerSm)
         u1 = min(u0 + p.min_units, start.units);
         parts = p.min_chunk.div(start.units + p.min_units - 1);
         if (u0 >= u1) {
-            if (start.units == 0 && u0 == 0 && p.row_tiles.mod(start.part) == 0)
-                write_empty(start.seq, p.row_tiles.div(start.part), p.row_tiles.div(start.part) + 1);
+            if (start.units == 0 && u0 == 0) write_empty(start.seq, start.part);
             return;
         }
     } else {
-        for (int i = blockIdx.x; i < a.batch * a.kv_heads; i += grid) {
-            const int b = i / a.kv_heads, h = i - b * a.kv_heads;
-            if (s_cum[b + 1] == s_cum[b]) write_empty(b, h, h + 1);
+        for (int i = blockIdx.x; i < a.batch * heads_tiles; i += grid) {
+            const int b = i / heads_tiles;
+            if (s_cum[b + 1] == s_cum[b]) write_empty(b, i - b * heads_tiles);
         }
         // last sequence whose cells (`sums`) begin at or before x, by the whole warp
         auto find = [&](const int* sums, int x) {
