@@ -840,7 +840,8 @@ int cl_kvattention(const void* q, const uint8_t* pages, const int32_t* page_tabl
     a.page_size = d->page_size;
     a.type = type16(d->dtype);
     a.causal = 1;
-    a.window = d->window;
+    // a window that holds every length the page table allows is none
+    a.window = d->window < (int64_t)d->max_pages * d->page_size ? d->window : 0;
     a.scale = d->scale;
     a.out = out;
     a.lse = lse;

@@ -258,9 +258,9 @@ __global__ void __launch_bounds__(kThreads, Shape<kDim, kBits, kNB>::kPerSm)
     // Units of each sequence (a window drops the blocks in front of the first
     // token that any row sees), and how the line of all segments is cut.
     auto first_block = [&](int len) {
-        if (a.window <= 0) return 0;
-        const int first = len - a.new_tokens + 1 - a.window;
-        return first > 0 ? first / kKvBlock : 0;
+        // len - new + 1 - window, of which no step passes 32 bits
+        const int behind = len - a.window;
+        return a.window > 0 && behind >= a.new_tokens ? (behind - a.new_tokens + 1) / kKvBlock : 0;
     };
     auto units_of = [&](int len) {
         return ((len + kKvBlock - 1) / kKvBlock - first_block(len) + kU - 1) / kU;
@@ -754,7 +754,8 @@ __global__ void __launch_bounds__(kThreads, Shape<kDim, kBits, kNB>::kPerSm)
                             const int r = row0 + 8 * n + 2 * t + c;
                             const int end = len - a.new_tokens + p.group.div(r) + 1;
                             const int hi = a.causal ? min(end, len) : len;
-                            const int lo = a.window > 0 ? end - a.window : 0;
+                            // (a row in front of the sequence sees nothing, by hi)
+                            const int lo = a.window > 0 ? max(end, 0) - a.window : 0;
 #pragma unroll
                             for (int k = 0; k < kU; ++k)
 #pragma unroll

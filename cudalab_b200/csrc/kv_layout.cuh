@@ -95,7 +95,7 @@ struct KvAttentionArgs {
     int fixed_length;        // >= 0: the length of every sequence (lengths unused)
     int batch, new_tokens, kv_heads, group, head_dim, bits, page_size, type;
     int causal;  // row i of a sequence sees tokens up to length - new + i
-    int window;  // > 0: the last `window` of those
+    int window;  // > 0: the last `window` of those; below max_pages * page_size
     float scale;
     void* out;        // [batch, new, heads, head_dim] contiguous (type), or null
     float* out_f32;   // the same in fp32 instead (partial results), or null

@@ -355,7 +355,7 @@ int cl_kvcache_read(const uint8_t* pages, const int64_t* slots, void* k, void* v
  * tokens of each sequence: page_table int32 [batch, max_pages] (row stride
  * table_stride), lengths int32 [batch], the new tokens included.  Row i of a
  * sequence sees its tokens up to length - new_tokens + i (with window > 0 the
- * last `window` of them); q_heads is a multiple of kv_heads, head h reads
+ * last `window` of them; any up to 2^31 - 1); q_heads is a multiple of kv_heads, head h reads
  * cache head h / (q_heads / kv_heads).  out [batch, new_tokens, q_heads,
  * head_dim] contiguous; lse fp32 [batch, new_tokens, q_heads] (natural log of
  * the softmax's denominator) or null.  A row that sees nothing gives zeros

@@ -1,0 +1,43 @@
+"""Attention over the quantised cache where it is easily wrong.  Oracle and
+tolerances as in test_gpu_kvattention.py."""
+import pytest
+import torch
+
+from cudalab_b200.build import build
+from test_gpu_kvattention import F16, Cache, _check, _q
+
+pytestmark = pytest.mark.gpu
+
+
+# An empty sequence in front of several new tokens, so that length - new tokens - window
+# passes 32 bits where it is taken as it stands; few sequences have CTAs of their own,
+# 300 are planned as one line.
+@pytest.mark.parametrize("copies", [1, 60])
+@pytest.mark.parametrize("D,bits,page", [(64, 8, 16), (128, 4, 64), (256, 8, 32)])
+def test_window_without_an_end(D, bits, page, copies):
+    lengths = [0, 1, 50, 3, 200] * copies
+    c = Cache(lengths, 2, D, bits, page, seed=81)
+    q = _q(len(lengths), 5, 6, D, F16, seed=82)
+    att = build("kvattention")
+    most = c.table.shape[1] * page
+    args = (q, c.pages, c.table, c.len_tensor())
+    out, lse = att.forward(*args, return_lse=True)
+    _check(out, lse, q, c, D ** -0.5)
+    for window in (most - 1, most, most + 4, most + 5, 2 ** 31 - 20, 2 ** 31 - 1):
+        o, z = att.forward(*args, window=window, return_lse=True)
+        if window >= 200:
+            assert torch.equal(o, out) and torch.equal(z, lse), window
+        _check(o, z, q, c, D ** -0.5, window)
+
+
+def test_window_below_the_longest_page_table():
+    """A page table of 2^31 - 16 tokens, in which a window of nearly as many counts."""
+    D, page, new = 64, 16, 40
+    c = Cache([50, 0, 7], 1, D, 8, page, seed=83)
+    q = _q(3, new, 1, D, F16, seed=84)
+    table = torch.zeros(3, (1 << 27) - 1, dtype=torch.int32, device="cuda")
+    table[:, :c.table.shape[1]] = c.table
+    att = build("kvattention")
+    for window in (2 ** 31 - 17, 2 ** 31 - 1):
+        out, lse = att.forward(q, c.pages, table, c.len_tensor(), window=window, return_lse=True)
+        _check(out, lse, q, c, D ** -0.5, window)
