@@ -46,8 +46,23 @@ def _fields(names: str, ctype) -> list:
     return [(n, ctype) for n in names.split()]
 
 
-class QkNormRopeDesc(ctypes.Structure):
+class _Desc(ctypes.Structure):
+    """A descriptor of the C ABI: `_wide` 64-bit fields, then `_narrow` 32-bit ones.  ctypes
+    keeps the low bits of an integer that its field does not hold; here such a value is
+    refused."""
+
+    def __init__(self, *values, **named):
+        narrow = values[self._wide:self._wide + self._narrow]
+        if narrow and max(narrow) >= 1 << 31:
+            i = next(i for i, v in enumerate(narrow) if v >= 1 << 31)
+            raise RuntimeError(f"{self._fields_[self._wide + i][0]} must be below 2^31, "
+                               f"got {narrow[i]}")
+        super().__init__(*values, **named)
+
+
+class QkNormRopeDesc(_Desc):
     """cl_qknorm_rope_desc"""
+    _wide, _narrow = 10, 7
     _fields_ = (_fields("tokens table_rows q_token q_head k_token k_head q_out_token q_out_head "
                         "k_out_token k_out_head", _i64)
                 + _fields("q_heads kv_heads head_dim rotary interleaved positions64 dtype",
@@ -55,14 +70,16 @@ class QkNormRopeDesc(ctypes.Structure):
                 + [("eps", ctypes.c_float)])
 
 
-class KvCacheDesc(ctypes.Structure):
+class KvCacheDesc(_Desc):
     """cl_kvcache_desc"""
+    _wide, _narrow = 6, 5
     _fields_ = (_fields("tokens num_pages k_token k_head v_token v_head", _i64)
                 + _fields("kv_heads head_dim bits page_size dtype", ctypes.c_int32))
 
 
-class KvAttentionDesc(ctypes.Structure):
+class KvAttentionDesc(_Desc):
     """cl_kvattention_desc"""
+    _wide, _narrow = 5, 12
     _fields_ = (_fields("num_pages table_stride q_batch q_new q_head", _i64)
                 + _fields("batch new_tokens q_heads kv_heads head_dim bits page_size max_pages "
                           "window dtype prefix_length prefix_page_count", ctypes.c_int32)

@@ -1,0 +1,28 @@
+"""What the attention operators refuse besides the cases of test_attention_cpu.py,
+without a GPU."""
+import ctypes
+
+import pytest
+
+from cudalab_b200 import _native as nat
+
+
+def _rej(fn, text):
+    with pytest.raises(RuntimeError) as e:
+        fn()
+    assert text in str(e.value), str(e.value)
+
+
+def test_descriptor_refuses_what_its_fields_do_not_hold():
+    """2^32 + 5 in a 32-bit field is an error, not 5."""
+    for cls in (nat.QkNormRopeDesc, nat.KvCacheDesc, nat.KvAttentionDesc):
+        for i, (name, ctype) in enumerate(cls._fields_):
+            values = [1] * len(cls._fields_)
+            for big in (1 << 31, (1 << 32) + 5):
+                values[i] = big
+                if ctype is ctypes.c_int32:
+                    _rej(lambda: cls(*values), f"{name} must be below 2^31, got {big}")
+                else:
+                    assert getattr(cls(*values), name) == big or ctype is ctypes.c_float
+            values[i] = (1 << 31) - 1
+            assert int(getattr(cls(*values), name)) in ((1 << 31) - 1, 1 << 31)

@@ -41,3 +41,14 @@ def test_window_below_the_longest_page_table():
     for window in (2 ** 31 - 17, 2 ** 31 - 1):
         out, lse = att.forward(q, c.pages, table, c.len_tensor(), window=window, return_lse=True)
         _check(out, lse, q, c, D ** -0.5, window)
+
+
+@pytest.mark.parametrize("workspace", [True, False])
+def test_window_past_32_bits_is_refused(workspace):
+    """Not cut to its low bits (5 tokens here)."""
+    att = build("kvattention")
+    c = Cache([20, 5], 1, 64, 8, 16, seed=85)
+    ws = att.workspace() if workspace else None
+    with pytest.raises(RuntimeError, match="window must be below"):
+        att.forward(_q(2, 1, 4, 64, F16, seed=86)[:, 0], c.pages, c.table, c.len_tensor(),
+                    window=(1 << 32) + 5, workspace=ws)
