@@ -499,11 +499,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prefix_kernel(const PrefixPara
                     for (int j = 0; j < 16; j += 4) {
                         const float4 ks = *reinterpret_cast<const float4*>(num + 16 * c + j);
                         const float4 vs = *reinterpret_cast<const float4*>(num + kTile + 16 * c + j);
-                        // a zero scale has all-zero values: any log will do
-                        const float x = logit(s[j], ks.x, fmaxf(lg2(vs.x), -24.f));
-                        const float y = logit(s[j + 1], ks.y, fmaxf(lg2(vs.y), -24.f));
-                        const float z = logit(s[j + 2], ks.z, fmaxf(lg2(vs.z), -24.f));
-                        const float w = logit(s[j + 3], ks.w, fmaxf(lg2(vs.w), -24.f));
+                        const float x = logit(s[j], ks.x, lg2(vs.x));
+                        const float y = logit(s[j + 1], ks.y, lg2(vs.y));
+                        const float z = logit(s[j + 2], ks.z, lg2(vs.z));
+                        const float w = logit(s[j + 3], ks.w, lg2(vs.w));
                         top = fmaxf(fmaxf(fmaxf(top, x), y), fmaxf(z, w));
                     }
                 }
@@ -612,8 +611,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prefix_kernel(const PrefixPara
             const bool seen = at != 0xffffffffu &&
                               (tile0 + i) * kTile + kKvBlock * w + (lane & 15) < length;
             const float s = seen ? __half2float(scale) : 0.f;
+            // A zero scale has all-zero values, so any other does as well: with fp16's
+            // smallest, a weight shows when the token's score passes the reference.
             numbers[(i & 3) * 2 * kTile + (lane >> 4) * kTile + kKvBlock * w + (lane & 15)] =
-                lane < 16 ? (seen ? s * log2_scale : 1.f) : s;
+                lane < 16 ? (seen ? s * log2_scale : 1.f) : (seen ? fmaxf(s, 0x1p-24f) : 0.f);
             store(0, kbuf + b * S::kOperandBytes);
             arrive(kfull + 8 * b);
             if (lane == 0) mbar_arrive(nfull + 8 * (i & 3));

@@ -1,12 +1,37 @@
 """Attention over the quantised cache where it is easily wrong.  Oracle and
 tolerances as in test_gpu_kvattention.py."""
+import numpy as np
 import pytest
 import torch
 
 from cudalab_b200.build import build
+from oracle import attention_oracle as oa
 from test_gpu_kvattention import F16, Cache, _check, _q
 
 pytestmark = pytest.mark.gpu
+
+
+def _set(c, k, v, bits):
+    """Writes k, v [tokens, H, D] over a one-sequence cache's tokens."""
+    j = torch.arange(len(k))
+    slots = c.table[0].cpu().long()[j // c.page] * c.page + j % c.page
+    k, v = k.half(), v.half()
+    c.ext.write(k.cuda(), v.cuda(), c.pages, slots.cuda())
+    for at, x in ((c.k, k), (c.v, v)):
+        q, s = oa.quantise(x.float().numpy(), bits)
+        at[0] = q.astype(np.float64) * s.astype(np.float64)[..., None]
+
+
+def _over_prefix(p, q, scale, own=0, bits=8, prefix_pages=None, ref=None):
+    """q [B, 1, Hq, D] over p's tokens as the shared prefix of B sequences of `own` tokens."""
+    B, D = q.shape[0], q.shape[-1]
+    c = Cache([own] * B, p.H, D, bits, p.page, seed=B)
+    pages = torch.cat((c.pages, p.pages))
+    table = p.table[0] if prefix_pages is None else prefix_pages
+    table = torch.where(table < len(p.pages), table + len(c.pages), table).int()
+    out, lse = build("kvattention").forward_shared(q, pages, table, p.lengths[0], c.table,
+                                                   c.len_tensor(), scale=scale, return_lse=True)
+    return out, lse, c
 
 
 # An empty sequence in front of several new tokens, so that length - new tokens - window
@@ -52,3 +77,23 @@ def test_window_past_32_bits_is_refused(workspace):
     with pytest.raises(RuntimeError, match="window must be below"):
         att.forward(_q(2, 1, 4, 64, F16, seed=86)[:, 0], c.pages, c.table, c.len_tensor(),
                     window=(1 << 32) + 5, workspace=ws)
+
+
+# one row a head: the register-fed kernel; 132: the tensor-core prefix kernel
+@pytest.mark.parametrize("batch", [1, 33])
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("above", [20.0, 100.0, 127.6, 200.0])
+def test_token_without_values_outweighs_all(above, bits, batch):
+    """Tokens of zero V whose base-2 logits lie far above all others', in the second or
+    third tile of a part (40 tiles of 128 tokens make parts of three)."""
+    n, D = 5000, 128
+    g = torch.Generator().manual_seed(71)
+    p = Cache([n], 1, D, bits, 64, seed=72)
+    d = torch.sign(torch.randn(D, generator=g))
+    k, v = 0.02 * torch.randn(n, 1, D, generator=g), torch.randn(n, 1, D, generator=g)
+    for at in (700, 1408):
+        k[at:at + 4, 0], v[at:at + 4] = d * (above * np.log(2) / D), 0
+    _set(p, k, v, bits)
+    q = d.expand(batch, 1, 4, D).half().cuda()
+    out, lse, c = _over_prefix(p, q, 1.0, 1, bits)
+    _check(out, lse, q, c, 1.0, prefix=p)
