@@ -272,6 +272,8 @@ class KvAttentionExt(_Ext):
              f"workspace must have {self.workspace_bytes} bytes, 16-byte aligned")
         n_prefix = 0
         if prefix_length:
+            _chk(prefix_pages is not None, f"prefix_length is {prefix_length}: prefix_pages must "
+                                           "be given")
             _plain("prefix_pages", prefix_pages, 1, (torch.int32,), dev)
             n_prefix = prefix_pages.size(0)
             _chk(0 <= prefix_length <= n_prefix * page_size,

@@ -270,8 +270,8 @@ py::object kvattention(const at::Tensor& q, const at::Tensor& pages, const at::T
         return n;
     }();
     if (static_cast<size_t>(workspace.numel()) < need) return py::none();
-    const bool shared = prefix.has_value() && prefix_length > 0;
-    if (shared && (!plain_ok(*prefix, 1, at::kInt, d) || window != 0 ||
+    const bool shared = prefix_length > 0;
+    if (shared && (!prefix.has_value() || !plain_ok(*prefix, 1, at::kInt, d) || window != 0 ||
                    prefix_length > prefix->size(0) * desc.page_size || prefix_length > INT32_MAX))
         return py::none();
     desc.num_pages = pages.size(0);

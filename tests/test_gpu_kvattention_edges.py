@@ -97,3 +97,13 @@ def test_token_without_values_outweighs_all(above, bits, batch):
     q = d.expand(batch, 1, 4, D).half().cuda()
     out, lse, c = _over_prefix(p, q, 1.0, 1, bits)
     _check(out, lse, q, c, 1.0, prefix=p)
+
+
+@pytest.mark.parametrize("workspace", [True, False])
+def test_prefix_without_pages_is_refused(workspace):
+    att = build("kvattention")
+    c = Cache([20, 5], 1, 64, 8, 16, seed=77)
+    ws = att.workspace() if workspace else None
+    with pytest.raises(RuntimeError, match="prefix_pages"):
+        att.forward_shared(_q(2, 1, 4, 64, F16, seed=78), c.pages, None, 16, c.table,
+                           c.len_tensor(), workspace=ws)
