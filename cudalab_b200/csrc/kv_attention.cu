@@ -100,29 +100,12 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
     return r;
 }
 
-// K's fields as halves without a conversion: the field with its sign bit
-// flipped, u = k + bias (bias 128 or 8), placed in the mantissa of a half whose
-// exponent is zero is the subnormal u 2^-22 (int8, bits 2 to 9) or u 2^-20
-// (int4, bits 4 to 7), exactly, and the tensor cores take subnormals as they
-// are.  What the bias adds to a score, bias sum_d q_d, is taken off in fp32 with
-// the scales.  The place matters: the tensor cores line products up by their
-// operands' exponents and drop what falls below, so a field in the lowest bits
-// loses as many bits of the sum as there are zeros above it.  One place for all
-// fields costs one more shift a word of int8, two of int4, than the lowest bits
-// (the log-sum-exp of some ten tokens of int4 was 1.8e-6 of itself off there).
-//
-// Bytes 0 and 2 of w << 2 or, of w >> 6, bytes 1 and 3 of w.
-__device__ __forceinline__ uint32_t biased_bytes(uint32_t w) {
-    return lop3_sel_xor_i<0x03FC03FCu, 0x02000200u>(w);
-}
-// Nibbles 1 and 5 of w; of w << 4, w >> 4, w >> 8: 0 and 4, 2 and 6, 3 and 7.
-__device__ __forceinline__ uint32_t biased_nibbles(uint32_t w) {
-    return lop3_sel_xor_i<0x00F000F0u, 0x00800080u>(w);
-}
-
-// V's fields as themselves: under an exponent of 1024 or 64, less that and the
-// flip of the sign bit.  (Without the subtraction the sum over the tokens would
-// carry the bias times the softmax's denominator, beside which O is small.)
+// Fields as exact halves: under an exponent of 1024 or 64, less that and the flip
+// of the sign bit.  The subtraction belongs before the products.  A score or an
+// output taken with the bias on (128 or 8) and rid of bias times sum(q), or times the
+// softmax's denominator, afterwards is a small difference of large sums: with a
+// strong channel in K and a q that does not average to zero a logit was off by
+// 3e-4, and it saved no time (the additions run beside the logic instructions).
 __device__ __forceinline__ uint32_t h2_add(uint32_t v, unsigned short bias) {
     const __half2 r = __hadd2(u32_as_h2(v), h2_const(bias));
     return *reinterpret_cast<const uint32_t*>(&r);
@@ -598,12 +581,12 @@ __global__ void __launch_bounds__(kThreads, Shape<kDim, kBits, kNB>::kPerSm)
 
         // q as B fragments.  Rows are brought to [1, 2) by a power of two (exact;
         // elements 2^14 below their row's largest lose bits that fp32 sums would
-        // not keep either).  rs brings a score to base-2 logits, qc is what the bias adds to it.
+        // not keep either).  rs brings a score to base-2 logits.
         uint32_t qf[kNB][kSteps][2];
-        float rs[kNB][2], qc[kNB][2];
+        float rs[kNB][2];
 #pragma unroll
         for (int n = 0; n < kNB; ++n) {
-            float x[kDim / 4], top = 0.f, sum = 0.f;
+            float x[kDim / 4], top = 0.f;
 #pragma unroll
             for (int i = 0; i < kDim / 32; ++i) unpack8<kBf16>(qraw[n][i], x + 8 * i);
 #pragma unroll
@@ -619,21 +602,8 @@ __global__ void __launch_bounds__(kThreads, Shape<kDim, kBits, kNB>::kPerSm)
                 for (int i = 0; i < kDim / 4; ++i) x[i] *= down;
                 unit *= __uint_as_float((uint32_t)(127 + e) << 23);
             }
-            // the sum of the elements as the tensor cores get them
 #pragma unroll
-            for (int i = 0; i < kDim / 4; i += 2) {
-                const float2 h = __half22float2(__floats2half2_rn(x[i], x[i + 1]));
-                sum += h.x + h.y;
-            }
-            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-            sum *= (kBits == 8 ? 128.f : 8.f) * unit;
-            unit *= kBits == 8 ? 4194304.f : 1048576.f;  // 2^22, 2^20
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                rs[n][c] = __shfl_sync(0xffffffffu, unit, 8 * t + 4 * c);
-                qc[n][c] = __shfl_sync(0xffffffffu, sum, 8 * t + 4 * c);
-            }
+            for (int c = 0; c < 2; ++c) rs[n][c] = __shfl_sync(0xffffffffu, unit, 8 * t + 4 * c);
 #pragma unroll
             for (int w = 0; w < kKWords; ++w) {
                 if (kBits == 8) {
@@ -689,37 +659,27 @@ __global__ void __launch_bounds__(kThreads, Shape<kDim, kBits, kNB>::kPerSm)
                         uint32_t w0[kKPer], w1[kKPer];
                         lds_words<kKPer>(kb, w0);
                         lds_words<kKPer>(kb + 8 * kRow, w1);
-                        // The tensor cores cut a sum off where they add to it.  With 16 of them
-                        // in a row, each on a sum that the bias makes large, that showed (1.6e-6
-                        // of the log-sum-exp of one token); so every access starts from zero there.
-                        constexpr bool kFresh = kBits == 8 && kDim == 256;
-                        float fresh[kNB][4] = {};
 #pragma unroll
                         for (int w = 0; w < kKPer; ++w) {
                             const int x = i * kKPer + w;
+                            const uint32_t u0 = w0[w] >> 8, u1 = w1[w] >> 8;
                             if (kBits == 8) {
-                                const uint32_t f[4] = {biased_bytes(w0[w] << 2), biased_bytes(w1[w] << 2),
-                                                       biased_bytes(w0[w] >> 6), biased_bytes(w1[w] >> 6)};
+                                const uint32_t f[4] = {bytes02(w0[w]), bytes02(w1[w]), bytes02(u0),
+                                                       bytes02(u1)};
 #pragma unroll
                                 for (int n = 0; n < kNB; ++n)
-                                    mma_16816(kFresh ? fresh[n] : s[k][n], f, qf[n][x][0], qf[n][x][1]);
+                                    mma_16816(s[k][n], f, qf[n][x][0], qf[n][x][1]);
                             } else {
-                                const uint32_t e[4] = {biased_nibbles(w0[w] << 4), biased_nibbles(w1[w] << 4),
-                                                       biased_nibbles(w0[w]), biased_nibbles(w1[w])};
-                                const uint32_t f[4] = {biased_nibbles(w0[w] >> 4), biased_nibbles(w1[w] >> 4),
-                                                       biased_nibbles(w0[w] >> 8), biased_nibbles(w1[w] >> 8)};
+                                const uint32_t e[4] = {nibbles04(w0[w]), nibbles04(w1[w]),
+                                                       nibbles15(w0[w]), nibbles15(w1[w])};
+                                const uint32_t f[4] = {nibbles04(u0), nibbles04(u1), nibbles15(u0),
+                                                       nibbles15(u1)};
 #pragma unroll
                                 for (int n = 0; n < kNB; ++n) {
                                     mma_16816(s[k][n], e, qf[n][2 * x][0], qf[n][2 * x][1]);
                                     mma_16816(s[k][n], f, qf[n][2 * x + 1][0], qf[n][2 * x + 1][1]);
                                 }
                             }
-                        }
-                        if (kFresh) {
-#pragma unroll
-                            for (int n = 0; n < kNB; ++n)
-#pragma unroll
-                                for (int c = 0; c < 4; ++c) s[k][n][c] += fresh[n][c];
                         }
                     }
                 // Scores of tokens j0 + g (0, 1) and j0 + g + 8 (2, 3) of each block,
@@ -738,8 +698,7 @@ __global__ void __launch_bounds__(kThreads, Shape<kDim, kBits, kNB>::kPerSm)
                         for (int n = 0; n < kNB; ++n)
 #pragma unroll
                             for (int c = 0; c < 2; ++c)
-                                s[k][n][2 * h + c] = fmaf(s[k][n][2 * h + c], ks * rs[n][c],
-                                                          fmaf(-ks, qc[n][c], lv));
+                                s[k][n][2 * h + c] = fmaf(s[k][n][2 * h + c], ks * rs[n][c], lv);
                     }
                 }
                 const int j0 = cu * (kU * kKvBlock) + token0;

@@ -6,7 +6,7 @@ import torch
 
 from cudalab_b200.build import build
 from oracle import attention_oracle as oa
-from test_gpu_kvattention import F16, Cache, _check, _q
+from test_gpu_kvattention import BF16, F16, Cache, _check, _q
 
 pytestmark = pytest.mark.gpu
 
@@ -107,3 +107,31 @@ def test_prefix_without_pages_is_refused(workspace):
     with pytest.raises(RuntimeError, match="prefix_pages"):
         att.forward_shared(_q(2, 1, 4, 64, F16, seed=78), c.pages, None, 16, c.table,
                            c.len_tensor(), workspace=ws)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=str)
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("mean,strong", [(0.0, 30.0), (1.0, 30.0), (4.0, 1.0)])
+def test_strong_channel_and_queries_with_a_mean(mean, strong, D, bits, dtype):
+    """A K channel that sets its token's scale, and rows of q whose elements do not
+    average to zero: a score keeps its bits whatever the fields' own sum is."""
+    lengths = [1, 40, 300, 517]
+    c = Cache(lengths, 2, D, bits, 32, seed=D + bits, spread=0.0)
+    g = torch.Generator().manual_seed(73)
+    for b, n in enumerate(lengths):
+        k, v = torch.randn(2, n, 2, D, generator=g)
+        k[..., 5] *= strong
+        j = torch.arange(n)
+        slots = c.table[b].cpu().long()[j // 32] * 32 + j % 32
+        c.ext.write(k.half().cuda(), v.half().cuda(), c.pages, slots.cuda())
+        for at, x in ((c.k, k), (c.v, v)):
+            qx, s = oa.quantise(x.half().float().numpy(), bits)
+            at[b] = qx.astype(np.float64) * s.astype(np.float64)[..., None]
+    for heads in (2, 8, 24):  # 1, 4 and 12 rows a head
+        q = (_q(4, 1, heads, D, F16, seed=heads).float() + mean)
+        q[..., 5] *= 0.1
+        q = q.to(dtype)
+        out, lse = build("kvattention").forward(q, c.pages, c.table, c.len_tensor(),
+                                                return_lse=True)
+        _check(out, lse, q, c, D ** -0.5)
