@@ -220,7 +220,9 @@ struct PrefixShape {
     static constexpr int kNumbers = 4 * kOperandBytes;
     static constexpr int kTops = kNumbers + 4 * 2 * kTile * 4;  // [2][kRows] exchanged by row halves
     static constexpr int kBars = kTops + 2 * kRows * 4;
-    static constexpr int kSmem = (kBars + 128 < 120 * 1024 ? 120 * 1024 : kBars + 128) + 1024;
+    static constexpr int kGone = kBars + 128;  // [4][kFillWarps] bytes: the block is missing
+    static constexpr int kEnd = kGone + 4 * kFillWarps;
+    static constexpr int kSmem = (kEnd < 120 * 1024 ? 120 * 1024 : kEnd) + 1024;
     static_assert(kRows * kOutStride <= 4 * kOperandBytes, "room for the output");
 };
 
@@ -283,6 +285,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prefix_kernel(const PrefixPara
     const uint32_t bars = smem_u32(smem + S::kBars);
     const uint32_t kfull = bars, vfull = bars + 16, kempty = bars + 32, vempty = bars + 48,
                    sfull = bars + 64, pfull = bars + 80, nfull = bars + 88;
+    uint8_t* gone = smem + S::kGone;
     volatile uint32_t* s_tmem = reinterpret_cast<volatile uint32_t*>(smem + S::kBars + 120);
     volatile int* s_fail = reinterpret_cast<volatile int*>(smem + S::kBars + 124);
 
@@ -339,7 +342,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prefix_kernel(const PrefixPara
         return true;
     };
 
-    float sum_l = 0.f, ref = -INFINITY;  // of this thread's row (and half of the tokens)
+    float sum_l = 0.f;  // of this thread's row (and half of the tokens)
+    // The row's reference, -inf until it has seen a token with a score (a page can be
+    // missing, a row NaN), and what stands for it in the arithmetic.
+    float top_seen = -INFINITY, ref = 0.f;
     bool finished = false;               // softmax warps: all tiles done
     const int quarter = warp & 3, half = warp >> 2 & 1;  // of the softmax warps
     const uint32_t lane_base = tmem + ((uint32_t)(32 * quarter) << 16);
@@ -413,18 +419,22 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prefix_kernel(const PrefixPara
             fence_after();
             const uint32_t s_at = lane_base + kColS + 128 * b + 64 * half;
             const float* num = numbers + (i & 3) * 2 * kTile + 64 * half;
-            // columns of this half that hold tokens
+            // columns of this half that hold tokens, and a byte for each of its 16-column
+            // blocks: not 0 if its page is not there
             const int live = length - (tile0 + i) * kTile - 64 * half;
-            // 16 columns of S have come; columns past the end at -inf
+            const uint32_t missing =
+                *reinterpret_cast<const uint32_t*>(gone + (i & 3) * kFillWarps + 4 * half);
+            // 16 columns of S have come; columns past the end, or of no page, at -inf
             auto take_s = [&](int c, uint32_t (&s)[16]) {
                 ld_wait(s);
                 if (kBf16 && scaled) {
 #pragma unroll
                     for (int j = 0; j < 16; ++j) s[j] = __float_as_uint(__uint_as_float(s[j]) * unit);
                 }
-                if (live < 16 * c + 16) {
+                if (live < 16 * c + 16 || missing != 0) {
+                    const bool none = (missing >> (8 * c) & 0xffu) != 0;
 #pragma unroll 1
-                    for (int j = max(0, live - 16 * c); j < 16; ++j)
+                    for (int j = none ? 0 : max(0, live - 16 * c); j < 16; ++j)
 #pragma unroll
                         for (int x = 0; x < 16; ++x)
                             if (x == j) s[x] = 0xff800000u;
@@ -444,9 +454,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prefix_kernel(const PrefixPara
                 return good;
             };
             // Until the weights fit the reference: usually once.  The first tile
-            // has none yet.  What the two warps of a row do next is decided by
+            // with a score has none yet.  What the two warps of a row do next is decided by
             // their barrier alone, so neither can wait for the other in vain.
-            bool fresh = i == 0;
+            const bool first = __any_sync(0xffffffffu, top_seen == -INFINITY);
+            bool fresh = first;
             for (int tries = 0;; ++tries, fresh = false) {
                 float try_l[2] = {l2[0], l2[1]};
                 __half2 most = __half2half2(__half(0.f));
@@ -513,10 +524,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prefix_kernel(const PrefixPara
                     break;
                 }
                 top = fmaxf(top, tops[(half ^ 1) * kRows + in_tile]);
-                top = fmaxf(top, ref);
-                if (top == -INFINITY) top = 0.f;  // a row of NaN has no largest score
-                const float f = ex2(ref - top);
-                ref = top;
+                top = fmaxf(top, top_seen);
+                const float next = top == -INFINITY ? 0.f : top;
+                const float f = ex2(top_seen - next);  // 0 over what nothing was seen of
+                top_seen = top;
+                ref = next;
                 l2[0] *= f, l2[1] *= f;
                 if (i > 0) {
 #pragma unroll 1
@@ -549,32 +561,34 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prefix_kernel(const PrefixPara
     } else if (warp < kMmaWarp) {
         // ---------------- expansion: one cache block a warp ----------------
         const int w = warp - kSoftWarps;
-        uint32_t where = 0xffffffffu;  // lane i: the block of the 32-tile batch's i-th tile
+        constexpr uint32_t kAbsent = 0xffffffffu, kInvalid = 0xfffffffeu;
+        uint32_t where = kAbsent;  // lane i: the block of the 32-tile batch's i-th tile
         const Pieces<kDim, kBits> pieces(lane);
         uint4 raw[2][S::kLoads];       // a block's K and V on their way
         __half scale = __half(0.f);
-        uint32_t at = 0xffffffffu;
+        uint32_t at = kAbsent;
         auto find = [&](int i) {  // tile i's block
             if (i >= tiles) return;
             if ((i & 31) == 0) {
                 const int blk = (tile0 + i + lane) * 8 + w;
-                where = 0xffffffffu;
+                where = kAbsent;
                 if (i + lane < tiles && blk * kKvBlock < length) {
                     const int index = p.page_blocks.div(blk);
-                    int page = __ldg(a.table + index);
-                    if (page < 0 || page >= a.num_pages) {  // recorded; page 0 is read
+                    const int page = __ldg(a.table + index);
+                    if (page < 0 || page >= a.num_pages) {  // recorded, its tokens left out
                         atomicCAS(&g_kv_prefix_status, 0, kStatusKvIndex);
-                        page = 0;
+                        where = kInvalid;
+                    } else {
+                        where = ((uint32_t)page * a.kv_heads + head) * p.page_blocks.d +
+                                (blk - index * p.page_blocks.d);
                     }
-                    where = ((uint32_t)page * a.kv_heads + head) * p.page_blocks.d +
-                            (blk - index * p.page_blocks.d);
                 }
             }
             at = __shfl_sync(0xffffffffu, where, i & 31);
         };
         auto fetch = [&](int x, int i) {  // its K (0, with the scales) or V (1)
             if (i >= tiles) return;
-            if (at == 0xffffffffu) {
+            if (at >= kInvalid) {
 #pragma unroll
                 for (int n = 0; n < S::kLoads; ++n) raw[x][n] = make_uint4(0, 0, 0, 0);
                 if (x == 0) scale = __half(0.f);
@@ -608,13 +622,14 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prefix_kernel(const PrefixPara
             if (i >= 2 && !__all_sync(0xffffffffu, wait(kempty + 8 * b, (i - 2) >> 1))) break;
             // K's scale (lanes 0-15) and V's (16-31) of token lane & 15, 0 past
             // the end; that S(i - 2) is done says that softmax i - 4 is
-            const bool seen = at != 0xffffffffu &&
+            const bool seen = at < kInvalid &&
                               (tile0 + i) * kTile + kKvBlock * w + (lane & 15) < length;
             const float s = seen ? __half2float(scale) : 0.f;
             // A zero scale has all-zero values, so any other does as well: with fp16's
             // smallest, a weight shows when the token's score passes the reference.
             numbers[(i & 3) * 2 * kTile + (lane >> 4) * kTile + kKvBlock * w + (lane & 15)] =
                 lane < 16 ? (seen ? s * log2_scale : 1.f) : (seen ? fmaxf(s, 0x1p-24f) : 0.f);
+            if (lane == 0) gone[(i & 3) * kFillWarps + w] = at == kInvalid;
             store(0, kbuf + b * S::kOperandBytes);
             arrive(kfull + 8 * b);
             if (lane == 0) mbar_arrive(nfull + 8 * (i & 3));
@@ -670,7 +685,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prefix_kernel(const PrefixPara
     // ---------------- the output, through shared memory ----------------
     if (finished) {
         sum_l += tops[(half ^ 1) * kRows + 32 * quarter + lane];
-        const float inv = sum_l > 0.f ? 1.f / sum_l : sum_l;  // 0 cannot be; NaN stays
+        const float inv = sum_l > 0.f ? 1.f / sum_l : sum_l;  // 0: no token; NaN stays
         float* row = reinterpret_cast<float*>(smem + (32 * quarter + lane) * S::kOutStride);
 #pragma unroll 1
         for (int c = half * (kDim / 2); c < (half + 1) * (kDim / 2); c += 32) {

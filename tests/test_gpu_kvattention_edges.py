@@ -4,6 +4,7 @@ import numpy as np
 import pytest
 import torch
 
+from cudalab_b200 import _native as nat
 from cudalab_b200.build import build
 from oracle import attention_oracle as oa
 from test_gpu_kvattention import BF16, F16, Cache, _check, _q
@@ -135,3 +136,28 @@ def test_strong_channel_and_queries_with_a_mean(mean, strong, D, bits, dtype):
         out, lse = build("kvattention").forward(q, c.pages, c.table, c.len_tensor(),
                                                 return_lse=True)
         _check(out, lse, q, c, D ** -0.5)
+
+
+@pytest.mark.parametrize("batch", [1, 33])
+@pytest.mark.parametrize("D,bits", [(64, 4), (128, 8)])
+@pytest.mark.parametrize("shift", [0.0, -300.0])
+@pytest.mark.parametrize("gone", [[3], [0, 1, 2, 3], list(range(8, 14)), [20], list(range(21))],
+                         ids=lambda g: "-".join(map(str, g[:4])))
+def test_prefix_pages_outside_the_cache_are_skipped(gone, shift, D, bits, batch):
+    """Their tokens are left out, in both kernels, wherever they lie and however low the
+    scores of what remains are; the error is recorded."""
+    n, page = 1300, 64
+    g = torch.Generator().manual_seed(79)
+    p = Cache([n], 1, D, bits, page, seed=80)
+    d = torch.sign(torch.randn(D, generator=g))
+    k = 0.1 * torch.randn(n, 1, D, generator=g) + d * (shift / D)
+    _set(p, k, torch.randn(n, 1, D, generator=g), bits)
+    table = p.table[0].clone()
+    table[gone] = 1 << 30
+    q = (d + 0.1 * torch.randn(batch, 1, 4, D, generator=g)).half().cuda()
+    out, lse, c = _over_prefix(p, q, 1.0, 0, bits, prefix_pages=table)
+    torch.cuda.synchronize()
+    assert nat.device_status(clear=True) == 7
+    keep = [j for j in range(n) if j // page not in gone]
+    p.k[0], p.v[0], p.lengths = p.k[0][keep], p.v[0][keep], [len(keep)]
+    _check(out, lse, q, c, 1.0, prefix=p)
