@@ -18,12 +18,15 @@
 // of k inside an mma is free, so a lane takes contiguous bytes and q is loaded
 // in the same order.
 //
-// Softmax.  Each row keeps one reference m, the running maximum of s_j + log2
-// vs_j (base 2): the V weights w_j = 2^(s_j + log2 vs_j - m) then lie in the
-// range fp16 represents with full relative precision whatever the scales are,
-// and the denominator sums w_j / vs_j in fp32 under the same reference.  m
-// only moves when a score exceeds it by more than kSlack, so the usual block
-// pays one vote instead of a reduction and a rescale.
+// Softmax.  Each row keeps one reference m, kLift below the running maximum of
+// s_j + log2 vs_j (base 2): the V weights w_j = 2^(s_j + log2 vs_j - m) then lie in
+// the range fp16 represents whatever the scales are, and the denominator sums
+// w_j / vs_j in fp32 under the same reference.  The weights round to fp16 (2^-11
+// of each, 2^-25 of one below 2^-14) because the tensor cores take them in V's
+// type; a second product with what the rounding left would double O's
+// instructions.  m only moves when a score exceeds the maximum it was taken from
+// by more than kSlack, so the usual block pays one vote instead of a reduction
+// and a rescale.
 //
 // Split.  The 16-token blocks of all (sequence, head, row tile) segments form
 // one line that is cut into equal ranges, one per CTA of a persistent grid, so
@@ -70,7 +73,11 @@ constexpr int kFan = 16;         // partial results added by one CTA at a time
 // unit.  Without it the CTA that gets the shortest sequences of a ragged batch
 // ends last (64 sequences of 1 to 1024 tokens: 91 us, with it 37).
 constexpr int kSegmentCost = 8;
-constexpr float kSlack = 8.f;    // weights stay below 2^8, far inside fp16
+// A row's weights are fp16: with its reference kLift below the largest logit the
+// largest weight is 2^7, one far smaller keeps 7 bits more than under a largest
+// of 1 (a long tail of them counts: 16384 tokens 2^-25.5 of the largest each were
+// lost whole), and with kSlack more before the reference moves it stays below 2^15.
+constexpr float kLift = 7.f, kSlack = 8.f;
 constexpr int kPartialFloats = 16 * 128 + 2 * 16;  // O, m and l of one partial result
 constexpr size_t kCounterBytes = (size_t)kMaxGrid * 3 * sizeof(int);
 
@@ -743,12 +750,12 @@ __global__ void __launch_bounds__(kThreads, Shape<kDim, kBits, kNB>::kPerSm)
 #pragma unroll
                             for (int x = 4; x < 32; x <<= 1)
                                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-                            top = fmaxf(top, m[n][c]);
+                            top = fmaxf(top - kLift, m[n][c]);
                             // a row that has seen nothing keeps -inf and zeros
                             const float f = top == -INFINITY ? 1.f : ex2(m[n][c] - top);
                             m[n][c] = top;
                             ref[n][c] = top == -INFINITY ? 0.f : top;
-                            limit[n][c] = top + kSlack;
+                            limit[n][c] = top + (kLift + kSlack);
                             l[n][c] *= f;
 #pragma unroll
                             for (int i = 0; i < kSteps; ++i) {

@@ -17,7 +17,8 @@
 //     Tensor Memory and the same layout of V read across (MN-major);
 //   * 8 warps, half a row's tokens a thread, do the softmax as in
 //     kv_attention.cu: p_j = 2^(s_j - m) summed in fp32, weights p_j vs_j in
-//     fp16, one lazy reference m per row near the maximum of s_j + log2 vs_j,
+//     fp16 (what the MMA takes beside V), one lazy reference m per row near the
+//     maximum of s_j + log2 vs_j,
 //     O is only rescaled when a weight exceeds kMostWeight,
 //     which the two warps of a row find out with one barrier a tile.
 // S is double-buffered: the tensor cores compute tile i + 1's S and tile i -
@@ -58,7 +59,9 @@ constexpr int kRows = 128, kTile = 128;  // query rows and tokens of a tile
 constexpr int kSoftWarps = 8, kFillWarps = 8;
 constexpr int kMmaWarp = kSoftWarps + kFillWarps;
 constexpr int kThreads = 32 * (kMmaWarp + 1);
-constexpr float kMostWeight = 256.f;  // far inside fp16
+// Weights are fp16: the row's largest is 2^7 when its reference is taken, so that
+// a tail of far smaller ones keeps its bits, and stays below fp16's 65504.
+constexpr float kLift = 7.f, kMostWeight = 32768.f;
 constexpr uint32_t kColS = 0, kColO = 256, kColP = 384, kColQ = 448, kColumns = 512;
 
 __device__ __forceinline__ float ex2(float x) {
@@ -343,9 +346,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prefix_kernel(const PrefixPara
     };
 
     float sum_l = 0.f;  // of this thread's row (and half of the tokens)
-    // The row's reference, -inf until it has seen a token with a score (a page can be
-    // missing, a row NaN), and what stands for it in the arithmetic.
-    float top_seen = -INFINITY, ref = 0.f;
+    // The row's reference, kLift below its largest s_j + log2 vs_j; -inf until it has
+    // seen a token with a score (a page can be missing, a row NaN), and what stands
+    // for it in the arithmetic.
+    float known = -INFINITY, ref = 0.f;
     bool finished = false;               // softmax warps: all tiles done
     const int quarter = warp & 3, half = warp >> 2 & 1;  // of the softmax warps
     const uint32_t lane_base = tmem + ((uint32_t)(32 * quarter) << 16);
@@ -456,8 +460,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prefix_kernel(const PrefixPara
             // Until the weights fit the reference: usually once.  The first tile
             // with a score has none yet.  What the two warps of a row do next is decided by
             // their barrier alone, so neither can wait for the other in vain.
-            const bool first = __any_sync(0xffffffffu, top_seen == -INFINITY);
-            bool fresh = first;
+            bool fresh = __any_sync(0xffffffffu, known == -INFINITY);
             for (int tries = 0;; ++tries, fresh = false) {
                 float try_l[2] = {l2[0], l2[1]};
                 __half2 most = __half2half2(__half(0.f));
@@ -524,11 +527,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prefix_kernel(const PrefixPara
                     break;
                 }
                 top = fmaxf(top, tops[(half ^ 1) * kRows + in_tile]);
-                top = fmaxf(top, top_seen);
-                const float next = top == -INFINITY ? 0.f : top;
-                const float f = ex2(top_seen - next);  // 0 over what nothing was seen of
-                top_seen = top;
-                ref = next;
+                top = fmaxf(top - kLift, known);
+                ref = top == -INFINITY ? 0.f : top;
+                const float f = ex2(known - ref);  // 0 while nothing has been seen
+                known = top;
                 l2[0] *= f, l2[1] *= f;
                 if (i > 0) {
 #pragma unroll 1

@@ -161,3 +161,35 @@ def test_prefix_pages_outside_the_cache_are_skipped(gone, shift, D, bits, batch)
     keep = [j for j in range(n) if j // page not in gone]
     p.k[0], p.v[0], p.lengths = p.k[0][keep], p.v[0][keep], [len(keep)]
     _check(out, lse, q, c, 1.0, prefix=p)
+
+
+@pytest.mark.parametrize("batch", [1, 33])
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("first", [0, 9000])
+def test_long_tail_of_small_weights(first, bits, batch):
+    """One token outweighs each of the others 2^25.5 times and has no value where they
+    have theirs, so those elements are the sum of the tail.  Tolerance: a weight is
+    fp16, of which the row's largest takes at least 2^7, so one of the tail is right
+    to half of fp16's smallest number, 2^-32 of the largest; the output rounds once
+    and 2^-9 covers the rest."""
+    n, D = 16384, 64
+    p = Cache([n], 1, D, bits, 64, seed=74)
+    k, v = torch.zeros(n, 1, D), torch.ones(n, 1, D)
+    k[first, 0] = 25.5 * np.log(2) / D
+    v[first, 0, 1:] = 0
+    _set(p, k, v, bits)
+    q = torch.ones(batch, 1, 4, D, dtype=F16, device="cuda")
+    out, lse, c = _over_prefix(p, q, 1.0, 0, bits)
+    ref, rl, _, _ = oa.attention(q[0].double().cpu().numpy(), p.k[0], p.v[0], n, 1.0)
+    assert 2.0 ** -12 < ref[0, 0, 1] < 2.0 ** -11
+    err = np.abs(out[:, 0].double().cpu().numpy() - ref)
+    tol = 2.0 ** -9 * np.abs(ref) + n * 2.0 ** -32
+    assert (err <= tol).all(), float((err / tol).max())
+    assert np.abs(lse[:, 0].double().cpu().numpy() - rl).max() < 1e-5
+    # 64 sequences of the same pages, so that a warp of the register-fed kernel meets the
+    # large token and hundreds of the others
+    table = p.table.expand(64, -1).contiguous()
+    lens = torch.full((64,), n, dtype=torch.int32, device="cuda")
+    out = build("kvattention").forward(q[:1, 0].expand(64, -1, -1), p.pages, table, lens, scale=1.0)
+    err = np.abs(out.double().cpu().numpy() - ref)
+    assert (err <= tol).all(), float((err / tol).max())
