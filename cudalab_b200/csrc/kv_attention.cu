@@ -586,9 +586,9 @@ __global__ void __launch_bounds__(kThreads, Shape<kDim, kBits, kNB>::kPerSm)
         const int len = chunked ? len0 : s_len[seg.seq];
         const int token0 = first_block(len) * kKvBlock - seg.begin * (kU * kKvBlock);
 
-        // q as B fragments.  Rows are brought to [1, 2) by a power of two (exact;
-        // elements 2^14 below their row's largest lose bits that fp32 sums would
-        // not keep either).  rs brings a score to base-2 logits.
+        // q as B fragments, in fp16.  Rows are brought to [2^15, 2^16) by a power of two,
+        // which holds fp16 elements exactly and bf16 ones down to 2^-32 of their row's
+        // largest.  rs brings a score to base-2 logits.
         uint32_t qf[kNB][kSteps][2];
         float rs[kNB][2];
 #pragma unroll
@@ -602,12 +602,12 @@ __global__ void __launch_bounds__(kThreads, Shape<kDim, kBits, kNB>::kPerSm)
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
             const int e = (int)(__float_as_uint(top) >> 23) - 127;
             float unit = a.scale * 1.4426950408889634f;
-            // zero, denormal and non-finite rows stay as they are
-            if (e > -126 && e < 127) {
-                const float down = __uint_as_float((uint32_t)(127 - e) << 23);
+            if (e < 128) {  // rows with an infinity stay as they are
+                const int up = min(15 - e, 126);
+                const float factor = __uint_as_float((uint32_t)(127 + up) << 23);
 #pragma unroll
-                for (int i = 0; i < kDim / 4; ++i) x[i] *= down;
-                unit *= __uint_as_float((uint32_t)(127 + e) << 23);
+                for (int i = 0; i < kDim / 4; ++i) x[i] *= factor;
+                unit *= __uint_as_float((uint32_t)(127 - up) << 23);
             }
 #pragma unroll
             for (int c = 0; c < 2; ++c) rs[n][c] = __shfl_sync(0xffffffffu, unit, 8 * t + 4 * c);

@@ -370,25 +370,33 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prefix_kernel(const PrefixPara
                 if (r < p.rows)
                     raw[c] = p.q_vec ? load8<kBf16, true>(src, 8 * c) : load8<kBf16, false>(src, 8 * c);
             }
-            // bf16 rows that fp16 would not hold are scaled into its range
-            float down = 1.f;
+            // A bf16 row that fp16 does not hold exactly is brought to [2^15, 2^16), where
+            // it does down to 2^-32 of the row's largest.  (Few are: rows in fp16's range
+            // without elements below 2^-17 need no multiplication of their scores.)
+            float factor = 1.f;
             if (kBf16) {
                 float top = 0.f;
+                bool exact = true;
 #pragma unroll
                 for (int c = 0; c < kDim / 16; ++c) {
                     float x[8];
                     unpack8<kBf16>(raw[c], x);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[i]));
+                    for (int i = 0; i < 8; i += 2) {
+                        top = fmaxf(top, fmaxf(fabsf(x[i]), fabsf(x[i + 1])));
+                        const float2 h = __half22float2(__floats2half2_rn(x[i], x[i + 1]));
+                        exact &= h.x == x[i] && h.y == x[i + 1];
+                    }
                 }
                 tops[half * kRows + in_tile] = top;
-                any_of_rows(1 + quarter, false);
+                exact = !any_of_rows(1 + quarter, !exact);
                 top = fmaxf(top, tops[(half ^ 1) * kRows + in_tile]);
                 any_of_rows(1 + quarter, false);  // read before it is written again
                 const int e = (int)(__float_as_uint(top) >> 23) - 127;
-                if ((e >= 15 || e < -6) && e > -126 && e < 127) {
-                    down = __uint_as_float((uint32_t)(127 - e) << 23);
-                    unit = __uint_as_float((uint32_t)(127 + e) << 23);
+                if (!exact && e < 128) {  // rows with an infinity stay as they are
+                    const int up = min(15 - e, 126);
+                    factor = __uint_as_float((uint32_t)(127 + up) << 23);
+                    unit = __uint_as_float((uint32_t)(127 - up) << 23);
                 }
             }
 #pragma unroll
@@ -399,7 +407,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prefix_kernel(const PrefixPara
                     float x[8];
                     unpack8<kBf16>(raw[d / 8 + c], x);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) x[i] *= down;
+                    for (int i = 0; i < 8; ++i) x[i] *= factor;
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
                         packed[4 * c + i] = kBits == 8 ? pack2<false>(x[2 * i], x[2 * i + 1])

@@ -193,3 +193,22 @@ def test_long_tail_of_small_weights(first, bits, batch):
     out = build("kvattention").forward(q[:1, 0].expand(64, -1, -1), p.pages, table, lens, scale=1.0)
     err = np.abs(out.double().cpu().numpy() - ref)
     assert (err <= tol).all(), float((err / tol).max())
+
+
+@pytest.mark.parametrize("batch", [1, 33])
+@pytest.mark.parametrize("top", [1.5 * 2.0 ** -6, 1.0, 1e20])
+def test_bf16_rows_of_mixed_magnitudes(top, batch):
+    """The row's largest element meets a zero of K, the others are 2^-20 of it and make
+    the scores alone: they keep bf16's bits."""
+    n, D = 600, 128
+    g = torch.Generator().manual_seed(75)
+    p = Cache([n], 1, D, 8, 64, seed=76)
+    k, v = torch.randn(2, n, 1, D, generator=g)
+    k[..., 0] = 0
+    _set(p, k, v, 8)
+    q = torch.randn(batch, 1, 4, D, generator=g) * (top * 2.0 ** -20)
+    q[..., 0] = top
+    q = q.to(BF16).cuda()
+    scale = float(0.3 / (top * 2.0 ** -20))
+    out, lse, c = _over_prefix(p, q, scale)
+    _check(out, lse, q, c, scale, prefix=p)
