@@ -40,8 +40,8 @@ def rotary_table(rows: int, rotary: int, base: float = 10000.0, device="cuda") -
 
 class AttentionLayer:
     """Weights, cache and workspace of one layer; up to 16 sequences (the rows that a quantised
-    projection takes at once).  Each sequence owns `context` tokens of pages; with a prefix the
-    cache holds its pages behind them."""
+    projection takes at once).  Each sequence owns the pages of `context` tokens, `capacity` in
+    all; with a prefix the cache holds its pages behind them."""
 
     def __init__(self, batch: int, hidden: int, q_heads: int, kv_heads: int, head_dim: int,
                  context: int, bits: int = 8, page_size: int = 64, prefix: int = 0, seed: int = 0):
@@ -61,8 +61,9 @@ class AttentionLayer:
         self.norm, self.q_norm, self.k_norm = (
             (1 + 0.1 * torch.randn(n, device="cuda", generator=g)).half()
             for n in (hidden, head_dim, head_dim))
-        self.table = rotary_table(prefix + context, head_dim)
         width, shared = -(-context // page_size), -(-prefix // page_size)
+        self.capacity = width * page_size
+        self.table = rotary_table(prefix + self.capacity, head_dim)
         self.pages = self.cache.empty(batch * width + shared, kv_heads, head_dim, bits, page_size)
         self.page_table = torch.arange(batch * width, device="cuda",
                                        dtype=torch.int32).view(batch, width)
@@ -73,27 +74,37 @@ class AttentionLayer:
 
     def fill(self, k, v, sequence: int | None) -> None:
         """Appends k, v [tokens, kv_heads, head_dim] (already rotated) to a sequence, or writes
-        the shared prefix (None)."""
+        the shared prefix (None).  Refuses what the pages do not hold."""
         if sequence is None:
-            first, pages = 0, self.prefix_pages.long()
+            first, most, pages = 0, self.prefix, self.prefix_pages.long()
         else:
-            first, pages = int(self.lengths[sequence]), self.page_table[sequence].long()
-            self.lengths[sequence] += k.size(0)
-        at = torch.arange(first, first + k.size(0), device="cuda")
+            first, most = int(self.lengths[sequence]), self.capacity
+            pages = self.page_table[sequence].long()
+        if first + k.size(0) > most:
+            raise RuntimeError(f"{k.size(0)} tokens after {first} exceed the {most} that the "
+                               f"{'prefix' if sequence is None else 'sequence'} holds")
+        at = torch.arange(first, first + k.size(0), device=self.pages.device)
         self.cache.write(k, v, self.pages, pages[at // self.page_size] * self.page_size
                          + at % self.page_size)
+        if sequence is not None:
+            self.lengths[sequence] += k.size(0)
 
     def slots(self) -> torch.Tensor:
-        """int64 [batch]: where each sequence's next token goes."""
+        """int64 [batch]: where each sequence's next token goes, -1 (skipped by the cache) for
+        one whose pages are full."""
         at = self.lengths.long()
-        page = self.page_table.gather(1, (at // self.page_size)[:, None])[:, 0].long()
-        return page * self.page_size + at % self.page_size
+        index = (at // self.page_size).clamp(max=self.page_table.size(1) - 1)
+        page = self.page_table.gather(1, index[:, None])[:, 0].long()
+        return torch.where(at < self.capacity, page * self.page_size + at % self.page_size, -1)
 
     def step(self, x: torch.Tensor) -> torch.Tensor:
-        """x fp16 [batch, hidden] of each sequence's next token -> the layer's output."""
+        """x fp16 [batch, hidden] of each sequence's next token -> the layer's output.  A
+        sequence past its capacity keeps its cache; its row attends to that without the new
+        token, and the device status records the length (7): a captured step has no other way
+        to refuse it."""
+        qkv = self.gemv.forward_rmsnorm("int4gemv_rmsnorm", *self.w_qkv, x, self.norm)
         slots, positions = self.slots(), self.lengths + self.prefix
         self.lengths += 1
-        qkv = self.gemv.forward_rmsnorm("int4gemv_rmsnorm", *self.w_qkv, x, self.norm)
         qkv = qkv.view(self.batch, -1, self.head_dim)
         q, k, v = qkv.split((self.q_heads, self.kv_heads, self.kv_heads), 1)
         q, k = self.rope.forward(q, k, self.q_norm, self.k_norm, self.table, positions)
