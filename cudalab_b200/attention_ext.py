@@ -62,10 +62,12 @@ def _plain(name: str, x: torch.Tensor, dims: int, dtypes, dev: torch.device) -> 
 
 
 def _apart(name: str, x: torch.Tensor) -> None:
-    """An output whose elements do not share memory (an expanded tensor's do)."""
-    span = 1 + sum((n - 1) * s for n, s in zip(x.shape, x.stride()) if n > 0)
-    _chk(x.numel() == 0 or (all(s > 0 for n, s in zip(x.shape, x.stride()) if n > 1)
-                            and span >= x.numel()), f"{name} must not overlap itself")
+    """An output whose elements do not share memory: each dimension steps past all that the
+    ones of smaller strides span (an expanded tensor's, or an overlapping window's, does not)."""
+    end = 0  # last element of the dimensions so far
+    for step, n in sorted((s, n) for n, s in zip(x.shape, x.stride()) if n > 1):
+        _chk(x.numel() == 0 or step > end, f"{name} must not overlap itself")
+        end += (n - 1) * step
 
 
 def _pages(pages: torch.Tensor, head_dim: int, dev: torch.device | None = None) -> tuple:

@@ -3,6 +3,7 @@ without a GPU."""
 import ctypes
 
 import pytest
+import torch
 
 from cudalab_b200 import _native as nat
 
@@ -26,3 +27,16 @@ def test_descriptor_refuses_what_its_fields_do_not_hold():
                     assert getattr(cls(*values), name) == big or ctype is ctypes.c_float
             values[i] = (1 << 31) - 1
             assert int(getattr(cls(*values), name)) in ((1 << 31) - 1, 1 << 31)
+
+
+def test_outputs_that_overlap_themselves():
+    from cudalab_b200.attention_ext import _apart
+
+    x = torch.zeros(4096)
+    for size, stride in (((2, 2, 64), (200, 10, 1)), ((3, 2, 64), (64, 64, 1)),
+                         ((2, 2, 64), (0, 64, 1)), ((2, 3, 64), (64, 63, 1)), ((2, 2), (1, 1))):
+        shared = torch.as_strided(x, size, stride)
+        _rej(lambda: _apart("out", shared), "out must not overlap itself")
+    for size, stride in (((2, 2, 64), (200, 64, 1)), ((2, 3, 64), (64, 128, 1)), ((1, 2, 64), (0, 64, 1)),
+                         ((2, 1, 64), (64, 5, 1)), ((0, 2, 64), (0, 0, 1)), ((3, 4, 60), (256, 61, 1))):
+        _apart("out", torch.as_strided(x, size, stride))
