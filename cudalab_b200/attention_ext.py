@@ -70,6 +70,16 @@ def _apart(name: str, x: torch.Tensor) -> None:
         end += (n - 1) * step
 
 
+def _separate(name: str, y: torch.Tensor, other: str, x: torch.Tensor) -> None:
+    """An output whose memory lies outside an input's first to last element."""
+    def ends(t):
+        last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+        return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+    if x.numel() and y.numel():
+        (a, b), (c, d) = ends(y), ends(x)
+        _chk(b <= c or d <= a, f"{name} must not overlap {other}")
+
+
 def _pages(pages: torch.Tensor, head_dim: int, dev: torch.device | None = None) -> tuple:
     """(bits, page_size) of a cache tensor for heads of head_dim elements."""
     _chk(head_dim in HEAD_DIMS, f"head_dim must be 64, 128 or 256, got {head_dim}")
@@ -287,6 +297,7 @@ class KvAttentionExt(_Ext):
             _chk(out.shape == q.shape and out.dtype == q.dtype and out.is_contiguous()
                  and out.device == dev and out.data_ptr() % 16 == 0,
                  f"out must be contiguous {q.dtype} {list(q.shape)} on {dev}, 16-byte aligned")
+            _separate("out", out, "q", q)  # rows are written while others are still read
         lse = torch.empty(q.shape[:-1], dtype=torch.float32, device=dev) if return_lse else None
         q4 = q.unsqueeze(1) if q.dim() == 3 else q
         if prefix_length and q4.size(0) > 1 and q4.size(1) > 1 \
@@ -334,7 +345,7 @@ class KvAttentionExt(_Ext):
 
     def forward_into(self, q, pages, page_table, lengths, out, scale: float | None = None,
                      window: int = 0, workspace=None) -> None:
-        """Same into `out` (contiguous, like q)."""
+        """Same into `out` (contiguous, like q, apart from it)."""
         self._forward(q, pages, page_table, lengths, scale, window, workspace, None, 0, out, False)
 
     def forward_shared(self, q, pages, prefix_pages, prefix_length: int, page_table, lengths,

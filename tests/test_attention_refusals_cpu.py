@@ -40,3 +40,14 @@ def test_outputs_that_overlap_themselves():
     for size, stride in (((2, 2, 64), (200, 64, 1)), ((2, 3, 64), (64, 128, 1)), ((1, 2, 64), (0, 64, 1)),
                          ((2, 1, 64), (64, 5, 1)), ((0, 2, 64), (0, 0, 1)), ((3, 4, 60), (256, 61, 1))):
         _apart("out", torch.as_strided(x, size, stride))
+
+
+def test_output_over_its_input():
+    from cudalab_b200.attention_ext import _separate
+
+    x = torch.zeros(3, 12, 64, dtype=torch.float16)
+    for y in (x, x[1:], x[2, 7:], x[:, 4:8], x.flatten()[64 * 7:64 * 9]):
+        _rej(lambda: _separate("out", y, "q", x[:, :8]), "out must not overlap q")
+    _separate("out", x[2, 8:], "q", x[:, :8])
+    _separate("out", x[2], "q", x[:2])
+    _separate("out", x[:0], "q", x)

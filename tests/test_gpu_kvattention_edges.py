@@ -212,3 +212,15 @@ def test_bf16_rows_of_mixed_magnitudes(top, batch):
     scale = float(0.3 / (top * 2.0 ** -20))
     out, lse, c = _over_prefix(p, q, scale)
     _check(out, lse, q, c, scale, prefix=p)
+
+
+def test_output_over_q_is_refused():
+    c = Cache([20, 5], 1, 64, 8, 16, seed=87)
+    q = _q(2, 1, 4, 64, F16, seed=88)[:, 0]
+    att = build("kvattention")
+    ref = att.forward(q, c.pages, c.table, c.len_tensor())
+    with pytest.raises(RuntimeError, match="out must not overlap q"):
+        att.forward_into(q, c.pages, c.table, c.len_tensor(), q)
+    out = torch.empty_like(q)
+    att.forward_into(q, c.pages, c.table, c.len_tensor(), out)
+    assert torch.equal(out, ref)
