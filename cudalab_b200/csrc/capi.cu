@@ -848,6 +848,7 @@ int cl_kvattention(const void* q, const uint8_t* pages, const int32_t* page_tabl
     a.workspace = workspace;
     if (!clb::kv_attention_fits(a))
         return bad(op, "the page tables span too many blocks for one launch");
+    if (!clb::kv_attention_tiles_fit(a)) return bad(op, "too many query rows for one launch");
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (d->prefix_length > 0) {
         if (!prefix_pages || !prefix_scratch) return bad(op, "null prefix pointer");
@@ -861,6 +862,8 @@ int cl_kvattention(const void* q, const uint8_t* pages, const int32_t* page_tabl
         if (!clb::kv_attention_fits(f))
             return bad(op, "the prefix spans too many blocks for one launch");
         const bool tensor = clb::kv_prefix_takes(f);
+        if (!tensor && !clb::kv_attention_tiles_fit(f))
+            return bad(op, "too many query rows for one launch over the prefix");
         a.front_parts = tensor ? clb::kv_prefix_parts(f) : 1;
         a.front_by_tensor_cores = tensor;
         a.front = f.out_f32 = prefix_scratch;

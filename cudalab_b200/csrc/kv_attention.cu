@@ -155,7 +155,9 @@ __device__ __forceinline__ int ceil_div(int n, float inv) {
     return __float2int_ru(((float)n - 0.5f) * inv);
 }
 
-// n / d for quotients below 2^21: an estimate, right to one, and its correction.
+// n / d for quotients below kMostQuotient: an estimate, right to one, and its
+// correction (beyond, 24 bits leave it two and more off).
+constexpr int kMostQuotient = 1 << 21;
 __device__ __forceinline__ int quotient(int n, int d) {
     int q = __float2int_rz(__fdividef((float)n, (float)d));
     const int r = n - q * d;
@@ -1055,6 +1057,11 @@ cudaError_t run(Params& p, cudaStream_t stream) {
     return launch_pdl(kernel, dim3((unsigned)grid), dim3(kThreads), smem, stream, p);
 }
 
+// Rows of a tile: 16 where a head has more than 8 and the registers hold them.
+int tile_rows(const KvAttentionArgs& a) {
+    return a.head_dim < 256 && (int64_t)a.new_tokens * a.group > 8 ? 16 : 8;
+}
+
 template <int kDim, int kBits>
 cudaError_t run_dim(Params& p, bool two, bool bf16, cudaStream_t s) {
     if constexpr (kDim < 256) {
@@ -1079,6 +1086,12 @@ bool kv_attention_fits(const KvAttentionArgs& a) {
            a.num_pages * a.kv_heads * per < ((int64_t)1 << 32) - 2;  // blocks are numbered
 }
 
+bool kv_attention_tiles_fit(const KvAttentionArgs& a) {
+    const int64_t rows = (int64_t)a.new_tokens * a.group;
+    const int tile = tile_rows(a);
+    return (rows + tile - 1) / tile * a.kv_heads < kMostQuotient;
+}
+
 cudaError_t launch_kv_attention(const KvAttentionArgs& a, cudaStream_t stream) {
     if (a.batch == 0) return cudaSuccess;
     Params p{};
@@ -1091,7 +1104,7 @@ cudaError_t launch_kv_attention(const KvAttentionArgs& a, cudaStream_t stream) {
     p.q_vec = (reinterpret_cast<uintptr_t>(a.q) & 15u) == 0 && a.q_batch % 8 == 0 &&
               a.q_new % 8 == 0 && a.q_head % 8 == 0;
     p.wait_cycles = wait_budget();
-    const bool two = a.new_tokens * a.group > 8, bf16 = a.type == kTypeBf16;
+    const bool two = tile_rows(a) == 16, bf16 = a.type == kTypeBf16;
     if (a.head_dim == 64)
         return a.bits == 8 ? run_dim<64, 8>(p, two, bf16, stream)
                            : run_dim<64, 4>(p, two, bf16, stream);

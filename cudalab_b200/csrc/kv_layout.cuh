@@ -111,6 +111,8 @@ size_t kv_attention_workspace();
 // Whether the kernel's 32-bit count of blocks holds every length that the page
 // table allows.
 bool kv_attention_fits(const KvAttentionArgs& a);
+// Whether its division by estimates holds the row tiles of a sequence's heads.
+bool kv_attention_tiles_fit(const KvAttentionArgs& a);
 cudaError_t launch_kv_attention(const KvAttentionArgs& a, cudaStream_t stream);
 
 // Attention of all rows (new_tokens of one sequence) over fixed_length tokens that

@@ -6,6 +6,7 @@ import pytest
 import torch
 
 from cudalab_b200 import _native as nat
+from cudalab_b200.build import build_library
 
 
 def _rej(fn, text):
@@ -51,3 +52,30 @@ def test_output_over_its_input():
     _separate("out", x[2, 8:], "q", x[:, :8])
     _separate("out", x[2], "q", x[:2])
     _separate("out", x[:0], "q", x)
+
+
+def test_more_row_tiles_than_the_plan_divides():
+    """Tiles of 16 rows (8 at head_dim 256) of all heads of a sequence: 2^21 and more are
+    refused before any device work."""
+    build_library()
+    lib = nat.load()
+    fake = [1 << 20] * 9
+
+    def call(**kw):
+        d = nat.KvAttentionDesc(num_pages=4, batch=1, kv_heads=2, head_dim=64, bits=8, page_size=64,
+                                max_pages=2, dtype=nat.CL_DTYPE_F16, scale=0.1, **kw)
+        return lib.cl_kvattention(*fake, ctypes.byref(d), None)
+
+    assert call(new_tokens=1 << 20, q_heads=32) == nat.CL_ERR_INVALID_ARGUMENT
+    assert "too many query rows" in nat.last_error(lib)
+    d = dict(num_pages=4, batch=1, kv_heads=1, head_dim=256, bits=8, page_size=64, max_pages=2,
+             dtype=nat.CL_DTYPE_F16, scale=0.1, new_tokens=1 << 20, q_heads=16)
+    assert lib.cl_kvattention(*fake, ctypes.byref(nat.KvAttentionDesc(**d)), None) == \
+        nat.CL_ERR_INVALID_ARGUMENT
+    assert "too many query rows" in nat.last_error(lib)
+    # a prefix that the register-fed kernel would take (head_dim 256)
+    d.update(batch=64, new_tokens=1 << 14, prefix_length=64, prefix_page_count=1, q_batch=1 << 14,
+             q_new=1)
+    assert lib.cl_kvattention(*fake, ctypes.byref(nat.KvAttentionDesc(**d)), None) == \
+        nat.CL_ERR_INVALID_ARGUMENT
+    assert "over the prefix" in nat.last_error(lib)
