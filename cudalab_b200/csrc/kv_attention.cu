@@ -179,6 +179,7 @@ struct Params {
     float inv_grid;
     int q_vec;
     long long wait_cycles;
+    uint32_t hold_ns;
 };
 
 template <int kDim, int kBits, int kNB>
@@ -644,12 +645,11 @@ __global__ void __launch_bounds__(kThreads, Shape<kDim, kBits, kNB>::kPerSm)
 #pragma unroll 1
         for (; cu < sb; cu += kWarps) {
             // every lane leaves the wait with the same answer
-            if (!failed && !__all_sync(0xffffffffu, mbar_try_wait_held(my_bars + 8 * stage, phase >> stage & 1u, kHoldNs))) {
+            if (!failed && !__all_sync(0xffffffffu, mbar_try_wait_held(my_bars + 8 * stage, phase >> stage & 1u, p.hold_ns))) {
                 const long long t0 = clock64();
-                while (!__all_sync(0xffffffffu, mbar_try_wait_held(my_bars + 8 * stage, phase >> stage & 1u, kHoldNs))) {
+                do
                     failed = __any_sync(0xffffffffu, clock64() - t0 > p.wait_cycles);
-                    if (failed) break;
-                }
+                while (!failed && !__all_sync(0xffffffffu, mbar_try_wait_held(my_bars + 8 * stage, phase >> stage & 1u, p.hold_ns)));
                 if (failed && lane == 0) atomicCAS(&g_kv_attention_status, 0, kStatusTimeoutKv);
             }
             if (!failed) {
@@ -998,7 +998,7 @@ __global__ void __launch_bounds__(kThreads, Shape<kDim, kBits, kNB>::kPerSm)
         // the units issued and not done are in the next stages of the ring.
         for (int i = 0; i < min(issued, mine) - done; ++i) {
             const int at_stage = (done + i) % kStages;
-            mbar_wait_held(my_bars + 8 * at_stage, phase >> at_stage & 1u, p.wait_cycles);
+            mbar_wait_held(my_bars + 8 * at_stage, phase >> at_stage & 1u, kWaitTimeoutCycles);
         }
     }
 }
@@ -1104,6 +1104,7 @@ cudaError_t launch_kv_attention(const KvAttentionArgs& a, cudaStream_t stream) {
     p.q_vec = (reinterpret_cast<uintptr_t>(a.q) & 15u) == 0 && a.q_batch % 8 == 0 &&
               a.q_new % 8 == 0 && a.q_head % 8 == 0;
     p.wait_cycles = wait_budget();
+    p.hold_ns = hold_within(p.wait_cycles);
     const bool two = tile_rows(a) == 16, bf16 = a.type == kTypeBf16;
     if (a.head_dim == 64)
         return a.bits == 8 ? run_dim<64, 8>(p, two, bf16, stream)

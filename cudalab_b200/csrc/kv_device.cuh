@@ -123,6 +123,11 @@ __device__ __forceinline__ bool mbar_try_wait_held(uint32_t bar, uint32_t parity
     return ok != 0;
 }
 constexpr uint32_t kHoldNs = 20000;
+// Nanoseconds for which a wait bounded by `budget` SM cycles (about half a
+// nanosecond each) is held.
+inline uint32_t hold_within(long long budget) {
+    return budget < 2 ? 1 : budget / 2 < kHoldNs ? (uint32_t)(budget / 2) : kHoldNs;
+}
 
 // Bounded wait on one phase, at most `budget` SM cycles and one poll more.
 __device__ __forceinline__ bool mbar_wait_held(uint32_t bar, uint32_t parity, long long budget) {

@@ -207,6 +207,7 @@ struct PrefixParams {
     int row_tiles, parts, part_tiles, tiles;
     int q_vec;
     long long wait_cycles;
+    uint32_t hold_ns;
 };
 
 template <int kDim, int kBits>
@@ -223,7 +224,7 @@ struct PrefixShape {
     static constexpr int kNumbers = 4 * kOperandBytes;
     static constexpr int kTops = kNumbers + 4 * 2 * kTile * 4;  // [2][kRows] exchanged by row halves
     static constexpr int kBars = kTops + 2 * kRows * 4;
-    static constexpr int kGone = kBars + 128;  // [4][kFillWarps] bytes: the block is missing
+    static constexpr int kGone = kBars + 136;  // [4][kFillWarps] bytes: the block is missing
     static constexpr int kEnd = kGone + 4 * kFillWarps;
     static constexpr int kSmem = (kEnd < 120 * 1024 ? 120 * 1024 : kEnd) + 1024;
     static_assert(kRows * kOutStride <= 4 * kOperandBytes, "room for the output");
@@ -287,7 +288,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prefix_kernel(const PrefixPara
     float* tops = reinterpret_cast<float*>(smem + S::kTops);
     const uint32_t bars = smem_u32(smem + S::kBars);
     const uint32_t kfull = bars, vfull = bars + 16, kempty = bars + 32, vempty = bars + 48,
-                   sfull = bars + 64, pfull = bars + 80, nfull = bars + 88;
+                   sfull = bars + 64, pfull = bars + 80, nfull = bars + 88, drained = bars + 128;
     uint8_t* gone = smem + S::kGone;
     volatile uint32_t* s_tmem = reinterpret_cast<volatile uint32_t*>(smem + S::kBars + 120);
     volatile int* s_fail = reinterpret_cast<volatile int*>(smem + S::kBars + 124);
@@ -310,6 +311,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prefix_kernel(const PrefixPara
         }
         for (int i = 0; i < 4; ++i) mbar_init(nfull + 8 * i, kFillWarps);
         mbar_init(pfull, kSoftWarps);
+        mbar_init(drained, 1);
         *s_fail = 0;
         fence_barrier_init();
     }
@@ -332,9 +334,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prefix_kernel(const PrefixPara
 
     // A bounded wait; false once it or any other of the CTA has run out.
     auto wait = [&](uint32_t bar, int phase) -> bool {
-        if (mbar_try_wait_held(bar, (uint32_t)phase & 1u, kHoldNs)) return true;
+        if (mbar_try_wait_held(bar, (uint32_t)phase & 1u, p.hold_ns)) return true;
         const long long t0 = clock64();
-        while (!mbar_try_wait_held(bar, (uint32_t)phase & 1u, kHoldNs)) {
+        while (!mbar_try_wait_held(bar, (uint32_t)phase & 1u, p.hold_ns)) {
             if (*s_fail) return false;
             if (clock64() - t0 > p.wait_cycles) {
                 atomicCAS(&g_kv_prefix_status, 0, kStatusTimeoutKv);
@@ -653,7 +655,6 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prefix_kernel(const PrefixPara
     } else if (lane == 0) {
         // ---------------- MMAs ----------------
         constexpr uint32_t kIdescS = instruction(kTile, false), kIdescO = instruction(kDim, true);
-        int committed = 0;
         bool ok = wait(pfull, 0);  // Q
         for (int i = 0; i <= tiles && ok; ++i) {
             if (i < tiles) {
@@ -680,13 +681,13 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prefix_kernel(const PrefixPara
                     mma(tmem + kColO, tmem + kColP + 8 * k, operand(vb + k * 2048, S::kHalfBytes),
                         kIdescO, i > 1 || k > 0);
                 commit(vempty + 8 * b);
-                committed = i;
             }
         }
-        if (!ok && committed > 0) {
-            // the MMAs issued so far end before the memory they use is given up
-            mbar_wait_held(vempty + 8 * ((committed - 1) & 1), (uint32_t)(committed - 1) >> 1 & 1u,
-                              p.wait_cycles);
+        if (!ok) {
+            // every MMA issued so far (the last ones have made S for a tile that nobody
+            // takes up) ends before the memory it uses is given up
+            commit(drained);
+            mbar_wait_held(drained, 0, kWaitTimeoutCycles);
         }
     }
 
@@ -787,6 +788,7 @@ cudaError_t launch_kv_prefix(const KvAttentionArgs& a, cudaStream_t stream) {
     p.part_tiles = (p.tiles + p.parts - 1) / p.parts;
     p.q_vec = aligned16(a.q, a.q_new, a.q_head);
     p.wait_cycles = wait_budget();
+    p.hold_ns = hold_within(p.wait_cycles);
     const bool bf16 = a.type == kTypeBf16;
     if (a.head_dim == 64)
         return a.bits == 8 ? (bf16 ? run<64, 8, true>(p, stream) : run<64, 8, false>(p, stream))
