@@ -587,7 +587,7 @@ __global__ void __launch_bounds__(kThreads, Shape<kDim, kBits, kNB>::kPerSm)
         const int sa = max(seg.begin, u0), sb = min(seg.begin + seg.units, u1);
         const int head = p.row_tiles.div(seg.part), row0 = p.row_tiles.mod(seg.part) * S::kCols;
         const int len = chunked ? len0 : s_len[seg.seq];
-        const int token0 = first_block(len) * kKvBlock - seg.begin * (kU * kKvBlock);
+        const int token0 = first_block(len) * kKvBlock;
 
         // q as B fragments, in fp16.  Rows are brought to [2^15, 2^16) by a power of two,
         // which holds fp16 elements exactly and bf16 ones down to 2^-32 of their row's
@@ -710,7 +710,7 @@ __global__ void __launch_bounds__(kThreads, Shape<kDim, kBits, kNB>::kPerSm)
                                 s[k][n][2 * h + c] = fmaf(s[k][n][2 * h + c], ks * rs[n][c], lv);
                     }
                 }
-                const int j0 = cu * (kU * kKvBlock) + token0;
+                const int j0 = (cu - seg.begin) * (kU * kKvBlock) + token0;
                 bool cut = j0 + kU * kKvBlock > all_hi || j0 < all_lo;
 #pragma unroll
                 for (int k = 0; k < kU; ++k) cut |= (bad[k] >> (done & 31)) & 1u;

@@ -751,11 +751,13 @@ cudaError_t run(const PrefixParams& p, cudaStream_t stream) {
 // set-up and output at about kSetUp tiles and one CTA per SM.
 int cut(int items, int tiles) {
     constexpr int kSetUp = 5, kSms = 148, kMostParts = 16;
-    int best = 1, cost = INT32_MAX;
+    int best = 1;
+    int64_t cost = INT64_MAX;
     for (int parts = 1; parts <= std::min(kMostParts, tiles); ++parts) {
         const int per = (tiles + parts - 1) / parts, used = (tiles + per - 1) / per;
         const int waves = (items * used + kSms - 1) / kSms;
-        if (waves * (per + kSetUp) < cost) cost = waves * (per + kSetUp), best = used;
+        const int64_t tile_times = (int64_t)waves * (per + kSetUp);
+        if (tile_times < cost) cost = tile_times, best = used;
     }
     return best;
 }

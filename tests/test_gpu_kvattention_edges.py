@@ -224,3 +224,25 @@ def test_output_over_q_is_refused():
     out = torch.empty_like(q)
     att.forward_into(q, c.pages, c.table, c.len_tensor(), out)
     assert torch.equal(out, ref)
+
+
+def test_line_of_more_than_2_to_31_tokens():
+    """64 sequences of 65536 tokens (the same pages) times 8 heads times 72 row tiles: the
+    line that the CTAs cut counts 2.4 * 10^9 tokens.  Every sequence gives the same."""
+    n, D, page, new, H, G = 65536, 64, 64, 144, 8, 8
+    g = torch.Generator(device="cuda").manual_seed(89)
+    cache, att = build("kvcache"), build("kvattention")
+    pages = cache.empty(n // page, H, D, 4, page)
+    k, v = torch.randn(2, n, H, D, device="cuda", generator=g).half()
+    cache.write(k, v, pages, torch.arange(n, device="cuda"))
+    q = torch.randn(1, new, H * G, D, device="cuda", generator=g).half()
+    table = torch.arange(n // page, device="cuda", dtype=torch.int32).expand(64, -1).contiguous()
+    lens = torch.full((64,), n, dtype=torch.int32, device="cuda")
+    one, z = att.forward(q, pages, table[:1], lens[:1], return_lse=True)
+    out, lse = att.forward(q.expand(64, -1, -1, -1), pages, table, lens, return_lse=True)
+    # other cuts of the same sums: the weights' sums differ by fp32 roundings, the outputs
+    # (0.02 and less) by one of fp16
+    assert (lse - z).abs().max() < 1e-5
+    assert (out.float() - one.float()).abs().max() < 2.0 ** -14
+    ref = att.forward(q[:, -1:], pages, table[:1], lens[:1])
+    assert (one[:, -1:].float() - ref.float()).abs().max() < 2.0 ** -14
