@@ -78,7 +78,9 @@ const char* cl_last_error(void);
  * device: 0 = no device-side wait expired and no index error was recorded
  * since the last clear.  1 to 6: a wait of a GEMV ran out (5: a peer of a sharded
  * step never arrived); 7: an index of the cache's operators was out of range; 8:
- * the attention's wait for data ran out. */
+ * the attention's wait for data ran out.  One code is reported, the first of its
+ * kernel; where kernels of several operators recorded one, in the order GEMV,
+ * attention, prefix, cache, rotation.  Clearing drops all. */
 int cl_device_status(int clear, int* status_out);
 
 /* No counterpart in the reference (its kernels never wait on device-side
