@@ -446,12 +446,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prefix_kernel(const PrefixPara
                     for (int j = 0; j < 16; ++j) s[j] = __float_as_uint(__uint_as_float(s[j]) * unit);
                 }
                 if (live < 16 * c + 16 || missing != 0) {
-                    const bool none = (missing >> (8 * c) & 0xffu) != 0;
-#pragma unroll 1
-                    for (int j = none ? 0 : max(0, live - 16 * c); j < 16; ++j)
+                    const int from = (missing >> (8 * c) & 0xffu) != 0 ? 0 : live - 16 * c;
 #pragma unroll
-                        for (int x = 0; x < 16; ++x)
-                            if (x == j) s[x] = 0xff800000u;
+                    for (int j = 0; j < 16; ++j)
+                        if (j >= from) s[j] = 0xff800000u;
                 }
             };
             // base-2 logit of a column, less the reference
