@@ -763,12 +763,19 @@ int cut(int items, int tiles) {
 }  // namespace
 
 bool kv_prefix_takes(const KvAttentionArgs& a) {
-    // Measured with 8 heads of 128 (int8), both kernels with the launch that
-    // joins them, us at 128 / 512 / 2048 / 8192 tokens: 32 rows 15.0 15.7 19.6
-    // 26.4 here, 14.4 18.3 19.8 32.1 on the register-fed kernel; 256 rows 17.0
-    // 18.3 21.6 35.8 against 16.1 20.0 32.1 72.1.
+    // Both kernels with the launch that joins them, us, here / register-fed, at 16, 300,
+    // 1024 and 8192 tokens:
+    //                     8 rows a head                        9 rows
+    //   8 x 128 int8   9.5/9.1 10.2/12.1 10.2/12.4 18.4/17.7   9.6/12.0 10.2/15.3
+    //   2 x 64 int4    7.9/7.1  8.5/9.3   8.6/9.6  14.0/12.0   8.0/9.0   8.3/11.7
+    //                     32 (16, 300: 24) rows                 256 rows
+    //   8 x 128 int8  10.6/12.9 11.8/16.7 12.0/18.1 21.6/31.6  12.8/14.4 16.3/18.8 17.1/25.2 28.6/71.5
+    //   1 x 128 int8  10.2/12.1 11.1/15.4 11.4/16.6 18.4/23.7  12.3/13.0 13.5/16.8 13.5/17.6 20.3/31.3
+    //   2 x 64 int4    8.1/9.1   8.8/11.8  8.8/12.4 14.3/17.0   9.4/9.7  10.0/12.2 10.0/13.3 15.5/22.2
+    // From 9 rows on (two column tiles there) this one; 512 rows of 8 heads lose 3 to 8 %
+    // below 256 tokens, and up to 8 rows gain between 256 and some 2000 only.
     const int64_t rows = (int64_t)a.new_tokens * a.group;
-    return a.head_dim <= 128 && rows >= 32 && rows < (1 << 24) && a.fixed_length >= 512;
+    return a.head_dim <= 128 && rows > 8 && rows < (1 << 24);
 }
 
 int kv_prefix_parts(const KvAttentionArgs& a) {

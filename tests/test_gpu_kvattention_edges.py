@@ -246,3 +246,15 @@ def test_line_of_more_than_2_to_31_tokens():
     assert (out.float() - one.float()).abs().max() < 2.0 ** -14
     ref = att.forward(q[:, -1:], pages, table[:1], lens[:1])
     assert (one[:, -1:].float() - ref.float()).abs().max() < 2.0 ** -14
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=str)
+@pytest.mark.parametrize("D,bits", [(64, 8), (64, 4), (128, 8), (128, 4)])
+@pytest.mark.parametrize("rows", [8, 9, 17])
+@pytest.mark.parametrize("prefix", [1, 15, 63, 64, 65, 127, 128, 129, 257, 511])
+def test_short_prefixes_of_few_rows(prefix, rows, D, bits, dtype):
+    """Around the rule's 9 rows a head, and tiles that end in either half."""
+    p = Cache([prefix], 2, D, bits, 32, seed=prefix)
+    q = _q(rows, 1, 2, D, dtype, seed=prefix + rows)
+    out, lse, c = _over_prefix(p, q, D ** -0.5, 1, bits)
+    _check(out, lse, q, c, D ** -0.5, prefix=p)
