@@ -69,6 +69,7 @@ class AttentionLayer:
                                        dtype=torch.int32).view(batch, width)
         self.prefix_pages = torch.arange(batch * width, batch * width + shared, device="cuda",
                                          dtype=torch.int32)
+        self._number_slots()
         self.lengths = torch.zeros(batch, dtype=torch.int32, device="cuda")
         self.workspace = self.attention.workspace("cuda")
 
@@ -89,13 +90,17 @@ class AttentionLayer:
         if sequence is not None:
             self.lengths[sequence] += k.size(0)
 
+    def _number_slots(self) -> None:
+        """The slot of every token of a sequence, and -1 (skipped by the cache) behind them."""
+        first = self.page_table.long() * self.page_size
+        of_tokens = first[..., None] + torch.arange(self.page_size, device=first.device)
+        self.slot_table = torch.nn.functional.pad(of_tokens.flatten(1), (0, 1), value=-1)
+
     def slots(self) -> torch.Tensor:
-        """int64 [batch]: where each sequence's next token goes, -1 (skipped by the cache) for
-        one whose pages are full."""
-        at = self.lengths.long()
-        index = (at // self.page_size).clamp(max=self.page_table.size(1) - 1)
-        page = self.page_table.gather(1, index[:, None])[:, 0].long()
-        return torch.where(at < self.capacity, page * self.page_size + at % self.page_size, -1)
+        """int64 [batch]: where each sequence's next token goes, -1 for one whose pages are
+        full."""
+        at = self.lengths.clamp(max=self.capacity).long()
+        return self.slot_table.gather(1, at[:, None])[:, 0]
 
     def step(self, x: torch.Tensor) -> torch.Tensor:
         """x fp16 [batch, hidden] of each sequence's next token -> the layer's output.  A

@@ -24,6 +24,7 @@ def _layer(lengths, width=2, page=16, prefix=0):
     layer.lengths = torch.tensor(lengths, dtype=torch.int32)
     layer.pages = torch.zeros(1, dtype=torch.uint8)
     layer.cache = _Written()
+    layer._number_slots()
     return layer
 
 
