@@ -39,13 +39,18 @@
 // partials in order (groups of kFan, then the groups), so the sum order, and
 // with it every bit of the result, does not depend on timing.
 //
-// Measured (8 heads of 128): 64 sequences of 4096 to 8192 tokens, 64 query
-// heads, int4 97 us = 4.3 TB/s, 0.65 of a copy; 16 ragged sequences to 4096,
-// int8 21 us, of which the bytes are 10.5; one sequence of 77 tokens 4.8 us.  The
-// long case is held by the logic instructions that expand the fields, which
-// come in bursts to one pipe: its copies alone take 70 us, all but V's
-// expansion 89, while HADD2, MMAs and shared-memory reads cost nothing beside
-// them.  The short ones are launch, plan, first bytes and join in a row.
+// Measured (8 heads of 128, a replayed graph; two boxes within 1 %): 64 sequences
+// with 64 query heads, int8 of 2048 to 4096 tokens 70 us = 5.9 TB/s, 0.90 of a
+// copy; int4 of 4096 to 8192 tokens 96 us = 4.35 TB/s, 0.66; 16 ragged sequences
+// to 4096, int8 20.7 us, of which the bytes are 10.5; one sequence of 77 tokens 4.5.
+// int8 is its copies (alone 67 us).  int4 has twice the elements a byte at three
+// warps a scheduler: copies alone 69, without the sum over V 72, without the
+// expansion of V's fields 88, of K's 90, of both 81, so what remains is the
+// length of a step's chain, reads, expansion, products and softmax one after the
+// other, which three warps do not cover (0.58 instructions a cycle and scheduler,
+// no pipe above 51 %).  With 16 rows a head (two column tiles, two CTAs an SM)
+// the same holds for both: 49 us for 31.6 (int8), 77 for 32 (int4).  The short ones
+// are launch, plan, first bytes and join in a row.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -71,7 +76,7 @@ constexpr int kFan = 16;         // partial results added by one CTA at a time
 // What a CTA pays for a segment besides its units (loading q, joining its
 // warps' results, latencies), in units: about 4000 cycles against 400 to 700 a
 // unit.  Without it the CTA that gets the shortest sequences of a ragged batch
-// ends last (64 sequences of 1 to 1024 tokens: 91 us, with it 37).
+// ends last (64 sequences of 1 to 1024 tokens: 52 us, with it 25).
 constexpr int kSegmentCost = 8;
 // A row's weights are fp16: with its reference kLift below the largest logit the
 // largest weight is 2^7, one far smaller keeps 7 bits more than under a largest

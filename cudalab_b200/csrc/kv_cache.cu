@@ -14,10 +14,11 @@
 // per element, the read the reverse.  head_dim / 16 lanes share a row; a lane
 // holds 8 elements in each half of it, so that the lanes touch the 16-bit
 // elements in whole lines (with 16 neighbours a lane every access was one of
-// half sectors: 37 us for the 33 to 35 below), and takes K and V, so that four
-// loads are in flight.  8 heads of 128: reading 32768 tokens, int8, 33 to 35 us,
-// 6 TB/s, 0.9 of a copy; writing 8192 tokens as int4 and reading them back 17 us, 4.9
-// TB/s, for two kernels of 6.5 us' bytes each and their ramps.  (The write's
+// half sectors: 37 us for the 33 below), and takes K and V, so that four
+// loads are in flight.  8 heads of 128: reading 32768 tokens, int8, 33.3 us (33.5 to
+// 34.1 in a loop of calls), 6.1 TB/s, 0.93 of a copy; writing 8192 tokens as int4
+// and reading them back 17.2 us (18.4), 4.9 TB/s, for two kernels of 6.5 us' bytes
+// each and their ramps.  (The write's
 // instructions show as well: 16 for each element took 21 us where 13 took 20.)
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

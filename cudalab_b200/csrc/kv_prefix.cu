@@ -34,10 +34,10 @@
 // sequences' own tokens.  Every wait is bounded (status 8 on expiry).
 //
 // Measured (8 heads of 128, int8): 16384 tokens for 512 rows a head with the
-// launch over 64 sequences' own tokens 89 us, 0.40 PFLOP/s; a tile takes a CTA
+// launch over 64 sequences' own tokens 90 us, 0.39 PFLOP/s; a tile takes a CTA
 // 1.6 us, of which its MMAs need 0.74 at the measured peak.  The rest is
-// instructions: 7200 of a warp per tile (softmax and expansion about halves),
-// 0.56 a cycle and scheduler.
+// instructions: 7700 of a warp per tile (softmax and expansion about halves),
+// 0.55 a cycle and scheduler.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
